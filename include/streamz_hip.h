@@ -284,6 +284,107 @@ int szh_net_get_gemm(const szh_net *net);
 int szh_net_vote_dev(szh_net *net, const float *feats_dev, uint64_t n, float threshold,
                      unsigned long long *counts_dev, void *stream);
 
+/* Between the sum over ranks and szh_net_apply_grad_dev: scales the gradient vector in place so that the norm of the
+ * mean gradient, norm = sqrt(sum of the squares of all param_count entries) / live_rows, is at most max_norm:
+ * every entry is multiplied by max_norm / norm where norm > max_norm and left as it is otherwise (a NaN norm included).
+ * Squares are added in f64 in a fixed order.  The two tail floats stay.  norm_dev (optional): one float, the norm
+ * before the scaling; 0 when live_rows is 0.  max_norm must be >= 0.  The first call on a net, and the first after
+ * szh_net_add_output_class, allocates and cannot be captured into a graph.  No counterpart in the reference. */
+int szh_net_clip_grad_dev(szh_net *net, float max_norm, float *norm_dev, void *stream);
+
+/* ---- gradient norms over many tensors ------------------------------------------------------ */
+/* The same for any list of f32 tensors in device memory, in groups that are scaled together: the tensors of several
+ * nets under one norm (one group), or of many small models with a norm each.  Tensor t is in[t][0 .. lengths[t]),
+ * its scaled values go to out[t] (out == NULL, or out[t] == in[t]: in place; otherwise the two must not overlap).
+ * group[t] < groups (group == NULL: all in group 0).  live_dev (optional): groups floats that the norms are divided by,
+ * read when the call runs; a group whose value is not > 0 has norm 0.  The handle keeps the addresses: the tensors must
+ * outlive it.  norms_dev (optional) receives `groups` floats.  Addresses are multiples of 4 bytes.
+ * Calls on one handle share its workspace: they must not overlap (two streams, two graphs in flight). */
+typedef struct szh_clip szh_clip;
+int szh_clip_create(const float *const *in, float *const *out, const uint64_t *lengths, const uint32_t *group, uint32_t n_tensors,
+                    uint32_t groups, const float *live_dev, szh_clip **clip);
+void szh_clip_destroy(szh_clip *clip);
+int szh_clip_run_dev(szh_clip *clip, float max_norm, float *norms_dev, void *stream);
+
+/* ---- controls on logits --------------------------------------------------------------------- */
+/* Per-request priors, candidate lists and penalties on a row's logits l[classes] before the softmax of lib.rs:887-890.
+ * All members are device arrays; NULL members are not used.  Row r takes set k = set_of_row[r] (set_of_row NULL: 0);
+ * outside 0 .. sets - 1 the row has no control.  With n = counts[k][c], how often class c was answered already:
+ *   z = l;   n > 0:  z = (z > 0 ? z / repetition[k] : z * repetition[k]) - presence[k]
+ *   z = z - frequency[k] * n + bias[k][c];   z = -inf where class c is not allowed
+ *   p = exp(z - max z) / sum of exp(z - max z); a class that is not allowed, whatever its logit, has p = 0, and a row
+ *   without any class left (every z = -inf) has p = 0 throughout.
+ * allow: bit c % 32 of word c / 32 set = class c is a candidate.  Penalties need counts; below zero (or a repetition
+ * below one) they favour who has spoken already.  No counterpart in the reference. */
+typedef struct szh_logit_controls {
+    const float *bias;          /* [sets][classes] */
+    const uint32_t *allow;      /* [sets][(classes + 31) / 32] */
+    const uint32_t *counts;     /* [sets][classes] */
+    const float *repetition;    /* [sets] */
+    const float *presence;      /* [sets] */
+    const float *frequency;     /* [sets] */
+    uint32_t sets;
+    const int32_t *set_of_row;  /* [rows] */
+} szh_logit_controls;
+#define SZH_CONTROL_LOGITS 0 /* out = z */
+#define SZH_CONTROL_PROBS 1  /* out = p */
+/* logits_dev[rows][ld_logits], out_dev[rows][ld_out] (strides in floats, >= classes); out_dev may be logits_dev itself with the
+ * same stride, any other overlap is refused.  Columns from `classes` on are not touched. */
+int szh_logits_control_dev(const float *logits_dev, uint64_t ld_logits, uint64_t rows, uint32_t classes,
+                           const szh_logit_controls *controls, int what, float *out_dev, uint64_t ld_out, void *stream);
+
+/* ---- low-rank adapters of many requests ------------------------------------------------------ */
+/* One net serving many requests (recordings, microphones, customers), each with a small adapter of its own beside the
+ * net's second hidden layer and its output layer.  A bank holds `slots` adapters of rank `rank` (1 .. SZH_ADAPTER_MAX_RANK)
+ * for nets of the shape of `net`; slot s is [a2[hidden1][rank] | b2[rank][hidden2] | a3[hidden2][rank] | b3[rank][output]], row-major:
+ *   h1 = relu(x w1 + b1)            h2 = tanh(h1 w2 + b2 + scale (h1 a2[s]) b2[s])
+ *   logits = h2 w3 + b3 + scale (h2 a3[s]) b3[s]
+ * A row of a call names its slot in slots_dev; any value outside 0 .. slots - 1 (say -1) means the net alone.  Rows
+ * are independent: what a row gets does not depend on what the other rows and their adapters hold, NaN included.
+ * The arithmetic mode of the net (szh_net_set_gemm) applies to the hidden-layer product.  No counterpart in the reference.
+ *
+ * init: NULL -> a2, a3 ~ U(-0.5, 0.5) / sqrt(inputs) from `seed`, b2 = b3 = 0 (a new adapter changes nothing); else
+ * [slots][szh_adapters_param_count] floats.
+ * The *_dev calls on one bank share its workspace and must be serialised by the caller (two streams, two captured graphs
+ * in flight race); banks may be used beside one another on one net.  The workspace grows to the largest call so far;
+ * szh_adapters_reserve sizes it (and the tables of szh_adapters_clip_grad_dev) ahead, which a caller that captures calls into a
+ * graph does first.  Calls of more than 131072 rows are walked in pieces of that size. */
+#define SZH_ADAPTER_MAX_RANK 64
+#define SZH_ADAPTER_MAX_SLOTS 8192
+typedef struct szh_adapters szh_adapters;
+int szh_adapters_create(const szh_net *net, uint32_t slots, uint32_t rank, float scale, const float *init, uint64_t seed,
+                        szh_adapters **bank);
+void szh_adapters_destroy(szh_adapters *bank);
+uint64_t szh_adapters_param_count(const szh_adapters *bank); /* of one slot */
+int szh_adapters_get_params(szh_adapters *bank, uint32_t slot, float *flat);
+int szh_adapters_set_params(szh_adapters *bank, uint32_t slot, const float *flat);
+int szh_adapters_reserve(szh_adapters *bank, uint64_t rows, int training);
+/* logits_dev[n][output] (before any control) and probs_dev[n][output]; either may be NULL.  controls may be NULL. */
+int szh_net_forward_adapted_dev(szh_net *net, szh_adapters *bank, const float *feats_dev, const int32_t *slots_dev, uint64_t n,
+                                const szh_logit_controls *controls, float *logits_dev, float *probs_dev, void *stream);
+/* Votes of identify_speaker_list (lib.rs:1391-1402) for many requests at once: a row's top class (the last maximum wins)
+ * is counted in counts_dev[group_of_row[row]][output] if its probability is >= threshold; a row without a
+ * candidate, and one whose group is outside 0 .. groups - 1, votes for nobody.  group_of_row NULL: group 0. */
+int szh_net_vote_adapted_dev(szh_net *net, szh_adapters *bank, const float *feats_dev, const int32_t *slots_dev, uint64_t n,
+                             const szh_logit_controls *controls, float threshold, const int32_t *group_of_row_dev, uint32_t groups,
+                             unsigned long long *counts_dev, void *stream);
+/* Training of a bank, the net frozen: zero_grad, accumulate over any number of blocks, (all-reduce,) clip, apply.
+ * The gradient vector is [slots][param_count] floats, then [slots]{loss sum, live rows}.  A row counts (is live) if it has a slot,
+ * a label in 0 .. output - 1 that its candidate list allows, and an input that is not zero after dropout
+ * (lib.rs:607-609); the loss is -ln(max(p[label], 1e-12)), its gradient p - t (lib.rs:611-615, 1028).  controls may hold
+ * a bias and a candidate list; penalties are refused.  Dropout draws are those of szh_net_accumulate_dev.
+ * Gradients are bit-identical on every call with the same arguments. */
+uint64_t szh_adapters_grad_len(const szh_adapters *bank);
+float *szh_adapters_grad_dev(szh_adapters *bank);
+int szh_adapters_zero_grad_dev(szh_adapters *bank, void *stream);
+int szh_adapters_accumulate_dev(szh_net *net, szh_adapters *bank, const float *feats_dev, const int32_t *labels_dev,
+                                const int32_t *slots_dev, uint64_t n, const szh_logit_controls *controls, float dropout, uint64_t seed,
+                                void *stream);
+/* szh_net_clip_grad_dev for every slot by itself; norms_dev (optional): one float per slot. */
+int szh_adapters_clip_grad_dev(szh_adapters *bank, float max_norm, float *norms_dev, void *stream);
+/* params[s] -= (lr / live_rows[s]) * grad[s]; slots without live rows stay as they are. */
+int szh_adapters_apply_grad_dev(szh_adapters *bank, float lr, void *stream);
+
 /* ---- the collective of a sharded epoch (RCCL over xGMI) --------------------------------- */
 /* No counterpart in the reference, which trains in one process (lib.rs:632-665, the loop the
  * shards split).  One process per GPU: each calls szh_init(local rank), builds the same net,
@@ -375,7 +476,8 @@ int szh_wav_info(const char *path, uint64_t *n_frames, uint32_t *sample_rate, ui
  * synchronises the device, writes one line "tag launches total_ms" per kernel tag seen since
  * the previous report into buf (NUL-terminated, truncated to capacity) and returns the full
  * text length.  Tags: mfcc_base, finish, prep, fwd1, fwd2, fwd3, softmax, delta2, delta1,
- * dw3, dw2, dw1, bias, reduce, apply, vote. */
+ * dw3, dw2, dw1, bias, reduce, apply, vote, clip, control, control_loss, adapt_group, adapt_low, adapt_grad,
+ * adapt_h1, adapt_h2, adapt_out, adapt_d2. */
 int szh_profile_enable(int on);
 int64_t szh_profile_report(char *buf, uint64_t capacity);
 

@@ -8,14 +8,14 @@ checked), but every compute call raises StreamzError when no HIP device is usabl
 loading raises if the library has not been built.
 """
 from . import _capi
-from ._capi import (Comm, comm_unique_id, extract_embedding, extract_embedding_from_features, median_embedding_from_features,
+from ._capi import (Adapters, Comm, GradClip, LogitControls, comm_unique_id, control_logits_dev, extract_embedding, extract_embedding_from_features, median_embedding_from_features,
                     FEATURE_SIZE, FeatureExtractor, augment, pretrain_network, Plan, SimpleNeuralNet, StreamzError, exported_symbols,
                     identify_from_features, identify_speaker, identify_speaker_with_threshold,
                     identify_speaker_with_threshold_feats, identify_speaker_list, identify_speaker_list_dev,
                     lib, library_path, load_cached_features, pretrain_from_features, profile_enable,
                     profile_report, shard_ranges, train_from_feature_map, wav_info, wav_read, window_count)
 
-__all__ = ["Comm", "comm_unique_id", "extract_embedding", "extract_embedding_from_features", "median_embedding_from_features", "FEATURE_SIZE", "FeatureExtractor", "augment", "pretrain_network", "Plan", "SimpleNeuralNet", "StreamzError", "exported_symbols",
+__all__ = ["Adapters", "Comm", "GradClip", "LogitControls", "comm_unique_id", "control_logits_dev", "extract_embedding", "extract_embedding_from_features", "median_embedding_from_features", "FEATURE_SIZE", "FeatureExtractor", "augment", "pretrain_network", "Plan", "SimpleNeuralNet", "StreamzError", "exported_symbols",
            "identify_from_features", "identify_speaker", "identify_speaker_with_threshold",
            "identify_speaker_with_threshold_feats", "identify_speaker_list", "identify_speaker_list_dev",
            "lib", "library_path", "load_cached_features", "pretrain_from_features", "profile_enable",

@@ -90,6 +90,31 @@ _SIGS = {
     "szh_net_apply_grad_dev": (C.c_int, [C.c_void_p, C.c_float, C.c_void_p]),
     "szh_net_forward_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p]),
     "szh_net_vote_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_float, C.c_void_p, C.c_void_p]),
+    "szh_net_clip_grad_dev": (C.c_int, [C.c_void_p, C.c_float, C.c_void_p, C.c_void_p]),
+    "szh_clip_create": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p,
+                                  C.POINTER(C.c_void_p)]),
+    "szh_clip_destroy": (None, [C.c_void_p]),
+    "szh_clip_run_dev": (C.c_int, [C.c_void_p, C.c_float, C.c_void_p, C.c_void_p]),
+    "szh_logits_control_dev": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32, C.c_void_p, C.c_int, C.c_void_p,
+                                         C.c_uint64, C.c_void_p]),
+    "szh_adapters_create": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_float, C.c_void_p, C.c_uint64,
+                                      C.POINTER(C.c_void_p)]),
+    "szh_adapters_destroy": (None, [C.c_void_p]),
+    "szh_adapters_param_count": (C.c_uint64, [C.c_void_p]),
+    "szh_adapters_get_params": (C.c_int, [C.c_void_p, C.c_uint32, C.c_void_p]),
+    "szh_adapters_set_params": (C.c_int, [C.c_void_p, C.c_uint32, C.c_void_p]),
+    "szh_adapters_reserve": (C.c_int, [C.c_void_p, C.c_uint64, C.c_int]),
+    "szh_net_forward_adapted_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p,
+                                              C.c_void_p, C.c_void_p, C.c_void_p]),
+    "szh_net_vote_adapted_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_float,
+                                           C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p]),
+    "szh_adapters_grad_len": (C.c_uint64, [C.c_void_p]),
+    "szh_adapters_grad_dev": (C.c_void_p, [C.c_void_p]),
+    "szh_adapters_zero_grad_dev": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "szh_adapters_accumulate_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p,
+                                              C.c_float, C.c_uint64, C.c_void_p]),
+    "szh_adapters_clip_grad_dev": (C.c_int, [C.c_void_p, C.c_float, C.c_void_p, C.c_void_p]),
+    "szh_adapters_apply_grad_dev": (C.c_int, [C.c_void_p, C.c_float, C.c_void_p]),
     "szh_comm_unique_id": (C.c_int, [C.c_void_p]),
     "szh_comm_create": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_void_p)]),
     "szh_comm_destroy": (None, [C.c_void_p]),
@@ -382,6 +407,21 @@ class SimpleNeuralNet:
     def apply_grad_dev(self, lr, stream=0):
         _check(lib().szh_net_apply_grad_dev(self._h, lr, C.c_void_p(stream)))
 
+    def clip_grad_dev(self, max_norm, norm_ptr=0, stream=0):
+        """Between the sum over ranks and apply_grad_dev: norm of the mean gradient at most max_norm (szh_net_clip_grad_dev)."""
+        _check(lib().szh_net_clip_grad_dev(self._h, max_norm, norm_ptr or None, stream or None))
+
+    def forward_adapted_dev(self, bank, feats_ptr, slots_ptr, n, probs_ptr=0, logits_ptr=0, controls=None, stream=0):
+        """Forward pass with an adapter per row (szh_net_forward_adapted_dev)."""
+        _check(lib().szh_net_forward_adapted_dev(self._h, bank._h, feats_ptr or None, slots_ptr or None, n, _controls(controls),
+                                                 logits_ptr or None, probs_ptr or None, stream or None))
+
+    def vote_adapted_dev(self, bank, feats_ptr, slots_ptr, n, threshold, counts_ptr, groups=1, group_of_row_ptr=0, controls=None,
+                         stream=0):
+        """identify_speaker_list's votes for many requests at once (szh_net_vote_adapted_dev)."""
+        _check(lib().szh_net_vote_adapted_dev(self._h, bank._h, feats_ptr or None, slots_ptr or None, n, _controls(controls),
+                                              threshold, group_of_row_ptr or None, groups, counts_ptr or None, stream or None))
+
     def forward_dev(self, feats_ptr, n, probs_ptr, stream=0):
         _check(lib().szh_net_forward_dev(self._h, C.c_void_p(feats_ptr), n, C.c_void_p(probs_ptr), C.c_void_p(stream)))
 
@@ -431,6 +471,119 @@ class SimpleNeuralNet:
         h = C.c_void_p()
         _check(lib().szh_net_load(os.fsencode(path), C.byref(h)))
         return SimpleNeuralNet(_handle=h)
+
+
+class LogitControls(C.Structure):
+    """Priors, candidate lists and penalties on logits (szh_logit_controls): device addresses of the arrays, 0 = not used.
+    The arrays must live as long as calls that use them run."""
+    _fields_ = [("bias", C.c_void_p), ("allow", C.c_void_p), ("counts", C.c_void_p), ("repetition", C.c_void_p),
+                ("presence", C.c_void_p), ("frequency", C.c_void_p), ("sets", C.c_uint32), ("set_of_row", C.c_void_p)]
+
+    def __init__(self, sets=1, bias=0, allow=0, counts=0, repetition=0, presence=0, frequency=0, set_of_row=0):
+        super().__init__(bias or None, allow or None, counts or None, repetition or None, presence or None, frequency or None,
+                         sets, set_of_row or None)
+
+
+def _controls(c):
+    return C.byref(c) if c is not None else None
+
+
+def control_logits_dev(logits_ptr, rows, classes, controls, out_ptr, probs=True, ld_logits=0, ld_out=0, stream=0):
+    """Controlled logits or their softmax (szh_logits_control_dev); row strides default to the number of classes."""
+    _check(lib().szh_logits_control_dev(logits_ptr or None, ld_logits or classes, rows, classes, _controls(controls), 1 if probs else 0,
+                                        out_ptr or None, ld_out or classes, stream or None))
+
+
+class GradClip:
+    """The norm of many f32 device tensors and their clipping (szh_clip_*).  tensors: (address, length) pairs; outputs:
+    addresses of the results (default: in place); groups: each tensor's group (default: one for all); live: address of one
+    float per group that its norm is divided by."""
+
+    def __init__(self, tensors, outputs=None, groups=None, live=0):
+        n = len(tensors)
+        ptrs = (C.c_void_p * n)(*[p for p, _ in tensors])
+        outs = (C.c_void_p * n)(*outputs) if outputs is not None else None
+        ln = np.array([k for _, k in tensors], np.uint64)
+        gr = np.ascontiguousarray(groups, np.uint32) if groups is not None else None
+        if (outputs is not None and len(outputs) != n) or (gr is not None and gr.size != n):
+            raise ValueError("one output and one group per tensor")
+        self.groups = int(gr.max()) + 1 if gr is not None and n else 1
+        h = C.c_void_p()
+        _check(lib().szh_clip_create(ptrs, outs, _p(ln), _p(gr), n, self.groups, live or None, C.byref(h)))
+        self._h = h
+
+    def __del__(self):
+        if getattr(self, "_h", None):
+            lib().szh_clip_destroy(self._h)
+            self._h = None
+
+    def run(self, max_norm, norms_ptr=0, stream=0):
+        _check(lib().szh_clip_run_dev(self._h, max_norm, norms_ptr or None, stream or None))
+
+
+class Adapters:
+    """A bank of low-rank adapters for nets of one shape (szh_adapters_*).  init: None, or [slots][param_count] floats."""
+
+    def __init__(self, net, slots, rank, scale=1.0, init=None, seed=0):
+        h = C.c_void_p()
+        flat = None
+        if init is not None:
+            i, h1, h2, o = net.dims()
+            flat = np.ascontiguousarray(init, np.float32)
+            if flat.size != slots * rank * (h1 + 2 * h2 + o):
+                raise ValueError("init holds [slots][param_count] floats")
+        _check(lib().szh_adapters_create(net._h, slots, rank, scale, _p(flat), seed, C.byref(h)))
+        self._h = h
+        self.slots, self.rank, self.scale = slots, rank, scale
+        self._dims = net.dims()
+
+    def __del__(self):
+        if getattr(self, "_h", None):
+            lib().szh_adapters_destroy(self._h)
+            self._h = None
+
+    def param_count(self):
+        return int(lib().szh_adapters_param_count(self._h))
+
+    def shapes(self):
+        _, h1, h2, o = self._dims
+        return [(h1, self.rank), (self.rank, h2), (h2, self.rank), (self.rank, o)]
+
+    def get_params(self, slot):
+        flat, out, pos = np.zeros(self.param_count(), np.float32), [], 0
+        _check(lib().szh_adapters_get_params(self._h, slot, _p(flat)))
+        for s in self.shapes():
+            out.append(flat[pos:pos + s[0] * s[1]].reshape(s).copy())
+            pos += s[0] * s[1]
+        return out
+
+    def set_params(self, slot, params):
+        flat = np.concatenate([np.asarray(a, np.float32).ravel() for a in params])
+        if flat.size != self.param_count():
+            raise ValueError("an adapter's parameters have the sizes of shapes()")
+        _check(lib().szh_adapters_set_params(self._h, slot, _p(flat)))
+
+    def reserve(self, rows, training=False):
+        _check(lib().szh_adapters_reserve(self._h, rows, 1 if training else 0))
+
+    def grad_len(self):
+        return int(lib().szh_adapters_grad_len(self._h))
+
+    def grad_ptr(self):
+        return int(lib().szh_adapters_grad_dev(self._h))
+
+    def zero_grad_dev(self, stream=0):
+        _check(lib().szh_adapters_zero_grad_dev(self._h, stream or None))
+
+    def accumulate_dev(self, net, feats_ptr, labels_ptr, slots_ptr, n, controls=None, dropout=0.0, seed=0, stream=0):
+        _check(lib().szh_adapters_accumulate_dev(net._h, self._h, feats_ptr or None, labels_ptr or None, slots_ptr or None, n,
+                                                 _controls(controls), dropout, seed, stream or None))
+
+    def clip_grad_dev(self, max_norm, norms_ptr=0, stream=0):
+        _check(lib().szh_adapters_clip_grad_dev(self._h, max_norm, norms_ptr or None, stream or None))
+
+    def apply_grad_dev(self, lr, stream=0):
+        _check(lib().szh_adapters_apply_grad_dev(self._h, lr, stream or None))
 
 
 class _Rng(C.Structure):

@@ -1,0 +1,426 @@
+// Low-rank adapters of many requests beside the shared projections of one network: the forward pass with an
+// adapter per row, the gradients of the adapters and their update.  No counterpart in the reference, which has
+// one network for everyone; what is shared is its forward and training pass (lib.rs:880-891, 1013-1059).
+//
+//   h1 = relu(x W1 + b1)                         shared by all rows
+//   h2 = tanh(h1 W2 + b2 + u2 B2[s]),  u2 = scale h1 A2[s]
+//   l  = h2 W3 + b3 + u3 B3[s],        u3 = scale h2 A3[s]          s = the row's slot
+//
+//   d3 = p - t            dB3[s] = sum u3^T d3    g3 = scale d3 B3[s]^T    dA3[s] = sum h2^T g3
+//   d2 = (d3 W3^T + g3 A3[s]^T)(1 - h2^2)
+//                         dB2[s] = sum u2^T d2    g2 = scale d2 B2[s]^T    dA2[s] = sum h1^T g2
+//
+// The network itself is frozen: no gradient passes below the first adapted projection.
+//
+// A call's rows are brought into the order of their slots first (a stable counting sort), so that the tiles of
+// every product hold rows of one slot, nearly always, and a slot's rows are one range of every row sum.
+// Rows are independent of one another in every product: what a row gets does not depend on who else is in the call.
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <type_traits>
+#include <vector>
+
+#include "adapt_kernel.h"
+#include "gemm_launch.h"
+#include "internal.h"
+#include "prof.h"
+#include "streamz_hip.h"
+
+namespace sz {
+
+namespace {
+
+using namespace adapt;
+
+// Rows per pass: a call with more is walked in pieces, whose workspace does not grow with it.
+constexpr uint64_t kAdaptRows = 131072;
+
+inline int round_up(int v, int to) { return (v + to - 1) / to * to; }
+
+bool capturing(hipStream_t s)
+{
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing(s, &st) == hipSuccess && st == hipStreamCaptureStatusActive;
+}
+
+// How the arrays of a pass lie in the workspace; `base` null: only the size.
+size_t lay_out(const Adapters* a, uint64_t rows, bool training, char* base, AdaptWorkspace* w)
+{
+    size_t at = 0;
+    auto take = [&](auto*& p, uint64_t count) {
+        p = reinterpret_cast<std::decay_t<decltype(p)>>(base + at);
+        at += (count * sizeof(*p) + 255) / 256 * 256;
+    };
+    AdaptWorkspace t;
+    AdaptWorkspace& o = w ? *w : t;
+    const uint64_t blocks = (rows + kGroupRows - 1) / kGroupRows, S = a->slots;
+    o.ldx = a->in + 1 <= 64 ? 64 : round_up((int)a->in + 1, 128);
+    o.ld1 = round_up((int)a->h1, 4); o.ld2 = round_up((int)a->h2, 4); o.ld3 = round_up((int)std::max(a->out, 1u), 4);
+    o.ldu = round_up((int)a->rank, 8);
+    take(o.order, rows); take(o.row_slot, rows); take(o.begin, S + 2); take(o.count, (S + 1) * blocks); take(o.total, S + 1);
+    take(o.xs, rows * o.ldx); take(o.live0, rows); take(o.live, rows);
+    take(o.h1, (rows + 32) * o.ld1); take(o.h2, (rows + 32) * o.ld2); take(o.lg, (rows + 32) * o.ld3);
+    take(o.u2, rows * o.ldu); take(o.u3, rows * o.ldu);
+    take(o.w1t, (uint64_t)a->h1 * o.ldx); take(o.w2t, (uint64_t)a->h1 * a->h2); take(o.w3t, (uint64_t)a->h2 * a->out + 1);
+    take(o.w2s, 3 * ((uint64_t)a->h1 * a->h2 + 1) / 2 + 4);
+    if (training) {
+        const uint64_t chunks = (rows + kFactorRows - 1) / kFactorRows;
+        take(o.d2, (rows + 32) * o.ld2); take(o.g2, rows * o.ldu); take(o.g3, rows * o.ldu); take(o.loss, rows);
+        take(o.slab, (chunks + S) * std::max({a->h1, a->h2, a->out}) * a->rank);
+    }
+    return at;
+}
+
+int ensure(Adapters* a, uint64_t rows, bool training, hipStream_t s)
+{
+    rows = std::min<uint64_t>(std::max<uint64_t>(rows, 256), kAdaptRows);
+    if (a->ws_rows >= rows && (a->ws_training || !training)) return SZH_OK;
+    if (capturing(s)) { set_error("adapters: the workspace must be reserved before a stream is captured (szh_adapters_reserve)"); return SZH_EINVAL; }
+    rows = std::max<uint64_t>(rows, a->ws_rows);
+    rows = (rows + 255) / 256 * 256;
+    training = training || a->ws_training;
+    char* p = nullptr;
+    SZ_HIP(hipMalloc((void**)&p, lay_out(a, rows, training, nullptr, nullptr)));
+    try { a->arenas.push_back(p); } catch (...) { (void)hipFree(p); throw; }
+    // the old workspace stays until the handle goes: a captured graph may still work in it
+    lay_out(a, rows, training, p, &a->ws);
+    a->ws_rows = rows;
+    a->ws_training = training;
+    return SZH_OK;
+}
+
+int check_pair(const Net* n, const Adapters* a)
+{
+    if (n->in != a->in || n->h1 != a->h1 || n->h2 != a->h2 || n->out != a->out) {
+        set_error("adapters were made for a network %u-%u-%u-%u, this one is %u-%u-%u-%u", a->in, a->h1, a->h2, a->out, n->in, n->h1,
+                  n->h2, n->out);
+        return SZH_EINVAL;
+    }
+    if (n->device != a->device) { set_error("adapters and network are on different devices"); return SZH_EINVAL; }
+    return SZH_OK;
+}
+
+int group_rows(Adapters* a, const int32_t* slots_dev, uint32_t rows, hipStream_t s)
+{
+    AdaptWorkspace& w = a->ws;
+    const int S = (int)a->slots, blocks = (int)((rows + kGroupRows - 1) / kGroupRows);
+    const size_t lds = (S + 1) * sizeof(uint32_t);
+    ProfScope prof("adapt_group", s);
+    hipLaunchKernelGGL(group_count_kernel, dim3(blocks), dim3(64), lds, s, slots_dev, rows, S, blocks, w.count);
+    hipLaunchKernelGGL(group_scan_kernel, dim3(S + 1), dim3(64), 0, s, w.count, blocks, w.total);
+    hipLaunchKernelGGL(group_begin_kernel, dim3(1), dim3(64), 0, s, w.total, S, rows, w.begin);
+    hipLaunchKernelGGL(group_place_kernel, dim3(blocks), dim3(64), lds, s, slots_dev, rows, S, blocks, w.count, w.begin, w.order, w.row_slot);
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
+}
+
+// u = scale * x F[slot]
+int low_product(const Adapters* a, const float* x, int ldx, int K, const float* factor, int f_k, int f_j, uint32_t rows, float* u,
+                hipStream_t s)
+{
+    LowArgs g{};
+    g.x = x; g.ldx = ldx; g.K = K; g.factor = factor; g.factor_slot = a->per_slot(); g.f_k = f_k; g.f_j = f_j;
+    g.rank = (int)a->rank; g.row_slot = a->ws.row_slot; g.rows = rows; g.u = u; g.ldu = a->ws.ldu; g.scale = a->scale;
+    const dim3 grid((rows + 31) / 32), block(256);
+    ProfScope prof("adapt_low", s);
+    switch ((a->rank + 15) / 16) {
+    case 1: hipLaunchKernelGGL((low_kernel<1>), grid, block, 0, s, g); break;
+    case 2: hipLaunchKernelGGL((low_kernel<2>), grid, block, 0, s, g); break;
+    case 3: hipLaunchKernelGGL((low_kernel<3>), grid, block, 0, s, g); break;
+    default: hipLaunchKernelGGL((low_kernel<4>), grid, block, 0, s, g); break;
+    }
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
+}
+
+// grad[slot] at `off` += sum over the slot's rows of p[i][m] w[i][j], element (m, j) at m * g_m + j * g_j
+int factor_gradient(Adapters* a, const float* p, int ldp, int M, const float* w, uint32_t rows, uint64_t off, int g_m, int g_j, hipStream_t s)
+{
+    FactorArgs g{};
+    g.p = p; g.ldp = ldp; g.M = M; g.w = w; g.ldw = a->ws.ldu; g.rank = (int)a->rank; g.slots = (int)a->slots;
+    g.begin = a->ws.begin; g.row_slot = a->ws.row_slot; g.slab = a->ws.slab;
+    const dim3 grid((M + 63) / 64, (rows + kFactorRows - 1) / kFactorRows), block(256);
+    ProfScope prof("adapt_grad", s);
+    switch ((a->rank + 15) / 16) {
+    case 1: hipLaunchKernelGGL((factor_grad_kernel<1>), grid, block, 0, s, g); break;
+    case 2: hipLaunchKernelGGL((factor_grad_kernel<2>), grid, block, 0, s, g); break;
+    case 3: hipLaunchKernelGGL((factor_grad_kernel<3>), grid, block, 0, s, g); break;
+    default: hipLaunchKernelGGL((factor_grad_kernel<4>), grid, block, 0, s, g); break;
+    }
+    hipLaunchKernelGGL(factor_reduce_kernel, dim3((M * a->rank + 255) / 256, a->slots), block, 0, s, g.slab, g.begin, M, g.rank, g_m, g_j,
+                       a->d_grad + off, a->per_slot());
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
+}
+
+void adapt_args(GemmArgs& g, const Adapters* a, const float* low, const float* up, int up_k, int up_n)
+{
+    g.low = low; g.ld_low = a->ws.ldu; g.up = up; g.up_slot = a->per_slot(); g.up_k = up_k; g.up_n = up_n; g.rank = (int)a->rank;
+    g.row_slot = a->ws.row_slot;
+}
+
+// logits of `rows` grouped rows in the workspace's lg, activations in h1, h2, rank columns in u2, u3
+int forward_rows(Net* n, Adapters* a, uint32_t rows, hipStream_t s)
+{
+    AdaptWorkspace& w = a->ws;
+    const float* P = n->d_params;
+    const float* F = a->d_params;
+    const int r = (int)a->rank;
+    const bool x3 = use_x3(n, rows), wide1 = use_wide_f32(n, rows), wide = !x3 && wide1;
+    int rc;
+    if (x3 || wide) {
+        ProfScope prof("w2t", s);
+        hipLaunchKernelGGL(transpose_kernel, dim3((n->h2 + 31) / 32, (n->h1 + 31) / 32), dim3(256), 0, s, P + n->off_w2(), (int)n->h1,
+                           (int)n->h2, w.w2t);
+        const uint64_t count = (uint64_t)n->h1 * n->h2;
+        if (x3)
+            hipLaunchKernelGGL(split_planes_kernel, dim3((unsigned)((count / 2 + 255) / 256)), dim3(256), 0, s, w.w2t, count, w.w2s, count / 2);
+    }
+    if (wide1) {
+        ProfScope prof("w2t", s);
+        hipLaunchKernelGGL(pad_transpose_kernel, dim3((n->h1 * w.ldx + 255) / 256), dim3(256), 0, s, P + n->off_w1(), (int)n->in, (int)n->h1,
+                           w.ldx, w.w1t);
+    }
+    SZ_HIP(hipGetLastError());
+    GemmArgs g{};
+    g.A = w.xs; g.lda = w.ldx; g.a_pad = 0; g.C = w.h1; g.ldc = w.ld1; g.M = (int)rows; g.N = (int)n->h1; g.bias = P + n->off_b1();
+    if (wide1) {
+        g.B = w.w1t; g.ldb = w.ldx; g.K = g.k_chunk = w.ldx;
+        rc = launch_gemm_f32w<EPI_BIAS_RELU, T_ADAPT1>(g, s);
+    } else {
+        g.B = P + n->off_w1(); g.ldb = (int)n->h1; g.K = g.k_chunk = (int)n->in;
+        rc = launch_gemm<A_ROWS, B_KROWS, EPI_BIAS_RELU, T_ADAPT1>(g, 1, s);
+    }
+    if (rc) return rc;
+    rc = low_product(a, w.h1, w.ld1, (int)n->h1, F + a->off_a2(), r, 1, rows, w.u2, s);
+    if (rc) return rc;
+    g = GemmArgs{};
+    g.A = w.h1; g.lda = w.ld1; g.C = w.h2; g.ldc = w.ld2; g.M = (int)rows; g.N = (int)n->h2; g.K = g.k_chunk = (int)n->h1;
+    g.bias = P + n->off_b2();
+    adapt_args(g, a, w.u2, F + a->off_b2(), (int)n->h2, 1);
+    if (x3) {
+        g.B = (const float*)w.w2s; g.ldb = (int)n->h1; g.b_plane = (uint64_t)n->h1 * n->h2;
+        rc = launch_gemm_x3<X3_ROWS_F32, X3_ROWS_SPLIT, EPI_ADAPT_TANH, T_ADAPT2>(g, 1, s);
+    } else if (wide) {
+        g.B = w.w2t; g.ldb = (int)n->h1;
+        rc = launch_gemm_f32w<EPI_ADAPT_TANH, T_ADAPT2>(g, s);
+    } else {
+        g.B = P + n->off_w2(); g.ldb = (int)n->h2;
+        rc = launch_gemm<A_ROWS, B_KROWS, EPI_ADAPT_TANH, T_ADAPT2>(g, 1, s);
+    }
+    if (rc || n->out == 0) return rc;
+    rc = low_product(a, w.h2, w.ld2, (int)n->h2, F + a->off_a3(), r, 1, rows, w.u3, s);
+    if (rc) return rc;
+    g = GemmArgs{};
+    g.A = w.h2; g.lda = w.ld2; g.C = w.lg; g.ldc = w.ld3; g.M = (int)rows; g.N = (int)n->out; g.K = g.k_chunk = (int)n->h2;
+    g.B = P + n->off_w3(); g.ldb = (int)n->out; g.bias = P + n->off_b3();
+    adapt_args(g, a, w.u3, F + a->off_b3(), (int)n->out, 1);
+    return launch_gemm<A_ROWS, B_KROWS, EPI_ADAPT_BIAS, T_ADAPT3>(g, 1, s);
+}
+
+int gather_rows(Adapters* a, const float* x, uint32_t rows, float dropout, uint64_t seed, uint64_t counter0, uint8_t* live, hipStream_t s)
+{
+    ProfScope prof("prep", s);
+    hipLaunchKernelGGL(gather_rows_kernel, dim3((rows + 3) / 4), dim3(256), 0, s, x, a->ws.order, rows, (int)a->in, dropout, seed, counter0,
+                       a->ws.xs, a->ws.ldx, live);
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
+}
+
+// the controls of the call's rows from row r0 on
+Controls from_row(const Controls& c, uint64_t r0)
+{
+    Controls d = c;
+    if (d.set_of_row) d.set_of_row += r0;
+    return d;
+}
+
+}  // namespace
+
+int adapters_create(const Net* n, uint32_t slots, uint32_t rank, float scale, const float* init, uint64_t seed, Adapters** out)
+{
+    Adapters* a = new (std::nothrow) Adapters();
+    if (!a) { set_error("out of host memory"); return SZH_ENOMEM; }
+    a->in = n->in; a->h1 = n->h1; a->h2 = n->h2; a->out = n->out;
+    a->slots = slots; a->rank = rank; a->scale = scale; a->device = n->device;
+    const uint64_t np = a->per_slot() * slots;
+    hipError_t he = hipMalloc((void**)&a->d_params, (np + 1) * sizeof(float));
+    if (he == hipSuccess) he = hipMalloc((void**)&a->d_grad, (np + 2ull * slots) * sizeof(float));
+    if (he == hipSuccess) he = hipMalloc((void**)&a->d_sums, 2ull * slots * sizeof(double));
+    if (he != hipSuccess) { adapters_destroy(a); return hip_fail(he, "adapter allocation"); }
+    int rc = adapters_zero_grad(a, nullptr);
+    if (!rc && init) rc = adapters_set_params(a, 0, slots, init);
+    if (!rc && !init) {
+        // A ~ U(-0.5, 0.5) / sqrt(its inputs), B = 0: a new adapter changes nothing until it is trained
+        try {
+            std::vector<float> p(np, 0.0f);
+            const float s2 = 1.0f / std::sqrt((float)a->h1), s3 = 1.0f / std::sqrt((float)a->h2);
+            for (uint32_t k = 0; k < slots; ++k) {
+                float* q = p.data() + k * a->per_slot();
+                for (uint64_t i = a->off_a2(); i < a->off_b2(); ++i) q[i] = s2 * init_uniform(seed, k * a->per_slot() + i);
+                for (uint64_t i = a->off_a3(); i < a->off_b3(); ++i) q[i] = s3 * init_uniform(seed, k * a->per_slot() + i);
+            }
+            rc = adapters_set_params(a, 0, slots, p.data());
+        } catch (const std::bad_alloc&) {
+            set_error("out of host memory");
+            rc = SZH_ENOMEM;
+        }
+    }
+    if (!rc && hipDeviceSynchronize() != hipSuccess) { set_error("device synchronize failed"); rc = SZH_ENODEVICE; }
+    if (rc) { adapters_destroy(a); return rc; }
+    *out = a;
+    return SZH_OK;
+}
+
+void adapters_destroy(Adapters* a)
+{
+    if (!a) return;
+    clip_destroy(a->clip);
+    if (a->d_params) (void)hipFree(a->d_params);
+    if (a->d_grad) (void)hipFree(a->d_grad);
+    if (a->d_sums) (void)hipFree(a->d_sums);
+    for (char* p : a->arenas) (void)hipFree(p);
+    delete a;
+}
+
+int adapters_set_params(Adapters* a, uint32_t slot0, uint32_t count, const float* flat)
+{
+    SZ_HIP(hipDeviceSynchronize());
+    SZ_HIP(hipMemcpy(a->d_params + slot0 * a->per_slot(), flat, count * a->per_slot() * sizeof(float), hipMemcpyHostToDevice));
+    return SZH_OK;
+}
+
+int adapters_get_params(Adapters* a, uint32_t slot0, uint32_t count, float* flat)
+{
+    SZ_HIP(hipDeviceSynchronize());
+    SZ_HIP(hipMemcpy(flat, a->d_params + slot0 * a->per_slot(), count * a->per_slot() * sizeof(float), hipMemcpyDeviceToHost));
+    return SZH_OK;
+}
+
+int adapters_reserve(Adapters* a, uint64_t rows, bool training)
+{
+    if (training)
+        if (int rc = adapters_clip_tables(a)) return rc;
+    return ensure(a, rows, training, nullptr);
+}
+
+int adapters_forward(Net* n, Adapters* a, const float* x, const int32_t* slots_dev, uint64_t rows, const Controls& ctl, float* logits,
+                     float* probs, hipStream_t s)
+{
+    if (int rc = check_pair(n, a)) return rc;
+    if (rows == 0 || n->out == 0) return SZH_OK;
+    if (int rc = ensure(a, rows, false, s)) return rc;
+    for (uint64_t r0 = 0; r0 < rows; r0 += kAdaptRows) {
+        const uint32_t R = (uint32_t)std::min<uint64_t>(kAdaptRows, rows - r0);
+        int rc = group_rows(a, slots_dev ? slots_dev + r0 : nullptr, R, s);
+        if (!rc) rc = gather_rows(a, x + r0 * n->in, R, 0.0f, 0, 0, nullptr, s);
+        if (!rc) rc = forward_rows(n, a, R, s);
+        if (rc) return rc;
+        ControlRun c{};
+        c.in = a->ws.lg; c.ld_in = a->ws.ld3; c.rows = R; c.classes = n->out; c.order = a->ws.order;
+        c.raw = logits ? logits + r0 * n->out : nullptr; c.ld_raw = n->out;
+        c.out = probs ? probs + r0 * n->out : nullptr; c.ld_out = n->out; c.probs = true;
+        rc = control_run(from_row(ctl, r0), c, s);
+        if (rc) return rc;
+    }
+    return SZH_OK;
+}
+
+int adapters_vote(Net* n, Adapters* a, const float* x, const int32_t* slots_dev, uint64_t rows, const Controls& ctl, float threshold,
+                  const int32_t* group, uint32_t groups, unsigned long long* counts, hipStream_t s)
+{
+    if (int rc = check_pair(n, a)) return rc;
+    if (rows == 0 || n->out == 0) return SZH_OK;
+    if (int rc = ensure(a, rows, false, s)) return rc;
+    for (uint64_t r0 = 0; r0 < rows; r0 += kAdaptRows) {
+        const uint32_t R = (uint32_t)std::min<uint64_t>(kAdaptRows, rows - r0);
+        int rc = group_rows(a, slots_dev ? slots_dev + r0 : nullptr, R, s);
+        if (!rc) rc = gather_rows(a, x + r0 * n->in, R, 0.0f, 0, 0, nullptr, s);
+        if (!rc) rc = forward_rows(n, a, R, s);
+        if (rc) return rc;
+        ControlRun c{};
+        c.in = a->ws.lg; c.ld_in = a->ws.ld3; c.rows = R; c.classes = n->out; c.order = a->ws.order;
+        c.threshold = threshold; c.group = group ? group + r0 : nullptr; c.groups = groups; c.votes = counts;
+        rc = control_run(from_row(ctl, r0), c, s);
+        if (rc) return rc;
+    }
+    return SZH_OK;
+}
+
+int adapters_accumulate(Net* n, Adapters* a, const float* x, const int32_t* labels, const int32_t* slots_dev, uint64_t rows,
+                        const Controls& ctl, float dropout, uint64_t seed, hipStream_t s)
+{
+    if (int rc = check_pair(n, a)) return rc;
+    if (rows == 0 || n->out == 0) return SZH_OK;
+    if (int rc = ensure(a, rows, true, s)) return rc;
+    AdaptWorkspace& w = a->ws;
+    const float* F = a->d_params;
+    const int r = (int)a->rank, h1 = (int)n->h1, h2 = (int)n->h2, out = (int)n->out;
+    for (uint64_t r0 = 0; r0 < rows; r0 += kAdaptRows) {
+        const uint32_t R = (uint32_t)std::min<uint64_t>(kAdaptRows, rows - r0);
+        int rc = group_rows(a, slots_dev + r0, R, s);
+        if (!rc) rc = gather_rows(a, x + r0 * n->in, R, dropout, seed, r0, w.live0, s);
+        if (!rc) rc = forward_rows(n, a, R, s);
+        if (rc) return rc;
+        ControlRun c{};
+        c.in = w.lg; c.ld_in = w.ld3; c.rows = R; c.classes = n->out; c.order = w.order;
+        c.out = w.lg; c.ld_out = w.ld3; c.labels = labels + r0; c.row_live = w.live0; c.row_slot = w.row_slot; c.loss = w.loss; c.live = w.live;
+        rc = control_run(from_row(ctl, r0), c, s);   // lg now holds d3
+        if (rc) return rc;
+        rc = low_product(a, w.lg, w.ld3, out, F + a->off_b3(), 1, out, R, w.g3, s);
+        if (rc) return rc;
+        GemmArgs g{};
+        g.A = w.lg; g.lda = w.ld3; g.B = n->d_params + n->off_w3(); g.ldb = out; g.C = w.d2; g.ldc = w.ld2;
+        g.M = (int)R; g.N = h2; g.K = g.k_chunk = out; g.aux = w.h2; g.ldaux = w.ld2;
+        adapt_args(g, a, w.g3, F + a->off_a3(), 1, r);
+        rc = launch_gemm<A_ROWS, B_ROWS, EPI_ADAPT_DTANH, T_ADAPT_D2>(g, 1, s);
+        if (!rc) rc = low_product(a, w.d2, w.ld2, h2, F + a->off_b2(), 1, h2, R, w.g2, s);
+        if (!rc) rc = factor_gradient(a, w.h1, w.ld1, h1, w.g2, R, a->off_a2(), r, 1, s);
+        if (!rc) rc = factor_gradient(a, w.d2, w.ld2, h2, w.u2, R, a->off_b2(), 1, h2, s);
+        if (!rc) rc = factor_gradient(a, w.h2, w.ld2, h2, w.g3, R, a->off_a3(), r, 1, s);
+        if (!rc) rc = factor_gradient(a, w.lg, w.ld3, out, w.u3, R, a->off_b3(), 1, out, s);
+        if (rc) return rc;
+        hipLaunchKernelGGL(slot_stats_kernel, dim3(a->slots), dim3(256), 0, s, w.loss, w.live, w.begin, a->d_sums,
+                           a->d_grad + a->per_slot() * a->slots);
+        SZ_HIP(hipGetLastError());
+    }
+    return SZH_OK;
+}
+
+int adapters_zero_grad(Adapters* a, hipStream_t s)
+{
+    const uint64_t n = (a->per_slot() + 2) * a->slots;
+    hipLaunchKernelGGL(adapter_clear_kernel, dim3((unsigned)std::min<uint64_t>((n + 1023) / 1024, 4096)), dim3(256), 0, s, a->d_grad, n, a->d_sums,
+                       2ull * a->slots);
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
+}
+
+int adapters_clip(Adapters* a, float max_norm, float* norms_dev, hipStream_t s)
+{
+    if (!a->clip) {
+        if (capturing(s)) { set_error("adapters: the first clipping allocates its tables and cannot be captured (szh_adapters_reserve makes them)"); return SZH_EINVAL; }
+        if (int rc = adapters_clip_tables(a)) return rc;
+    }
+    return clip_run(a->clip, max_norm, norms_dev, s);
+}
+
+int adapters_clip_tables(Adapters* a)
+{
+    if (a->clip) return SZH_OK;
+    std::vector<ClipTensor> t(a->slots);
+    for (uint32_t k = 0; k < a->slots; ++k) t[k] = {a->d_grad + k * a->per_slot(), a->d_grad + k * a->per_slot(), a->per_slot(), k};
+    return clip_create(t.data(), a->slots, a->slots, a->d_grad + a->per_slot() * a->slots + 1, 2, &a->clip);
+}
+
+int adapters_apply(Adapters* a, float lr, hipStream_t s)
+{
+    ProfScope prof("apply", s);
+    hipLaunchKernelGGL(adapter_apply_kernel, dim3((unsigned)((a->per_slot() + 255) / 256), a->slots), dim3(256), 0, s, a->d_params, a->d_grad,
+                       a->d_grad + a->per_slot() * a->slots, a->per_slot(), lr);
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
+}
+
+}  // namespace sz

@@ -1,0 +1,361 @@
+// Kernels of the low-rank adapters (adapt.hip): grouping of a call's rows by adapter, the products with the
+// rank columns, the factors' gradients and the update.  The large products are the GEMM kernels of
+// gemm_kernel.h / gemm_bf16x3.h with an EPI_ADAPT_* epilogue.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "rng.h"
+
+namespace sz {
+namespace adapt {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// ---- grouping: the rows of a call in the order of their slots ---------------------------------
+// A stable counting sort: key = slot for 0 <= slot < slots, else `slots` (rows without an adapter, last).
+// One wave counts / places kGroupRows rows, 64 at a time, so that a row's rank among the rows of its key is
+// the wave's running count plus the members among the lower lanes: the order, and with it every sum over
+// rows, is the same on every call.
+constexpr int kGroupRows = 512;
+
+__device__ __forceinline__ int group_key(const int32_t* slot, uint64_t r, int slots)
+{
+    const int s = slot ? slot[r] : -1;
+    return s >= 0 && s < slots ? s : slots;
+}
+
+// Visits the distinct keys of the wave's active lanes: f(key, mask of the lanes that hold it).
+template <class F>
+__device__ __forceinline__ void each_key(int key, bool active, F f)
+{
+    unsigned long long left = __ballot(active);
+    while (left) {
+        const int k = __builtin_amdgcn_readlane(key, __ffsll(left) - 1);
+        const unsigned long long member = __ballot(active && key == k);
+        left &= ~member;
+        f(k, member);
+    }
+}
+
+// count[key][block] of a block of rows
+__global__ __launch_bounds__(64) void group_count_kernel(const int32_t* __restrict__ slot, uint32_t rows, int slots, int blocks,
+                                                         uint32_t* __restrict__ count)
+{
+    extern __shared__ uint32_t hist[];
+    for (int k = threadIdx.x; k <= slots; k += 64) hist[k] = 0;
+    __syncthreads();
+    const uint32_t r0 = blockIdx.x * kGroupRows, r1 = min(rows, r0 + kGroupRows);
+    for (uint32_t r = r0; r < r1; r += 64) {
+        const bool in = r + threadIdx.x < r1;
+        const int key = in ? group_key(slot, r + threadIdx.x, slots) : 0;
+        each_key(key, in, [&](int k, unsigned long long member) {
+            if (threadIdx.x == 0) hist[k] += (uint32_t)__popcll(member);
+        });
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k <= slots; k += 64) count[(size_t)k * blocks + blockIdx.x] = hist[k];
+}
+
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v)  // inclusive
+{
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t u = __shfl_up(v, o);
+        if ((int)(threadIdx.x & 63) >= o) v += u;
+    }
+    return v;
+}
+
+// count[key][0 .. blocks) becomes its exclusive prefix sums, total[key] the sum; one wave per key
+__global__ __launch_bounds__(64) void group_scan_kernel(uint32_t* __restrict__ count, int blocks, uint32_t* __restrict__ total)
+{
+    uint32_t* c = count + (size_t)blockIdx.x * blocks;
+    uint32_t run = 0;
+    for (int b = 0; b < blocks; b += 64) {
+        const int i = b + (int)threadIdx.x;
+        const uint32_t v = i < blocks ? c[i] : 0;
+        const uint32_t inc = wave_scan(v);
+        if (i < blocks) c[i] = run + inc - v;
+        run += __shfl(inc, 63);
+    }
+    if (threadIdx.x == 0) total[blockIdx.x] = run;
+}
+
+// begin[key] = first place of the key's rows, begin[slots + 1] = rows; one wave
+__global__ __launch_bounds__(64) void group_begin_kernel(const uint32_t* __restrict__ total, int slots, uint32_t rows,
+                                                         uint32_t* __restrict__ begin)
+{
+    uint32_t run = 0;
+    for (int b = 0; b <= slots; b += 64) {
+        const int i = b + (int)threadIdx.x;
+        const uint32_t v = i <= slots ? total[i] : 0;
+        const uint32_t inc = wave_scan(v);
+        if (i <= slots) begin[i] = run + inc - v;
+        run += __shfl(inc, 63);
+    }
+    if (threadIdx.x == 0) begin[slots + 1] = rows;
+}
+
+// order[place] = row, row_slot[place] = its slot or -1
+__global__ __launch_bounds__(64) void group_place_kernel(const int32_t* __restrict__ slot, uint32_t rows, int slots, int blocks,
+                                                         const uint32_t* __restrict__ count, const uint32_t* __restrict__ begin,
+                                                         uint32_t* __restrict__ order, int32_t* __restrict__ row_slot)
+{
+    extern __shared__ uint32_t next[];
+    for (int k = threadIdx.x; k <= slots; k += 64) next[k] = begin[k] + count[(size_t)k * blocks + blockIdx.x];
+    __syncthreads();
+    const uint32_t r0 = blockIdx.x * kGroupRows, r1 = min(rows, r0 + kGroupRows);
+    for (uint32_t r = r0; r < r1; r += 64) {
+        const bool in = r + threadIdx.x < r1;
+        const int key = in ? group_key(slot, r + threadIdx.x, slots) : 0;
+        uint32_t place = 0;
+        each_key(key, in, [&](int k, unsigned long long member) {
+            const uint32_t base = next[k];
+            if (in && key == k) place = base + (uint32_t)__popcll(member & ((1ull << threadIdx.x) - 1));
+            __syncthreads();  // (one wave: every lane has read next[k])
+            if (threadIdx.x == 0) next[k] = base + (uint32_t)__popcll(member);
+            __syncthreads();
+        });
+        if (in) {
+            order[place] = r + threadIdx.x;
+            row_slot[place] = key < slots ? key : -1;
+        }
+    }
+}
+
+// ---- rows in that order -------------------------------------------------------------------------
+// xs[i] = [x[order[i]] | 1 | 0 ...] with input dropout (element j of row r zeroed where uniform01(seed,
+// counter0 + r, j) < dropout: the draws of szh_net_accumulate_dev), live[i] = any element left.  One wave per row.
+__global__ __launch_bounds__(256) void gather_rows_kernel(const float* __restrict__ x, const uint32_t* __restrict__ order,
+                                                          uint32_t rows, int in, float dropout, uint64_t seed, uint64_t counter0,
+                                                          float* __restrict__ xs, int ldx, uint8_t* __restrict__ live)
+{
+    const uint32_t i = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= rows) return;
+    const uint32_t r = order[i];
+    const int lane = threadIdx.x & 63;
+    bool any = false;
+    for (int j = lane; j < ldx; j += 64) {
+        float v = j == in ? 1.0f : 0.0f;
+        if (j < in) {
+            v = x[(size_t)r * in + j];
+            if (dropout > 0.0f && uniform01(seed, counter0 + r, (uint64_t)j) < dropout) v = 0.0f;
+            any = any || v != 0.0f;
+        }
+        xs[(size_t)i * ldx + j] = v;
+    }
+    if (live) {
+        const bool some = __any(any);
+        if (lane == 0) live[i] = some ? 1 : 0;
+    }
+}
+
+// ---- products with the rank columns ----------------------------------------------------------------
+// u[i][j] = scale * sum_k x[i][k] F[k][j],  F = the [K][rank] matrix of row i's slot with element (k, j) at
+// k * f_k + j * f_j.  Columns from rank to ldu, and rows without a slot, are zero.
+struct LowArgs {
+    const float* x;      // [rows][ldx], 16-byte aligned rows
+    const float* factor; // slot 0's matrix
+    uint64_t factor_slot;
+    const int32_t* row_slot;
+    float* u;
+    uint32_t rows;
+    int ldx, K, f_k, f_j, rank, ldu;
+    float scale;
+};
+
+// 32 rows per workgroup on v_mfma_f32_16x16x4_f32, the K range split over its four waves and joined in LDS.
+// A step pairs lane group q's k with k0 + 4 q + t, so that a lane reads 16 bytes of its row for four steps.
+template <int NT>
+__global__ __launch_bounds__(256) void low_kernel(LowArgs a)
+{
+    __shared__ __attribute__((aligned(16))) float part[4][32][NT * 16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r16 = lane & 15, q = lane >> 4;
+    const uint32_t row0 = blockIdx.x * 32;
+    const uint32_t my_row = row0 + (lane & 31);
+    const int mine = my_row < a.rows ? a.row_slot[my_row] : -1;
+    uint32_t left = (uint32_t)__ballot(mine >= 0);
+    const int blocks = (a.K + 15) / 16, per = (blocks + 3) / 4;
+    const int b0 = wave * per, b1 = min(blocks, b0 + per);
+    const float* x[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) x[t] = a.x + (size_t)min(row0 + 16 * t + r16, a.rows - 1) * a.ldx + 4 * q;
+    // rows without an adapter
+    const uint32_t none = ~left;
+    for (int e = threadIdx.x; e < 32 * a.ldu; e += 256) {
+        const int r = e / a.ldu;
+        if (row0 + r < a.rows && ((none >> r) & 1u)) a.u[(size_t)(row0 + r) * a.ldu + e % a.ldu] = 0.0f;
+    }
+    while (left) {
+        const int slot = __builtin_amdgcn_readlane(mine, __builtin_ctz(left));
+        const uint32_t member = (uint32_t)__ballot(mine == slot);
+        left &= ~member;
+        const float* f = a.factor + (size_t)slot * a.factor_slot;
+        f32x4 acc[2][NT];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int b = b0; b < b1; ++b) {
+            f32x4 xv[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) xv[t] = *reinterpret_cast<const f32x4*>(x[t] + 16 * b);
+            const int k0 = 16 * b + 4 * q;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool in_k = k0 + e < a.K;
+                const float* fk = f + (size_t)min(k0 + e, a.K - 1) * a.f_k;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int j = 16 * n + r16;
+                    float v = fk[(size_t)min(j, a.rank - 1) * a.f_j];
+                    v = in_k && j < a.rank ? v : 0.0f;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(in_k ? xv[t][e] : 0.0f, v, acc[t][n], 0, 0, 0);
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[wave][16 * t + 4 * q + i][16 * n + r16] = acc[t][n][i];
+        __syncthreads();
+        for (int e = threadIdx.x; e < 32 * NT * 16; e += 256) {
+            const int r = e / (NT * 16), j = e % (NT * 16);
+            if (j < a.ldu && row0 + r < a.rows && ((member >> r) & 1u))
+                a.u[(size_t)(row0 + r) * a.ldu + j] = a.scale * ((part[0][r][j] + part[1][r][j]) + (part[2][r][j] + part[3][r][j]));
+        }
+        __syncthreads();
+    }
+}
+
+// ---- factor gradients -----------------------------------------------------------------------------
+// slab[chunk + slot][m][j] = sum over the slot's rows i in the chunk of p[i][m] w[i][j].  Rows are sorted by
+// slot, so (chunk, slot) pairs that hold rows lie on a staircase and chunk + slot numbers them without a gap
+// table; factor_reduce_kernel adds a slot's chunks in order.
+constexpr int kFactorRows = 512;
+struct FactorArgs {
+    const float* p;        // [rows][ldp], 16-byte aligned rows
+    const float* w;        // [rows][ldw], the rank columns
+    const uint32_t* begin; // [slots + 2]
+    const int32_t* row_slot;
+    float* slab;
+    int ldp, M, ldw, rank, slots;
+};
+
+// 64 columns of p per workgroup; its four waves take rows in turn and are joined in LDS.  A lane reads 16
+// bytes of a row of p for four matrix instructions: step t's columns are 4 c + t.
+template <int NT>
+__global__ __launch_bounds__(256) void factor_grad_kernel(FactorArgs a)
+{
+    __shared__ __attribute__((aligned(16))) float part[4][64][NT * 16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c16 = lane & 15, q = lane >> 4;
+    const int m0 = blockIdx.x * 64;
+    const uint32_t end = min(a.begin[a.slots], (blockIdx.y + 1) * (uint32_t)kFactorRows);
+    uint32_t r = blockIdx.y * (uint32_t)kFactorRows;
+    while (r < end) {
+        const int slot = a.row_slot[r];
+        const uint32_t stop = min(end, a.begin[slot + 1]);
+        f32x4 acc[4][NT];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t i = r + 4 * wave; i < stop; i += 16) {
+            const bool in = i + q < stop;
+            const size_t row = in ? i + q : stop - 1;
+            const int col = m0 + 4 * c16;
+            f32x4 pv = *reinterpret_cast<const f32x4*>(a.p + row * a.ldp + min(col, a.ldp - 4));
+#pragma unroll
+            for (int t = 0; t < 4; ++t) pv[t] = in && col + t < a.M ? pv[t] : 0.0f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int j = 16 * n + c16;
+                float v = a.w[row * a.ldw + min(j, a.rank - 1)];
+                v = in && j < a.rank ? v : 0.0f;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[t], v, acc[t][n], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[wave][4 * (4 * q + i) + t][16 * n + c16] = acc[t][n][i];
+        __syncthreads();
+        float* slab = a.slab + ((size_t)blockIdx.y + slot) * a.M * a.rank;
+        for (int e = threadIdx.x; e < 64 * a.rank; e += 256) {
+            const int m = e / a.rank, j = e % a.rank;
+            if (m0 + m < a.M)
+                slab[(size_t)(m0 + m) * a.rank + j] = (part[0][m][j] + part[1][m][j]) + (part[2][m][j] + part[3][m][j]);
+        }
+        __syncthreads();
+        r = stop;
+    }
+}
+
+// grad[slot][m * g_m + j * g_j] += the slot's chunks of the slab; 64-bit sums, in chunk order
+__global__ __launch_bounds__(256) void factor_reduce_kernel(const float* __restrict__ slab, const uint32_t* __restrict__ begin, int M,
+                                                            int rank, int g_m, int g_j, float* __restrict__ grad,
+                                                            uint64_t grad_slot)
+{
+    const int slot = blockIdx.y;
+    const uint32_t b = begin[slot], e = begin[slot + 1];
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (b == e || i >= M * rank) return;
+    const uint32_t c0 = b / kFactorRows, c1 = (e - 1) / kFactorRows;
+    double t = 0.0;
+    for (uint32_t c = c0; c <= c1; ++c) t += (double)slab[(size_t)(c + slot) * M * rank + i];
+    float* g = grad + (size_t)slot * grad_slot + (size_t)(i / rank) * g_m + (size_t)(i % rank) * g_j;
+    *g += (float)t;
+}
+
+// sums[slot] += {loss, live rows} of the slot's rows (64 bits, fixed order); tail = the same as floats
+__global__ __launch_bounds__(256) void slot_stats_kernel(const float* __restrict__ loss, const uint8_t* __restrict__ live,
+                                                         const uint32_t* __restrict__ begin, double* __restrict__ sums,
+                                                         float* __restrict__ tail)
+{
+    __shared__ double sl[256], sc[256];
+    const int slot = blockIdx.x;
+    double l = 0.0, c = 0.0;
+    for (uint32_t i = begin[slot] + threadIdx.x; i < begin[slot + 1]; i += 256) { l += (double)loss[i]; c += (double)live[i]; }
+    sl[threadIdx.x] = l; sc[threadIdx.x] = c;
+    __syncthreads();
+    for (int o = 128; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) { sl[threadIdx.x] += sl[threadIdx.x + o]; sc[threadIdx.x] += sc[threadIdx.x + o]; }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        const double a = sums[2 * slot] + sl[0], b = sums[2 * slot + 1] + sc[0];
+        sums[2 * slot] = a; sums[2 * slot + 1] = b;
+        tail[2 * slot] = (float)a; tail[2 * slot + 1] = (float)b;
+    }
+}
+
+// params -= (lr / live) * grad for every slot with live rows (lib.rs:1047-1059, a slot at a time)
+__global__ __launch_bounds__(256) void adapter_apply_kernel(float* __restrict__ params, const float* __restrict__ grad,
+                                                            const float* __restrict__ tail, uint64_t per_slot, float lr)
+{
+    const float live = tail[2 * blockIdx.y + 1];
+    if (!(live > 0.0f)) return;
+    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < per_slot) params[blockIdx.y * per_slot + i] -= grad[blockIdx.y * per_slot + i] * (lr / live);
+}
+
+// (a kernel and not a memory-set node, which must not be captured into a graph)
+__global__ __launch_bounds__(256) void adapter_clear_kernel(float* __restrict__ grad, uint64_t n, double* __restrict__ sums, uint64_t n_sums)
+{
+    const uint64_t step = (uint64_t)gridDim.x * 256;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) grad[i] = 0.0f;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n_sums; i += step) sums[i] = 0.0;
+}
+
+}  // namespace adapt
+}  // namespace sz

@@ -1116,6 +1116,219 @@ int szh_net_vote_dev(szh_net* net, const float* feats_dev, uint64_t n, float thr
     SZ_CATCH
 }
 
+// ---- gradient clipping, controls on logits, adapters ------------------------------------------
+
+int szh_net_clip_grad_dev(szh_net* net, float max_norm, float* norm_dev, void* stream)
+{
+    SZ_TRY
+    if (!net) { set_error("null argument"); return SZH_EINVAL; }
+    if (!(max_norm >= 0.0f)) { set_error("max_norm must not be negative"); return SZH_EINVAL; }
+    Net* n = reinterpret_cast<Net*>(net);
+    if (int rc = check_device(n->device)) return rc;
+    return net_clip(n, max_norm, norm_dev, static_cast<hipStream_t>(stream));
+    SZ_CATCH
+}
+
+int szh_clip_create(const float* const* in, float* const* out, const uint64_t* lengths, const uint32_t* group, uint32_t n_tensors,
+                    uint32_t groups, const float* live_dev, szh_clip** clip)
+{
+    SZ_TRY
+    if (!clip || groups == 0 || (n_tensors && (!in || !lengths))) { set_error("null argument"); return SZH_EINVAL; }
+    if (groups > (1u << 20)) { set_error("at most %u groups", 1u << 20); return SZH_EINVAL; }
+    std::vector<ClipTensor> t(n_tensors);
+    std::vector<std::pair<uintptr_t, uintptr_t>> written;
+    for (uint32_t k = 0; k < n_tensors; ++k) {
+        t[k] = {in[k], out ? out[k] : const_cast<float*>(in[k]), lengths[k], group ? group[k] : 0};
+        if (t[k].group >= groups) { set_error("tensor %u: group %u of %u", k, t[k].group, groups); return SZH_EINVAL; }
+        if (lengths[k] && (!t[k].src || !t[k].dst)) { set_error("tensor %u: null address", k); return SZH_EINVAL; }
+        if (lengths[k] > (1ull << 48)) { set_error("tensor %u: length", k); return SZH_EINVAL; }
+        if (((uintptr_t)t[k].src | (uintptr_t)t[k].dst) & 3) { set_error("tensor %u: address is not a multiple of 4", k); return SZH_EINVAL; }
+        if (lengths[k]) written.push_back({(uintptr_t)t[k].dst, (uintptr_t)(t[k].dst + lengths[k])});
+    }
+    // every element is written once, and no tensor is read where another is written
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+        if (written[i].first < written[i - 1].second) { set_error("output tensors overlap"); return SZH_EINVAL; }
+    for (uint32_t k = 0; k < n_tensors; ++k) {
+        if (!lengths[k]) continue;
+        const uintptr_t b = (uintptr_t)t[k].src, e = b + lengths[k] * sizeof(float);
+        auto it = std::upper_bound(written.begin(), written.end(), std::make_pair(b, UINTPTR_MAX));
+        if (it != written.begin()) --it;
+        for (; it != written.end() && it->first < e; ++it) {
+            if (it->second <= b) continue;
+            if (t[k].src == t[k].dst && it->first == b) continue;
+            set_error("tensor %u is read where a result is written", k);
+            return SZH_EINVAL;
+        }
+    }
+    Clip* c = nullptr;
+    if (int rc = clip_create(t.data(), n_tensors, groups, live_dev, 1, &c)) return rc;
+    *clip = reinterpret_cast<szh_clip*>(c);
+    return SZH_OK;
+    SZ_CATCH
+}
+void szh_clip_destroy(szh_clip* clip) { clip_destroy(reinterpret_cast<Clip*>(clip)); }
+int szh_clip_run_dev(szh_clip* clip, float max_norm, float* norms_dev, void* stream)
+{
+    if (!clip) { set_error("null argument"); return SZH_EINVAL; }
+    if (!(max_norm >= 0.0f)) { set_error("max_norm must not be negative"); return SZH_EINVAL; }
+    Clip* c = reinterpret_cast<Clip*>(clip);
+    if (int rc = check_device(c->device)) return rc;
+    return clip_run(c, max_norm, norms_dev, static_cast<hipStream_t>(stream));
+}
+
+static int read_controls(const szh_logit_controls* c, Controls* out)
+{
+    *out = Controls{};
+    if (!c) return SZH_OK;
+    if (c->sets == 0) { set_error("controls without a set"); return SZH_EINVAL; }
+    if (!c->counts && (c->repetition || c->presence || c->frequency)) { set_error("penalties need counts"); return SZH_EINVAL; }
+    out->bias = c->bias; out->allow = c->allow; out->counts = c->counts;
+    out->repetition = c->repetition; out->presence = c->presence; out->frequency = c->frequency;
+    out->sets = c->sets; out->set_of_row = c->set_of_row;
+    return SZH_OK;
+}
+
+int szh_logits_control_dev(const float* logits_dev, uint64_t ld_logits, uint64_t rows, uint32_t classes,
+                           const szh_logit_controls* controls, int what, float* out_dev, uint64_t ld_out, void* stream)
+{
+    SZ_TRY
+    if (what != SZH_CONTROL_LOGITS && what != SZH_CONTROL_PROBS) { set_error("unknown output %d", what); return SZH_EINVAL; }
+    Controls c;
+    if (int rc = read_controls(controls, &c)) return rc;
+    if (rows == 0 || classes == 0) return SZH_OK;
+    if (!logits_dev || !out_dev) { set_error("null argument"); return SZH_EINVAL; }
+    if (classes > (1u << 30) || rows > (1ull << 40)) { set_error("too many rows or classes"); return SZH_EINVAL; }
+    if (ld_logits < classes || ld_out < classes || ld_logits > (1ull << 40) || ld_out > (1ull << 40)) { set_error("row strides must be at least the number of classes"); return SZH_EINVAL; }
+    const uintptr_t a0 = (uintptr_t)logits_dev, a1 = a0 + ((rows - 1) * ld_logits + classes) * sizeof(float);
+    const uintptr_t b0 = (uintptr_t)out_dev, b1 = b0 + ((rows - 1) * ld_out + classes) * sizeof(float);
+    if (a0 < b1 && b0 < a1 && !(a0 == b0 && ld_logits == ld_out)) { set_error("logits and result overlap"); return SZH_EINVAL; }
+    ControlRun r{};
+    r.in = logits_dev; r.ld_in = ld_logits; r.rows = rows; r.classes = classes;
+    r.out = out_dev; r.ld_out = ld_out; r.probs = what == SZH_CONTROL_PROBS;
+    return control_run(c, r, static_cast<hipStream_t>(stream));
+    SZ_CATCH
+}
+
+int szh_adapters_create(const szh_net* net, uint32_t slots, uint32_t rank, float scale, const float* init, uint64_t seed,
+                        szh_adapters** bank)
+{
+    SZ_TRY
+    if (!net || !bank) { set_error("null argument"); return SZH_EINVAL; }
+    if (slots == 0 || slots > SZH_ADAPTER_MAX_SLOTS) { set_error("a bank has 1 to %d slots, not %u", SZH_ADAPTER_MAX_SLOTS, slots); return SZH_EINVAL; }
+    if (rank == 0 || rank > SZH_ADAPTER_MAX_RANK) { set_error("an adapter's rank is 1 to %d, not %u", SZH_ADAPTER_MAX_RANK, rank); return SZH_EINVAL; }
+    if (!std::isfinite(scale)) { set_error("scale must be finite"); return SZH_EINVAL; }
+    const Net* n = reinterpret_cast<const Net*>(net);
+    if (int rc = check_device(n->device)) return rc;
+    Adapters* a = nullptr;
+    if (int rc = adapters_create(n, slots, rank, scale, init, seed, &a)) return rc;
+    *bank = reinterpret_cast<szh_adapters*>(a);
+    return SZH_OK;
+    SZ_CATCH
+}
+void szh_adapters_destroy(szh_adapters* bank) { adapters_destroy(reinterpret_cast<Adapters*>(bank)); }
+uint64_t szh_adapters_param_count(const szh_adapters* bank) { return bank ? reinterpret_cast<const Adapters*>(bank)->per_slot() : 0; }
+
+static int check_slot(const szh_adapters* bank, uint32_t slot, const void* p)
+{
+    if (!bank || !p) { set_error("null argument"); return SZH_EINVAL; }
+    const Adapters* a = reinterpret_cast<const Adapters*>(bank);
+    if (slot >= a->slots) { set_error("slot %u of %u", slot, a->slots); return SZH_EINVAL; }
+    return check_device(a->device);
+}
+int szh_adapters_get_params(szh_adapters* bank, uint32_t slot, float* flat)
+{
+    if (int rc = check_slot(bank, slot, flat)) return rc;
+    return adapters_get_params(reinterpret_cast<Adapters*>(bank), slot, 1, flat);
+}
+int szh_adapters_set_params(szh_adapters* bank, uint32_t slot, const float* flat)
+{
+    if (int rc = check_slot(bank, slot, flat)) return rc;
+    return adapters_set_params(reinterpret_cast<Adapters*>(bank), slot, 1, flat);
+}
+int szh_adapters_reserve(szh_adapters* bank, uint64_t rows, int training)
+{
+    SZ_TRY
+    if (!bank) { set_error("null argument"); return SZH_EINVAL; }
+    Adapters* a = reinterpret_cast<Adapters*>(bank);
+    if (int rc = check_device(a->device)) return rc;
+    return adapters_reserve(a, rows, training != 0);
+    SZ_CATCH
+}
+
+int szh_net_forward_adapted_dev(szh_net* net, szh_adapters* bank, const float* feats_dev, const int32_t* slots_dev, uint64_t n,
+                                const szh_logit_controls* controls, float* logits_dev, float* probs_dev, void* stream)
+{
+    SZ_TRY
+    if (!net || !bank || (n && (!feats_dev || !slots_dev))) { set_error("null argument"); return SZH_EINVAL; }
+    if (n && !logits_dev && !probs_dev) { set_error("no result asked for"); return SZH_EINVAL; }
+    Controls c;
+    if (int rc = read_controls(controls, &c)) return rc;
+    if (int rc = check_device(reinterpret_cast<Net*>(net)->device)) return rc;
+    return adapters_forward(reinterpret_cast<Net*>(net), reinterpret_cast<Adapters*>(bank), feats_dev, slots_dev, n, c, logits_dev,
+                            probs_dev, static_cast<hipStream_t>(stream));
+    SZ_CATCH
+}
+int szh_net_vote_adapted_dev(szh_net* net, szh_adapters* bank, const float* feats_dev, const int32_t* slots_dev, uint64_t n,
+                             const szh_logit_controls* controls, float threshold, const int32_t* group_of_row_dev, uint32_t groups,
+                             unsigned long long* counts_dev, void* stream)
+{
+    SZ_TRY
+    if (!net || !bank || (n && (!feats_dev || !slots_dev || !counts_dev))) { set_error("null argument"); return SZH_EINVAL; }
+    if (groups == 0) { set_error("votes need a group"); return SZH_EINVAL; }
+    Controls c;
+    if (int rc = read_controls(controls, &c)) return rc;
+    if (int rc = check_device(reinterpret_cast<Net*>(net)->device)) return rc;
+    return adapters_vote(reinterpret_cast<Net*>(net), reinterpret_cast<Adapters*>(bank), feats_dev, slots_dev, n, c, threshold,
+                         group_of_row_dev, groups, counts_dev, static_cast<hipStream_t>(stream));
+    SZ_CATCH
+}
+
+uint64_t szh_adapters_grad_len(const szh_adapters* bank)
+{
+    const Adapters* a = reinterpret_cast<const Adapters*>(bank);
+    return a ? (a->per_slot() + 2) * a->slots : 0;
+}
+float* szh_adapters_grad_dev(szh_adapters* bank) { return bank ? reinterpret_cast<Adapters*>(bank)->d_grad : nullptr; }
+int szh_adapters_zero_grad_dev(szh_adapters* bank, void* stream)
+{
+    if (!bank) { set_error("null argument"); return SZH_EINVAL; }
+    Adapters* a = reinterpret_cast<Adapters*>(bank);
+    if (int rc = check_device(a->device)) return rc;
+    return adapters_zero_grad(a, static_cast<hipStream_t>(stream));
+}
+int szh_adapters_accumulate_dev(szh_net* net, szh_adapters* bank, const float* feats_dev, const int32_t* labels_dev,
+                                const int32_t* slots_dev, uint64_t n, const szh_logit_controls* controls, float dropout, uint64_t seed,
+                                void* stream)
+{
+    SZ_TRY
+    if (!net || !bank || (n && (!feats_dev || !labels_dev || !slots_dev))) { set_error("null argument"); return SZH_EINVAL; }
+    Controls c;
+    if (int rc = read_controls(controls, &c)) return rc;
+    if (c.counts) { set_error("training takes no penalties"); return SZH_EINVAL; }
+    if (int rc = check_device(reinterpret_cast<Net*>(net)->device)) return rc;
+    return adapters_accumulate(reinterpret_cast<Net*>(net), reinterpret_cast<Adapters*>(bank), feats_dev, labels_dev, slots_dev, n, c,
+                               dropout, seed, static_cast<hipStream_t>(stream));
+    SZ_CATCH
+}
+int szh_adapters_clip_grad_dev(szh_adapters* bank, float max_norm, float* norms_dev, void* stream)
+{
+    SZ_TRY
+    if (!bank) { set_error("null argument"); return SZH_EINVAL; }
+    if (!(max_norm >= 0.0f)) { set_error("max_norm must not be negative"); return SZH_EINVAL; }
+    Adapters* a = reinterpret_cast<Adapters*>(bank);
+    if (int rc = check_device(a->device)) return rc;
+    return adapters_clip(a, max_norm, norms_dev, static_cast<hipStream_t>(stream));
+    SZ_CATCH
+}
+int szh_adapters_apply_grad_dev(szh_adapters* bank, float lr, void* stream)
+{
+    if (!bank) { set_error("null argument"); return SZH_EINVAL; }
+    Adapters* a = reinterpret_cast<Adapters*>(bank);
+    if (int rc = check_device(a->device)) return rc;
+    return adapters_apply(a, lr, static_cast<hipStream_t>(stream));
+}
+
 // ---- metadata ---------------------------------------------------------------------------
 
 int szh_net_record_training_file(szh_net* net, uint32_t speaker, const char* path)

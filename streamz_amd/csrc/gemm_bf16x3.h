@@ -45,7 +45,7 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_
 }
 
 // dst[plane][i] = piece `plane` of src[i]; count is even and both arrays are 4-byte aligned
-__global__ __launch_bounds__(256) void split_planes_kernel(const float* __restrict__ src, uint64_t count,
+static __global__ __launch_bounds__(256) void split_planes_kernel(const float* __restrict__ src, uint64_t count,
                                                            uint32_t* __restrict__ dst, uint64_t plane_words)
 {
     const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
@@ -276,7 +276,8 @@ __global__ __launch_bounds__(XW_THREADS) void gemm_x3w_kernel(GemmArgs g)
             multiply(L + XW_STAGE, 2);
             __syncthreads();
         }
-        finish_tile<EPI, XW_TM, TN, WN>(g, C, acc, cur.m0, cur.n0, wm, wn, l31, half);
+        if constexpr (EPI >= EPI_ADAPT_TANH) adapt_add<TN, WN>(g, acc, cur.m0, cur.n0, wm, wn, l31, half);
+        finish_tile<plain_epi(EPI), XW_TM, TN, WN>(g, C, acc, cur.m0, cur.n0, wm, wn, l31, half);
         if (!has_next) break;
         tile = next;
         cur = nxt;
@@ -458,7 +459,8 @@ __global__ __launch_bounds__(XW_THREADS) void gemm_f32w_kernel(GemmArgs g)
             fa.template stash<1>(L + FW_STAGE);
             fb.template stash<1>(L + FW_STAGE + FW_OPER);
         }
-        finish_tile<EPI, XW_TM, TN, WN>(g, C, acc, cur.m0, cur.n0, wm, wn, l31, half);
+        if constexpr (EPI >= EPI_ADAPT_TANH) adapt_add<TN, WN>(g, acc, cur.m0, cur.n0, wm, wn, l31, half);
+        finish_tile<plain_epi(EPI), XW_TM, TN, WN>(g, C, acc, cur.m0, cur.n0, wm, wn, l31, half);
         if (!has_next) break;
         tile = next;
         cur = nxt;

@@ -34,8 +34,16 @@ enum Epi {
     EPI_MUL_DRELU = 4,  // C = acc * (aux > 0)            (lib.rs:1039-1040)
     EPI_SLAB = 5,       // C[z] (+)= acc                  (split-K partial)
     EPI_BIAS_RELU_MASK = 6,  // EPI_BIAS_RELU, and bit (m % 32) of mask[m / 32][n] = (C > 0)
-    EPI_MUL_MASK = 7    // C = acc * bit of mask[m / 32][n]   (same product as EPI_MUL_DRELU)
+    EPI_MUL_MASK = 7,   // C = acc * bit of mask[m / 32][n]   (same product as EPI_MUL_DRELU)
+    // the same with the low-rank part of each row's adapter added to the product first (adapt_add)
+    EPI_ADAPT_TANH = 8,   // EPI_BIAS_TANH
+    EPI_ADAPT_BIAS = 9,   // EPI_BIAS
+    EPI_ADAPT_DTANH = 10  // EPI_MUL_DTANH
 };
+constexpr int plain_epi(int epi)
+{
+    return epi == EPI_ADAPT_TANH ? EPI_BIAS_TANH : epi == EPI_ADAPT_BIAS ? EPI_BIAS : epi == EPI_ADAPT_DTANH ? EPI_MUL_DTANH : epi;
+}
 
 struct GemmArgs {
     const float* A;
@@ -57,6 +65,14 @@ struct GemmArgs {
     uint64_t b_plane = 0;      // split-bf16 kernel: elements between the three planes of a pre-split B
     int tiles_x = 0, tiles_y = 0, tiles_z = 0;  // split-bf16 kernel: tiles along N, M and the K ranges
     uint64_t slab_stride = 0;  // split-bf16 kernel, EPI_SLAB: floats between the slabs of two K ranges (0: M * ldc)
+    // EPI_ADAPT_*: row m of the product gets low[m][0 .. rank) . U, U = the [rank][N] matrix at
+    // up + row_slot[m] * up_slot with element (k, n) at k * up_k + n * up_n; a negative slot adds nothing.
+    // ld_low is a multiple of 8 and columns from rank on hold zeros.
+    const float* low = nullptr;
+    const float* up = nullptr;
+    const int32_t* row_slot = nullptr;
+    uint64_t up_slot = 0;
+    int ld_low = 0, rank = 0, up_k = 0, up_n = 0;
 };
 
 struct Frag4 { float v[4]; };
@@ -298,6 +314,55 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& g, float* C, f32x16 
     store_tile<EPI, TM, TN, WN>(g, C, acc, m0, n0, wm, wn, l31, half);
 }
 
+// The low-rank part of each row's adapter on top of a finished product, before its epilogue.  Rows of one
+// call belong to different adapters ("slots"); they arrive sorted by slot, so nearly every 32-row MFMA tile
+// has one slot, and the others loop over the slots they hold.  Each slot's part is formed apart and added to
+// that slot's rows alone: zero factors for the other rows instead would let an inf or NaN in one request's
+// adapter reach its neighbours, and a row's sum would be rounded by the company it is in.
+// A step pairs k = st with st + ld_low / 2, so a lane's values of `low` are contiguous.
+template <int TN, int WN>
+__device__ __forceinline__ void adapt_add(const GemmArgs& g, f32x16 (&acc)[2][TN], int m0, int n0, int wm, int wn, int l31,
+                                          int half)
+{
+    const int steps = g.ld_low >> 1;  // a multiple of 4
+#pragma unroll
+    for (int tm = 0; tm < 2; ++tm) {
+        const int row = m0 + wm * 64 + tm * 32 + l31;
+        const int mine = row < g.M ? g.row_slot[row] : -1;
+        uint32_t left = (uint32_t)__ballot(mine >= 0);
+        const float* low = g.low + (size_t)min(row, g.M - 1) * g.ld_low + half * steps;
+        while (left) {
+            const int slot = __builtin_amdgcn_readlane(mine, __builtin_ctz(left));
+            const uint32_t member = (uint32_t)__ballot(mine == slot);
+            left &= ~member;
+            const uint32_t rows = member >> (4 * half);
+            const float* up = g.up + (size_t)slot * g.up_slot;
+#pragma unroll
+            for (int tn = 0; tn < TN; ++tn) {
+                const int col = min(n0 + wn * WN + tn * 32 + l31, g.N - 1);
+                const float* u = up + (size_t)col * g.up_n;
+                f32x16 c;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) c[r] = 0.0f;
+                for (int st = 0; st < steps; st += 4) {
+                    const float4 a4 = *reinterpret_cast<const float4*>(low + st);
+                    const float av[4] = {a4.x, a4.y, a4.z, a4.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int k = half * steps + st + j;
+                        float b = u[(size_t)min(k, g.rank - 1) * g.up_k];
+                        b = k < g.rank ? b : 0.0f;
+                        c = __builtin_amdgcn_mfma_f32_32x32x2f32(av[j], b, c, 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if ((rows >> ((r & 3) + 8 * (r >> 2))) & 1u) acc[tm][tn][r] += c[r];
+            }
+        }
+    }
+}
+
 // TAG only separates instantiations, so that each call site is its own kernel in a profile.
 // TM = rows of the block tile, KT = K tile (16 or 32), DB = double-buffered LDS tiles, BNT = columns
 // of the block tile (128; 256 for a k-major B under a 64-row tile: twice the matrix work between the
@@ -457,7 +522,8 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_kernel(GemmArgs g)
         }
     }
 
-    finish_tile<EPI, TM, TN, WN>(g, C, acc, m0, n0, wm, wn, l31, half);
+    if constexpr (EPI >= EPI_ADAPT_TANH) adapt_add<TN, WN>(g, acc, m0, n0, wm, wn, l31, half);
+    finish_tile<plain_epi(EPI), TM, TN, WN>(g, C, acc, m0, n0, wm, wn, l31, half);
 }
 
 

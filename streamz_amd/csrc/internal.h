@@ -112,6 +112,8 @@ struct Staging {
     size_t pinned_cap = 0;
 };
 
+struct Clip;
+
 struct Net {
     uint32_t in = 0, h1 = 0, h2 = 0, out = 0;
     float* d_params = nullptr;  // [w1|b1|w2|b2|w3|b3]
@@ -128,6 +130,9 @@ struct Net {
         void* buf[3] = {};       // features, two PCM staging buffers
         size_t cap[3] = {};
     } keep;
+    Clip* clip = nullptr;       // tables of szh_net_clip_grad_dev, made on its first call
+    const float* clip_of = nullptr;  // the gradient vector they were made for, and its length
+    uint64_t clip_len = 0;
     int device = 0;
     int gemm_mode = 0;          // SZH_GEMM_*: arithmetic of the large batched products
     // metadata carried by model.npz (lib.rs:755-761)
@@ -241,6 +246,102 @@ int net_stage_pinned(Net* n, size_t bytes, void** out);
 // host or a device pointer; counts_dev[out] / psums_dev[out] (either may be null) are added to.
 int identify_tiled(Net* n, Extractor* e, const int16_t* pcm, bool pcm_on_device, uint64_t n_samples, float threshold,
                    uint32_t tile_windows, unsigned long long* counts_dev, double* psums_dev);
+
+// ---- gradient clipping (clip.hip) ------------------------------------------------------
+struct ClipTensor { const float* src; float* dst; uint64_t len; uint32_t group; };
+struct ClipPiece { const float* src; float* dst; uint32_t len, group; };
+struct Clip {
+    ClipPiece* d_pieces = nullptr;  // ordered by group
+    double* d_part = nullptr;       // each piece's sum of squares
+    uint32_t* d_first = nullptr;    // [groups + 1] first piece of each group
+    uint32_t n_pieces = 0, groups = 0;
+    bool has_empty = false;         // a group without elements
+    const float* live = nullptr;    // the group's norm is that of its tensors divided by live[group * live_step]
+    uint32_t live_step = 1;
+    int device = 0;
+};
+int clip_create(const ClipTensor* tensors, uint32_t n, uint32_t groups, const float* live, uint32_t live_step, Clip** out);
+void clip_destroy(Clip* c);
+int clip_run(Clip* c, float max_norm, float* norms_dev, hipStream_t s);
+int net_clip(Net* n, float max_norm, float* norm_dev, hipStream_t s);
+
+// ---- controls on logits (control.hip) ----------------------------------------------------
+struct Controls {                 // device arrays, [sets][classes] unless noted; null = not used
+    const float* bias = nullptr;
+    const uint32_t* allow = nullptr;   // [sets][(classes + 31) / 32]
+    const uint32_t* counts = nullptr;
+    const float *repetition = nullptr, *presence = nullptr, *frequency = nullptr;  // [sets]
+    uint32_t sets = 0;                 // 0: no controls
+    const int32_t* set_of_row = nullptr;  // [rows]; null: set 0 for every row; outside [0, sets): the row has none
+};
+struct ControlRun {
+    const float* in = nullptr;  // [rows][ld_in] logits
+    uint64_t ld_in = 0, rows = 0;
+    uint32_t classes = 0;
+    const uint32_t* order = nullptr;  // place -> row (null: the same): rows of raw, out, set_of_row, labels and group
+    float* raw = nullptr;       // a copy of the logits
+    uint64_t ld_raw = 0;
+    float* out = nullptr;       // controlled logits or probabilities
+    uint64_t ld_out = 0;
+    bool probs = false;
+    // training (labels set): out, by place, becomes p - t, or zeros where the row does not count
+    const int32_t* labels = nullptr;
+    const uint8_t* row_live = nullptr;   // by place
+    const int32_t* row_slot = nullptr;   // by place
+    float* loss = nullptr;               // by place
+    uint8_t* live = nullptr;             // by place
+    // votes (votes set): the row's top class if its probability is >= threshold
+    float threshold = 0.0f;
+    const int32_t* group = nullptr;
+    uint32_t groups = 0;
+    unsigned long long* votes = nullptr; // [groups][classes], added to
+};
+int control_run(const Controls& ctl, const ControlRun& a, hipStream_t s);
+
+// ---- low-rank adapters (adapt.hip) ---------------------------------------------------------
+constexpr uint32_t kAdaptMaxSlots = 8192, kAdaptMaxRank = 64;
+struct AdaptWorkspace {
+    int ldx = 0, ld1 = 0, ld2 = 0, ld3 = 0, ldu = 0;  // row strides
+    uint32_t *order = nullptr, *begin = nullptr, *count = nullptr, *total = nullptr, *w2s = nullptr;
+    int32_t* row_slot = nullptr;
+    float *xs = nullptr, *h1 = nullptr, *h2 = nullptr, *lg = nullptr, *u2 = nullptr, *u3 = nullptr, *w1t = nullptr, *w2t = nullptr,
+          *w3t = nullptr, *d2 = nullptr, *g2 = nullptr, *g3 = nullptr, *loss = nullptr, *slab = nullptr;
+    uint8_t *live0 = nullptr, *live = nullptr;
+};
+struct Adapters {
+    uint32_t in = 0, h1 = 0, h2 = 0, out = 0, slots = 0, rank = 0;
+    float scale = 1.0f;
+    int device = 0;
+    float* d_params = nullptr;  // [slots][a2 | b2 | a3 | b3]
+    float* d_grad = nullptr;    // the same, then [slots]{loss, live rows}
+    double* d_sums = nullptr;   // [slots]{loss, live rows} since zero_grad
+    Clip* clip = nullptr;
+    AdaptWorkspace ws;
+    uint64_t ws_rows = 0;
+    bool ws_training = false;
+    std::vector<char*> arenas;  // the last one holds ws; earlier ones stay for graphs captured in them
+
+    uint64_t off_a2() const { return 0; }
+    uint64_t off_b2() const { return (uint64_t)h1 * rank; }
+    uint64_t off_a3() const { return off_b2() + (uint64_t)rank * h2; }
+    uint64_t off_b3() const { return off_a3() + (uint64_t)h2 * rank; }
+    uint64_t per_slot() const { return off_b3() + (uint64_t)rank * out; }
+};
+int adapters_create(const Net* n, uint32_t slots, uint32_t rank, float scale, const float* init, uint64_t seed, Adapters** out);
+void adapters_destroy(Adapters* a);
+int adapters_set_params(Adapters* a, uint32_t slot0, uint32_t count, const float* flat);
+int adapters_get_params(Adapters* a, uint32_t slot0, uint32_t count, float* flat);
+int adapters_reserve(Adapters* a, uint64_t rows, bool training);
+int adapters_forward(Net* n, Adapters* a, const float* x, const int32_t* slots_dev, uint64_t rows, const Controls& ctl, float* logits,
+                     float* probs, hipStream_t s);
+int adapters_vote(Net* n, Adapters* a, const float* x, const int32_t* slots_dev, uint64_t rows, const Controls& ctl, float threshold,
+                  const int32_t* group, uint32_t groups, unsigned long long* counts, hipStream_t s);
+int adapters_accumulate(Net* n, Adapters* a, const float* x, const int32_t* labels, const int32_t* slots_dev, uint64_t rows,
+                        const Controls& ctl, float dropout, uint64_t seed, hipStream_t s);
+int adapters_zero_grad(Adapters* a, hipStream_t s);
+int adapters_clip_tables(Adapters* a);
+int adapters_clip(Adapters* a, float max_norm, float* norms_dev, hipStream_t s);
+int adapters_apply(Adapters* a, float lr, hipStream_t s);
 
 // uniform in [-0.5, 0.5) from a counter-based generator; used for weight initialisation
 float init_uniform(uint64_t seed, uint64_t index);
