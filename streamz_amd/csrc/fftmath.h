@@ -10,7 +10,7 @@
 
 namespace sz {
 
-// One complex number = one 8-byte vector, so that complex add/sub map to packed f32 ops.
+// One complex number = one 8-byte vector.
 typedef float v2f __attribute__((vector_size(8)));
 
 SZ_HD v2f mk(float re, float im) { v2f r = {re, im}; return r; }
@@ -20,49 +20,15 @@ SZ_HD v2f conj(v2f a) { return mk(a[0], -a[1]); }
 SZ_HD v2f scale(v2f a, float s) { return mk(a[0] * s, a[1] * s); }
 
 #if defined(__HIP_DEVICE_COMPILE__)
-// On the device the operations that swap or negate one half of a complex number are written as
-// the packed instruction with its half-select (op_sel) and negate modifiers.  Left to itself the
-// compiler builds the swapped operand with a move and an exclusive-or first, and spends two
-// packed multiply-adds and a move on the second half of a complex product.  The roundings are
-// those of the expressions in the other branch with the product-sum contracted into one fma.
-SZ_HD v2f cmul(v2f a, v2f b)
-{
-    v2f t, r;
-    asm("v_pk_mul_f32 %0, %1, %2 op_sel:[1,1] op_sel_hi:[1,0]" : "=v"(t) : "v"(a), "v"(b));   // (a.im b.im, a.im b.re)
-    asm("v_pk_fma_f32 %0, %1, %2, %3 op_sel_hi:[0,1,1] neg_lo:[0,0,1]" : "=v"(r) : "v"(a), "v"(b), "v"(t));  // (a.re b.re - t.lo, a.re b.im + t.hi)
-    return r;
-}
-SZ_HD v2f add_negi(v2f a, v2f b)   // a + (-i) b = (a.re + b.im, a.im - b.re)
-{
-    v2f r;
-    asm("v_pk_add_f32 %0, %1, %2 op_sel:[0,1] op_sel_hi:[1,0] neg_hi:[0,1]" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
-SZ_HD v2f sub_negi(v2f a, v2f b)   // a - (-i) b = (a.re - b.im, a.im + b.re)
-{
-    v2f r;
-    asm("v_pk_add_f32 %0, %1, %2 op_sel:[0,1] op_sel_hi:[1,0] neg_lo:[0,1]" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
-SZ_HD v2f add_conj(v2f a, v2f b)   // a + conj(b)
-{
-    v2f r;
-    asm("v_pk_add_f32 %0, %1, %2 neg_hi:[0,1]" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
-SZ_HD v2f sub_conj(v2f a, v2f b)   // a - conj(b)
-{
-    v2f r;
-    asm("v_pk_add_f32 %0, %1, %2 neg_lo:[0,1]" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
+// On the device the product-sums are contracted into one fma each, by name.
+SZ_HD v2f cmul(v2f a, v2f b) { return mk(__builtin_fmaf(a[0], b[0], -(a[1] * b[1])), __builtin_fmaf(a[0], b[1], a[1] * b[0])); }
 #else
 SZ_HD v2f cmul(v2f a, v2f b) { return mk(a[0] * b[0] - a[1] * b[1], a[0] * b[1] + a[1] * b[0]); }
-SZ_HD v2f add_negi(v2f a, v2f b) { return a + mul_negi(b); }
-SZ_HD v2f sub_negi(v2f a, v2f b) { return a - mul_negi(b); }
-SZ_HD v2f add_conj(v2f a, v2f b) { return a + conj(b); }
-SZ_HD v2f sub_conj(v2f a, v2f b) { return a - conj(b); }
 #endif
+SZ_HD v2f add_negi(v2f a, v2f b) { return mk(a[0] + b[1], a[1] - b[0]); }  // a + (-i) b
+SZ_HD v2f sub_negi(v2f a, v2f b) { return mk(a[0] - b[1], a[1] + b[0]); }  // a - (-i) b
+SZ_HD v2f add_conj(v2f a, v2f b) { return mk(a[0] + b[0], a[1] - b[1]); }
+SZ_HD v2f sub_conj(v2f a, v2f b) { return mk(a[0] - b[0], a[1] + b[1]); }
 
 // 4-point DFT
 SZ_HD void dft4(v2f a, v2f b, v2f c, v2f d, v2f& y0, v2f& y1, v2f& y2, v2f& y3)
