@@ -6,6 +6,10 @@
 //   p = exp(z - max z) / sum exp(z - max z);  a row whose every z is -inf: p = 0
 //
 // A class outside the mask never enters the arithmetic (its logit may be inf or NaN).
+//
+// Bound by memory: logits, counts, biases and the result once each.  A row's controlled logits stay in registers
+// between the maximum, the sum and the result, so nothing is read twice up to kRowMax classes: some lanes of a
+// wave per row up to 1024 classes (control_rows_kernel), a workgroup per row beyond (control_row_kernel).
 #include <algorithm>
 
 #include "internal.h"
@@ -16,23 +20,29 @@ namespace sz {
 
 namespace {
 
+enum Mode { M_INFER = 0, M_TRAIN = 1, M_VOTE = 2 };
+
 struct RowControl {
     const float* bias;
     const uint32_t* allow;
     const uint32_t* counts;
-    float repetition, presence, frequency;
+    float repetition, inverse, presence, frequency;
 };
 
-__device__ __forceinline__ RowControl row_control(const Controls& c, int C, uint64_t row)
+__device__ __forceinline__ int32_t row_set(const Controls& c, uint64_t row)
 {
-    RowControl r{nullptr, nullptr, nullptr, 1.0f, 0.0f, 0.0f};
-    const int32_t set = c.sets == 0 ? -1 : c.set_of_row ? c.set_of_row[row] : 0;
+    return c.sets == 0 ? -1 : c.set_of_row ? c.set_of_row[row] : 0;
+}
+
+__device__ __forceinline__ RowControl row_control(const Controls& c, int C, int32_t set)
+{
+    RowControl r{nullptr, nullptr, nullptr, 1.0f, 1.0f, 0.0f, 0.0f};
     if (set < 0 || (uint32_t)set >= c.sets) return r;
     if (c.bias) r.bias = c.bias + (uint64_t)set * C;
     if (c.allow) r.allow = c.allow + (uint64_t)set * ((C + 31) / 32);
     if (c.counts) {
         r.counts = c.counts + (uint64_t)set * C;
-        if (c.repetition) r.repetition = c.repetition[set];
+        if (c.repetition) { r.repetition = c.repetition[set]; r.inverse = 1.0f / r.repetition; }
         if (c.presence) r.presence = c.presence[set];
         if (c.frequency) r.frequency = c.frequency[set];
     }
@@ -41,95 +51,403 @@ __device__ __forceinline__ RowControl row_control(const Controls& c, int C, uint
 
 __device__ __forceinline__ bool allowed(const RowControl& r, int c) { return !r.allow || ((r.allow[c >> 5] >> (c & 31)) & 1u); }
 
+// (the division by the repetition penalty is a product with its reciprocal: two roundings instead of one)
+__device__ __forceinline__ float penalised(const RowControl& r, float z, uint32_t count)
+{
+    const float n = (float)count;
+    const float seen = (z > 0.0f ? z * r.inverse : z * r.repetition) - r.presence;
+    return (n > 0.0f ? seen : z) - r.frequency * n;
+}
+
 __device__ __forceinline__ float controlled(const RowControl& r, float z, int c)
 {
-    if (r.counts) {
-        const float n = (float)r.counts[c];
-        if (n > 0.0f) z = (z > 0.0f ? z / r.repetition : z * r.repetition) - r.presence;
-        z -= r.frequency * n;
-    }
+    if (r.counts) z = penalised(r, z, r.counts[c]);
     if (r.bias) z += r.bias[c];
     return allowed(r, c) ? z : -INFINITY;
 }
 
-__device__ __forceinline__ float wave_max(float v)
+// e^x for x <= 0 (or NaN): 2^(x log2 e) by the hardware instruction with the rounding of the product, which would
+// cost |x| 2^-24, put back to first order.  0 below -200.
+__device__ __forceinline__ float exp_low(float x)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
-__device__ __forceinline__ float wave_sum(float v)
-{
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    const float kL = 1.44269502f, kR = 1.92596299e-8f, kLn2 = 0.693147182f;  // log2 e in two parts
+    const float y = x < -200.0f ? -200.0f : x;
+    const float t = y * kL;
+    const float r = __builtin_fmaf(y, kR, __builtin_fmaf(y, kL, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return __builtin_fmaf(e, r * kLn2, e);
 }
 
-// One wave per row, any number of classes.
-template <bool TRAIN>
-__global__ __launch_bounds__(256) void control_kernel(Controls ctl, ControlRun a)
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v)
 {
-    const int lane = threadIdx.x & 63;
-    const int C = (int)a.classes;
-    const uint64_t step = (uint64_t)gridDim.x * 4;
-    for (uint64_t i = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < a.rows; i += step) {
-        const uint64_t row = a.order ? a.order[i] : i;
-        const RowControl rc = row_control(ctl, C, row);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v)
+{
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+// the last of the largest values over the lanes: (p, c) pairs, c = -1 for none
+template <int LANES>
+__device__ __forceinline__ void lanes_best(float& p, int& c)
+{
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+        const float q = __shfl_xor(p, o);
+        const int b = __shfl_xor(c, o);
+        if (q > p || (q == p && b > c)) { p = q; c = b; }
+    }
+}
+
+// the vote of identify_speaker_list (lib.rs:1391-1402): the last maximum wins; a row without a candidate has none.
+// Counts are integers: the order of the additions is of no matter.
+__device__ __forceinline__ void cast_vote(const ControlRun& a, uint64_t row, int C, bool some, float p, int best)
+{
+    const int32_t g = a.group ? a.group[row] : 0;
+    if (some && best >= 0 && p >= a.threshold && g >= 0 && (uint32_t)g < a.groups) atomicAdd(&a.votes[(uint64_t)g * C + best], 1ull);
+}
+
+struct TrainRow { int label; bool live; };
+__device__ __forceinline__ TrainRow train_row(const ControlRun& a, const RowControl& rc, uint64_t i, uint64_t row, int C, bool some)
+{
+    TrainRow t;
+    t.label = a.labels[row];
+    t.live = a.row_live[i] && a.row_slot[i] >= 0 && t.label >= 0 && t.label < C && some && allowed(rc, t.label);
+    return t;
+}
+
+// LANES lanes of a wave per row, Q groups of four classes per lane: class 4 (l + LANES q) + e.  A row's logits
+// and the number of its set are asked for while the row before is worked on.
+template <int MODE, int LANES, int Q>
+__global__ __launch_bounds__(256) void control_rows_kernel(Controls ctl, ControlRun a, int vec_in, int vec_table, int vec_raw, int vec_out)
+{
+    constexpr int ROWS = 64 / LANES;
+    const int l = threadIdx.x % LANES, C = (int)a.classes;
+    const uint64_t base = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * ROWS, mine = (threadIdx.x & 63) / LANES;
+    const uint64_t step = (uint64_t)gridDim.x * 4 * ROWS;
+    float z[Q][4], next_z[Q][4];
+    uint64_t next_row = 0;
+    int32_t next_set = -1;
+    auto fetch = [&](uint64_t i0) {  // (lanes behind the last row take it again; they store nothing)
+        const uint64_t i = i0 < a.rows ? i0 : a.rows - 1;
+        next_row = a.order ? a.order[i] : i;
         const float* in = a.in + i * a.ld_in;
-        float top = -INFINITY;
-        for (int c = lane; c < C; c += 64) {
-            const float l = in[c];
-            if (!TRAIN && a.raw) a.raw[row * a.ld_raw + c] = l;
-            top = fmaxf(top, controlled(rc, l, c));
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const int c = 4 * (l + LANES * q);
+            if (vec_in && c < C) {
+                const float4 v = *reinterpret_cast<const float4*>(in + c);
+                next_z[q][0] = v.x; next_z[q][1] = v.y; next_z[q][2] = v.z; next_z[q][3] = v.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) next_z[q][e] = c + e < C ? in[c + e] : -INFINITY;
+            }
         }
-        if (!TRAIN && !a.out && !a.votes) continue;
-        top = wave_max(top);
-        if (!TRAIN && !a.probs && !a.votes) {
-            for (int c = lane; c < C; c += 64) a.out[row * a.ld_out + c] = controlled(rc, in[c], c);
-            continue;
+        next_set = row_set(ctl, next_row);
+    };
+    if (base < a.rows) fetch(base + mine);
+    for (uint64_t at = base; at < a.rows; at += step) {
+        const bool in_rows = at + mine < a.rows;
+        const uint64_t i = in_rows ? at + mine : a.rows - 1, row = next_row;
+        const RowControl rc = row_control(ctl, C, next_set);
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[q][e] = next_z[q][e];
+        if (at + step < a.rows) fetch(at + step + mine);
+        if (MODE == M_INFER && a.raw && in_rows) {
+            float* raw = a.raw + row * a.ld_raw;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                const int c = 4 * (l + LANES * q);
+                if (vec_raw && c < C) *reinterpret_cast<float4*>(raw + c) = make_float4(z[q][0], z[q][1], z[q][2], z[q][3]);
+                else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < C) raw[c + e] = z[q][e];
+                }
+            }
+            if (!a.out) continue;
         }
-        const float shift = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f;
-        for (int c = lane; c < C; c += 64) sum += expf(controlled(rc, in[c], c) - shift);
-        sum = wave_sum(sum);
-        const bool some = !(sum <= 0.0f);  // (a NaN row stays one)
-        if (!TRAIN && a.votes) {
-            // the vote of identify_speaker_list (lib.rs:1391-1402): the last maximum wins; a row without a
-            // candidate has none.  Counts are integers: the order of the additions is of no matter.
-            const int32_t g = a.group ? a.group[row] : 0;
-            int best = -1;
-            float bp = -1.0f;
-            for (int c = lane; c < C; c += 64) {
-                const float p = expf(controlled(rc, in[c], c) - shift) / sum;
-                if (p >= bp) { bp = p; best = c; }
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const int c = 4 * (l + LANES * q);
+            if (rc.counts) {
+                uint32_t n[4] = {0, 0, 0, 0};
+                if (vec_table && c < C) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(rc.counts + c);
+                    n[0] = v.x; n[1] = v.y; n[2] = v.z; n[3] = v.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < C) n[e] = rc.counts[c + e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[q][e] = penalised(rc, z[q][e], n[e]);
             }
-            for (int o = 32; o > 0; o >>= 1) {
-                const float q = __shfl_xor(bp, o);
-                const int b = __shfl_xor(best, o);
-                if (q > bp || (q == bp && b > best)) { bp = q; best = b; }
+            if (rc.bias) {
+                if (vec_table && c < C) {
+                    const float4 v = *reinterpret_cast<const float4*>(rc.bias + c);
+                    z[q][0] += v.x; z[q][1] += v.y; z[q][2] += v.z; z[q][3] += v.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < C) z[q][e] += rc.bias[c + e];
+                }
             }
-            if (lane == 0 && some && best >= 0 && bp >= a.threshold && g >= 0 && (uint32_t)g < a.groups)
-                atomicAdd(&a.votes[(uint64_t)g * C + best], 1ull);
-        } else if (!TRAIN) {
-            float* out = a.out + row * a.ld_out;
-            for (int c = lane; c < C; c += 64) out[c] = some ? expf(controlled(rc, in[c], c) - shift) / sum : 0.0f;
-        } else {
-            const int label = a.labels[row];
-            const bool live = a.row_live[i] && a.row_slot[i] >= 0 && label >= 0 && label < C && allowed(rc, label) && some;
-            float* out = a.out + i * a.ld_out;
-            float loss = 0.0f;
-            for (int c = lane; c < C; c += 64) {
-                const float p = expf(controlled(rc, in[c], c) - shift) / sum;
-                if (c == label) loss = -logf(fmaxf(p, 1e-12f));
-                out[c] = live ? (c == label ? p - 1.0f : p) : 0.0f;
+            const uint32_t bits = c < C ? (rc.allow ? rc.allow[c >> 5] >> (c & 31) : 15u) : 0u;  // four classes lie in one word
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[q][e] = c + e < C && ((bits >> e) & 1u) ? z[q][e] : -INFINITY;
+        }
+        if (MODE != M_INFER || a.probs) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) top = fmaxf(top, fmaxf(fmaxf(z[q][0], z[q][1]), fmaxf(z[q][2], z[q][3])));
+            top = lanes_max<LANES>(top);
+            const float shift = top == -INFINITY ? 0.0f : top;
+            float sum = 0.0f;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[q][e] = exp_low(z[q][e] - shift);
+                sum += (z[q][0] + z[q][1]) + (z[q][2] + z[q][3]);
             }
-            loss = wave_sum(loss);
-            if (lane == 0) {
-                a.loss[i] = live ? loss : 0.0f;
-                a.live[i] = live ? 1 : 0;
+            sum = lanes_sum<LANES>(sum);
+            const bool some = !(sum <= 0.0f);  // (a NaN row stays one)
+            const float inv = some ? 1.0f / sum : 0.0f;
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) z[q][e] *= inv;
+            if (MODE == M_VOTE) {
+                float bp = -1.0f;
+                int best = -1;
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int c = 4 * (l + LANES * q) + e;
+                        if (c < C && z[q][e] >= bp) { bp = z[q][e]; best = c; }
+                    }
+                lanes_best<LANES>(bp, best);
+                if (l == 0 && in_rows) cast_vote(a, row, C, some, bp, best);
+                continue;
+            }
+            if (MODE == M_TRAIN) {
+                const TrainRow t = train_row(a, rc, i, row, C, some);
+                float loss = 0.0f;
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (4 * (l + LANES * q) + e == t.label) {
+                            loss = -logf(fmaxf(z[q][e], 1e-12f));
+                            z[q][e] -= 1.0f;
+                        }
+                        if (!t.live) z[q][e] = 0.0f;
+                    }
+                loss = lanes_sum<LANES>(loss);
+                if (l == 0 && in_rows) {
+                    a.loss[i] = t.live ? loss : 0.0f;
+                    a.live[i] = t.live ? 1 : 0;
+                }
+            }
+        }
+        if (!in_rows) continue;
+        float* out = a.out + (MODE == M_TRAIN ? i : row) * a.ld_out;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const int c = 4 * (l + LANES * q);
+            if (vec_out && c < C) *reinterpret_cast<float4*>(out + c) = make_float4(z[q][0], z[q][1], z[q][2], z[q][3]);
+            else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < C) out[c + e] = z[q][e];
             }
         }
     }
+}
+
+constexpr int kRowThreads = 1024, kRowMax = 50 * kRowThreads;
+
+// joins a value of every wave
+template <class F>
+__device__ __forceinline__ float join_waves(float v, float* part, F f)
+{
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float r = part[0];
+#pragma unroll
+    for (int w = 1; w < kRowThreads / 64; ++w) r = f(r, part[w]);
+    return r;
+}
+
+// The thread's index, which the compiler takes for a new value: what it computes from it (offsets and bounds of
+// every class) is not kept in registers from one use to the next.
+__device__ __forceinline__ uint32_t fresh_thread()
+{
+    uint32_t t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
+// One workgroup per row, V values per thread in registers (class t + 1024 q: whole lines whatever the row's
+// alignment); V = 0: any number of classes, the row read twice more (out of the caches, mostly).
+template <int MODE, int V>
+__global__ __launch_bounds__(kRowThreads) void control_row_kernel(Controls ctl, ControlRun a, uint64_t first)
+{
+    __shared__ float part[kRowThreads / 64];
+    __shared__ int part_c[kRowThreads / 64];
+    const int C = (int)a.classes;
+    const int n_mine = ((int)C - (int)threadIdx.x + kRowThreads - 1) / kRowThreads;
+    const uint64_t i = first + blockIdx.x;
+    const uint64_t row = a.order ? (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)a.order[i]) : i;
+    const RowControl rc = row_control(ctl, C, __builtin_amdgcn_readfirstlane(row_set(ctl, row)));  // (addresses in scalar registers)
+    const float* in = a.in + i * a.ld_in;
+    float* raw = MODE == M_INFER && a.raw ? a.raw + row * a.ld_raw : nullptr;
+    float* out = a.out ? a.out + (MODE == M_TRAIN ? i : row) * a.ld_out : nullptr;
+    // a thread goes through its values some at a time: their loads are all in flight, and what a step needs beside
+    // them does not take V registers more
+    constexpr int STEP = V % 10 == 0 && V ? 10 : V < 8 ? (V ? V : 1) : 8;
+    float z[V ? V : 1];
+    auto each = [&](auto f) {   // f(value, class) over the thread's classes
+        if (V) {
+#pragma unroll
+            for (int q0 = 0; q0 < V; q0 += STEP) {
+                const uint32_t t = fresh_thread();
+#pragma unroll
+                for (int q = q0; q < q0 + STEP; ++q)
+                    if (t + (uint32_t)(kRowThreads * q) < (uint32_t)C) f(z[q % (V ? V : 1)], t + (uint32_t)(kRowThreads * q));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+#pragma unroll 4
+            for (int q = 0; q < n_mine; ++q) {
+                const int c = threadIdx.x + kRowThreads * q;
+                float v = controlled(rc, in[c], c);
+                f(v, c);
+            }
+        }
+    };
+    if (raw) {
+#pragma unroll 4
+        for (int c = threadIdx.x; c < C; c += kRowThreads) raw[c] = in[c];
+        if (!out) return;
+    }
+    if (V) {
+#pragma unroll
+        for (int q0 = 0; q0 < V; q0 += STEP) {
+            const uint32_t t = fresh_thread();
+            // (tables that are not used count as zeros and ones: no branches between the loads and their use)
+            uint32_t n[STEP], w[STEP];
+            float h[STEP];
+#pragma unroll
+            for (int q = 0; q < STEP; ++q) {
+                const uint32_t c = min(t + (uint32_t)(kRowThreads * (q0 + q)), (uint32_t)C - 1);
+                z[(q0 + q) % (V ? V : 1)] = in[c];
+                n[q] = 0; w[q] = ~0u; h[q] = 0.0f;
+            }
+            if (rc.counts) {
+#pragma unroll
+                for (int q = 0; q < STEP; ++q) n[q] = rc.counts[min(t + (uint32_t)(kRowThreads * (q0 + q)), (uint32_t)C - 1)];
+            }
+            if (rc.bias) {
+#pragma unroll
+                for (int q = 0; q < STEP; ++q) h[q] = rc.bias[min(t + (uint32_t)(kRowThreads * (q0 + q)), (uint32_t)C - 1)];
+            }
+            if (rc.allow) {
+#pragma unroll
+                for (int q = 0; q < STEP; ++q) w[q] = rc.allow[min(t + (uint32_t)(kRowThreads * (q0 + q)), (uint32_t)C - 1) >> 5];
+            }
+#pragma unroll
+            for (int q = 0; q < STEP; ++q) {
+                const float v = penalised(rc, z[(q0 + q) % (V ? V : 1)], n[q]) + h[q];
+                const bool on = t + (uint32_t)(kRowThreads * (q0 + q)) < (uint32_t)C && ((w[q] >> (t & 31)) & 1u);
+                z[(q0 + q) % (V ? V : 1)] = on ? v : -INFINITY;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    if (MODE == M_INFER && !a.probs) {
+        each([&](float& v, uint32_t c) { out[c] = v; });
+        return;
+    }
+    float top = -INFINITY;
+    each([&](float& v, uint32_t) { top = fmaxf(top, v); });
+    top = join_waves(lanes_max<64>(top), part, [](float x, float y) { return fmaxf(x, y); });
+    const float shift = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    each([&](float& v, uint32_t) { v = exp_low(v - shift); sum += v; });
+    sum = join_waves(lanes_sum<64>(sum), part, [](float x, float y) { return x + y; });
+    const bool some = !(sum <= 0.0f);
+    const float inv = some ? 1.0f / sum : 0.0f;
+    // (without registers the values come again as controlled logits)
+    auto prob = [&](float v) { return (V ? v : exp_low(v - shift)) * inv; };
+    if (MODE == M_VOTE) {
+        float bp = -1.0f;
+        int best = -1;
+        each([&](float& v, uint32_t c) { const float p = prob(v); if (p >= bp) { bp = p; best = (int)c; } });
+        lanes_best<64>(bp, best);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) { part[threadIdx.x >> 6] = bp; part_c[threadIdx.x >> 6] = best; }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < kRowThreads / 64; ++w)
+                if (part[w] > bp || (part[w] == bp && part_c[w] > best)) { bp = part[w]; best = part_c[w]; }
+            cast_vote(a, row, C, some, bp, best);
+        }
+    } else if (MODE == M_INFER) {
+        each([&](float& v, uint32_t c) { out[c] = prob(v); });
+    } else {
+        const TrainRow t = train_row(a, rc, i, row, C, some);
+        if (threadIdx.x == 0 && !(t.label >= 0 && t.label < C)) { a.loss[i] = 0.0f; a.live[i] = 0; }
+        each([&](float& v, uint32_t c) {
+            const float p = prob(v);
+            if ((int)c == t.label) { a.loss[i] = t.live ? -logf(fmaxf(p, 1e-12f)) : 0.0f; a.live[i] = t.live ? 1 : 0; }
+            out[c] = t.live ? ((int)c == t.label ? p - 1.0f : p) : 0.0f;
+        });
+    }
+}
+
+template <int MODE>
+int launch(const Controls& ctl, const ControlRun& a, hipStream_t s)
+{
+    const uint32_t C = a.classes;
+    const auto vec = [&](const void* p, uint64_t ld) { return C % 4 == 0 && ld % 4 == 0 && ((uintptr_t)p & 15) == 0 ? 1 : 0; };
+    const int vi = vec(a.in, a.ld_in), vt = vec(ctl.bias, C) && vec(ctl.counts, C), vr = vec(a.raw, a.ld_raw), vo = vec(a.out, a.ld_out);
+#define SZ_ROWS(LANES, Q)                                                                                                       \
+    hipLaunchKernelGGL((control_rows_kernel<MODE, LANES, Q>), dim3((unsigned)std::min<uint64_t>((a.rows * (LANES) + 255) / 256, 8192)), \
+                       dim3(256), 0, s, ctl, a, vi, vt, vr, vo)
+    // (a launch has fewer than 2^32 threads)
+#define SZ_ROW(V)                                                                                                               \
+    for (uint64_t r = 0; r < a.rows; r += 1u << 20)                                                                             \
+        hipLaunchKernelGGL((control_row_kernel<MODE, V>), dim3((unsigned)std::min<uint64_t>(a.rows - r, 1u << 20)), dim3(kRowThreads), 0, s, ctl, a, r)
+    if (C <= 4) SZ_ROWS(1, 1);
+    else if (C <= 8) SZ_ROWS(2, 1);
+    else if (C <= 16) SZ_ROWS(4, 1);
+    else if (C <= 32) SZ_ROWS(8, 1);
+    else if (C <= 64) SZ_ROWS(16, 1);
+    else if (C <= 128) SZ_ROWS(32, 1);
+    else if (C <= 256) SZ_ROWS(64, 1);
+    else if (C <= 512) SZ_ROWS(64, 2);
+    else if (C <= 1024) SZ_ROWS(64, 4);
+    else if (C <= 2 * kRowThreads) SZ_ROW(2);
+    else if (C <= 4 * kRowThreads) SZ_ROW(4);
+    else if (C <= 8 * kRowThreads) SZ_ROW(8);
+    else if (C <= 16 * kRowThreads) SZ_ROW(16);
+    else if (C <= 32 * kRowThreads) SZ_ROW(32);
+    else if (C <= kRowMax) SZ_ROW(50);
+    else SZ_ROW(0);
+#undef SZ_ROWS
+#undef SZ_ROW
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
 }
 
 }  // namespace
@@ -138,11 +456,7 @@ int control_run(const Controls& ctl, const ControlRun& a, hipStream_t s)
 {
     if (a.rows == 0 || a.classes == 0) return SZH_OK;
     ProfScope prof(a.labels ? "control_loss" : "control", s);
-    const unsigned blocks = (unsigned)std::min<uint64_t>((a.rows + 3) / 4, 8192);
-    if (a.labels) hipLaunchKernelGGL((control_kernel<true>), dim3(blocks), dim3(256), 0, s, ctl, a);
-    else hipLaunchKernelGGL((control_kernel<false>), dim3(blocks), dim3(256), 0, s, ctl, a);
-    SZ_HIP(hipGetLastError());
-    return SZH_OK;
+    return a.labels ? launch<M_TRAIN>(ctl, a, s) : a.votes ? launch<M_VOTE>(ctl, a, s) : launch<M_INFER>(ctl, a, s);
 }
 
 }  // namespace sz
