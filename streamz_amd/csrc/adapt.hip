@@ -22,6 +22,7 @@
 #include <vector>
 
 #include "adapt_kernel.h"
+#include "adapt_rows.h"
 #include "gemm_launch.h"
 #include "internal.h"
 #include "prof.h"
@@ -35,6 +36,9 @@ using namespace adapt;
 
 // Rows per pass: a call with more is walked in pieces, whose workspace does not grow with it.
 constexpr uint64_t kAdaptRows = 131072;
+
+// Calls of up to this many rows go row by row (adapt_rows.h).
+constexpr uint64_t kFewRows = 512;
 
 inline int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
@@ -62,12 +66,13 @@ size_t lay_out(const Adapters* a, uint64_t rows, bool training, char* base, Adap
     take(o.xs, rows * o.ldx); take(o.live0, rows); take(o.live, rows);
     take(o.h1, (rows + 32) * o.ld1); take(o.h2, (rows + 32) * o.ld2); take(o.lg, (rows + 32) * o.ld3);
     take(o.u2, rows * o.ldu); take(o.u3, rows * o.ldu);
+    take(o.add2, kFewRows * o.ld2); take(o.add3, kFewRows * o.ld3);
     take(o.w1t, (uint64_t)a->h1 * o.ldx); take(o.w2t, (uint64_t)a->h1 * a->h2); take(o.w3t, (uint64_t)a->h2 * a->out + 1);
     take(o.w2s, 3 * ((uint64_t)a->h1 * a->h2 + 1) / 2 + 4);
     if (training) {
         const uint64_t chunks = (rows + kFactorRows - 1) / kFactorRows;
         take(o.d2, (rows + 32) * o.ld2); take(o.g2, rows * o.ldu); take(o.g3, rows * o.ldu); take(o.loss, rows);
-        take(o.slab, (chunks + S) * std::max({a->h1, a->h2, a->out}) * a->rank);
+        take(o.slab, (chunks + S) * a->per_slot());
     }
     return at;
 }
@@ -107,6 +112,11 @@ int group_rows(Adapters* a, const int32_t* slots_dev, uint32_t rows, hipStream_t
     const int S = (int)a->slots, blocks = (int)((rows + kGroupRows - 1) / kGroupRows);
     const size_t lds = (S + 1) * sizeof(uint32_t);
     ProfScope prof("adapt_group", s);
+    if (blocks == 1) {
+        hipLaunchKernelGGL(group_few_kernel, dim3(1), dim3(64), lds, s, slots_dev, rows, S, w.begin, w.order, w.row_slot);
+        SZ_HIP(hipGetLastError());
+        return SZH_OK;
+    }
     hipLaunchKernelGGL(group_count_kernel, dim3(blocks), dim3(64), lds, s, slots_dev, rows, S, blocks, w.count);
     hipLaunchKernelGGL(group_scan_kernel, dim3(S + 1), dim3(64), 0, s, w.count, blocks, w.total);
     hipLaunchKernelGGL(group_begin_kernel, dim3(1), dim3(64), 0, s, w.total, S, rows, w.begin);
@@ -134,22 +144,35 @@ int low_product(const Adapters* a, const float* x, int ldx, int K, const float* 
     return SZH_OK;
 }
 
-// grad[slot] at `off` += sum over the slot's rows of p[i][m] w[i][j], element (m, j) at m * g_m + j * g_j
-int factor_gradient(Adapters* a, const float* p, int ldp, int M, const float* w, uint32_t rows, uint64_t off, int g_m, int g_j, hipStream_t s)
+// the gradients of a pass's four factors, added to the bank's
+int factor_gradients(Adapters* a, uint32_t rows, hipStream_t s)
 {
+    const AdaptWorkspace& w = a->ws;
+    const int h1 = (int)a->h1, h2 = (int)a->h2, out = (int)a->out, r = (int)a->rank;
     FactorArgs g{};
-    g.p = p; g.ldp = ldp; g.M = M; g.w = w; g.ldw = a->ws.ldu; g.rank = (int)a->rank; g.slots = (int)a->slots;
-    g.begin = a->ws.begin; g.row_slot = a->ws.row_slot; g.slab = a->ws.slab;
-    const dim3 grid((M + 63) / 64, (rows + kFactorRows - 1) / kFactorRows), block(256);
+    g.ldw = w.ldu; g.rank = r; g.slots = (int)a->slots; g.begin = w.begin; g.row_slot = w.row_slot;
+    g.job[0] = {w.h1, w.g2, nullptr, a->off_a2(), w.ld1, h1, r, 1, 0, 0};
+    g.job[1] = {w.d2, w.u2, nullptr, a->off_b2(), w.ld2, h2, 1, h2, 0, 0};
+    g.job[2] = {w.h2, w.g3, nullptr, a->off_a3(), w.ld2, h2, r, 1, 0, 0};
+    g.job[3] = {w.lg, w.u3, nullptr, a->off_b3(), w.ld3, out, 1, out, 0, 0};
+    const uint64_t chunks = (rows + kFactorRows - 1) / kFactorRows;
+    float* slab = w.slab;
+    int tiles = 0, blocks = 0;
+    for (FactorJob& j : g.job) {
+        j.first = tiles; j.first_out = blocks; j.slab = slab;
+        tiles += (j.M + 63) / 64;
+        blocks += (j.M * r + 255) / 256;
+        slab += (chunks + a->slots) * (uint64_t)j.M * r;
+    }
+    const dim3 grid(tiles, (unsigned)chunks), block(256);
     ProfScope prof("adapt_grad", s);
-    switch ((a->rank + 15) / 16) {
+    switch ((r + 15) / 16) {
     case 1: hipLaunchKernelGGL((factor_grad_kernel<1>), grid, block, 0, s, g); break;
     case 2: hipLaunchKernelGGL((factor_grad_kernel<2>), grid, block, 0, s, g); break;
     case 3: hipLaunchKernelGGL((factor_grad_kernel<3>), grid, block, 0, s, g); break;
     default: hipLaunchKernelGGL((factor_grad_kernel<4>), grid, block, 0, s, g); break;
     }
-    hipLaunchKernelGGL(factor_reduce_kernel, dim3((M * a->rank + 255) / 256, a->slots), block, 0, s, g.slab, g.begin, M, g.rank, g_m, g_j,
-                       a->d_grad + off, a->per_slot());
+    hipLaunchKernelGGL(factor_reduce_kernel, dim3(blocks, a->slots), block, 0, s, g, a->d_grad, a->per_slot());
     SZ_HIP(hipGetLastError());
     return SZH_OK;
 }
@@ -219,6 +242,81 @@ int forward_rows(Net* n, Adapters* a, uint32_t rows, hipStream_t s)
     return launch_gemm<A_ROWS, B_KROWS, EPI_ADAPT_BIAS, T_ADAPT3>(g, 1, s);
 }
 
+// Whether a call takes the few-row path: its row kernels hold a row's activations in LDS.
+bool few_rows(const Net* n, uint64_t rows)
+{
+    return rows <= kFewRows && n->in + n->h1 + 2 * n->h2 + n->out <= 24576;
+}
+
+// w3 beyond this is not streamed by every row: the logits become a product of their own
+constexpr uint64_t kRowOutFloats = 65536;
+
+RowArgs row_args(const Net* n, Adapters* a, const float* x, uint64_t ldx, const int32_t* slot)
+{
+    const AdaptWorkspace& w = a->ws;
+    const float* P = n->d_params;
+    RowArgs g{};
+    g.x = x; g.ldx = ldx; g.w1 = P + n->off_w1(); g.b1 = P + n->off_b1(); g.w3 = P + n->off_w3(); g.b3 = P + n->off_b3();
+    g.factors = a->d_params; g.per_slot = a->per_slot();
+    g.off_a2 = a->off_a2(); g.off_b2 = a->off_b2(); g.off_a3 = a->off_a3(); g.off_b3 = a->off_b3();
+    g.slot = slot; g.slots = (int)a->slots; g.in = (int)n->in; g.n1 = (int)n->h1; g.n2 = (int)n->h2; g.out = (int)n->out;
+    g.rank = (int)a->rank; g.ldu = w.ldu; g.ld1 = w.ld1; g.ld2 = w.ld2; g.ld3 = w.ld3; g.scale = a->scale;
+    g.h1 = w.h1; g.h2 = w.h2; g.add2 = w.add2; g.add3 = w.add3;
+    return g;
+}
+
+template <bool TANH>
+int thin_product(const float* A, int lda, int K, const float* W, const float* add, int ldadd, const float* bias, float* C, int ldc, int N,
+                 uint32_t rows, const char* tag, hipStream_t s)
+{
+    ThinArgs g{};
+    g.A = A; g.lda = lda; g.W = W; g.add = add; g.ldadd = ldadd; g.bias = bias; g.C = C; g.ldc = ldc; g.M = (int)rows; g.N = N; g.K = K;
+    ProfScope prof(tag, s);
+    hipLaunchKernelGGL((thin_kernel<TANH>), dim3((N + 31) / 32, (rows + 31) / 32), dim3(64 * kThinWaves), 0, s, g);
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
+}
+
+template <int OUT>
+int launch_row_out(const RowArgs& g, const Controls& ctl, const ControlRun& c, uint32_t rows, hipStream_t s)
+{
+    const size_t lds = (kRowPart + 2 * g.n2 + 64 + g.out) * sizeof(float);
+    if (int rc = allow_dynamic_lds((const void*)row_out_kernel<OUT>, lds)) return rc;
+    ProfScope prof("adapt_row_out", s);
+    hipLaunchKernelGGL((row_out_kernel<OUT>), dim3(rows), dim3(kRowT), lds, s, g, ctl, c);
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
+}
+
+// The call of few rows, in the caller's order; c holds what it wants of the logits (by row).
+int forward_few(Net* n, Adapters* a, const float* x, uint64_t ldx, const int32_t* slot, uint32_t rows, const Controls& ctl, const ControlRun& c,
+                float* u2, float* u3, hipStream_t s)
+{
+    AdaptWorkspace& w = a->ws;
+    const float* P = n->d_params;
+    RowArgs g = row_args(n, a, x, ldx, slot);
+    g.u2 = u2; g.u3 = u3;
+    const size_t lds = (kRowPart + g.n1 + 64 + g.in) * sizeof(float);
+    if (int rc = allow_dynamic_lds((const void*)row_hidden_kernel, lds)) return rc;
+    {
+        ProfScope prof("adapt_row_h1", s);
+        hipLaunchKernelGGL(row_hidden_kernel, dim3(rows), dim3(kRowT), lds, s, g);
+        SZ_HIP(hipGetLastError());
+    }
+    int rc = thin_product<true>(w.h1, w.ld1, (int)n->h1, P + n->off_w2(), w.add2, w.ld2, P + n->off_b2(), w.h2, w.ld2, (int)n->h2, rows,
+                                "adapt_h2", s);
+    if (rc) return rc;
+    const bool train = c.labels != nullptr;
+    if ((uint64_t)n->h2 * n->out <= kRowOutFloats) {
+        if (train) { g.g2 = w.g2; g.g3 = w.g3; g.d2 = w.d2; g.d3 = w.lg; return launch_row_out<OUT_TRAIN>(g, ctl, c, rows, s); }
+        return launch_row_out<OUT_INFER>(g, ctl, c, rows, s);
+    }
+    rc = launch_row_out<OUT_ADD>(g, ctl, c, rows, s);
+    if (!rc) rc = thin_product<false>(w.h2, w.ld2, (int)n->h2, P + n->off_w3(), w.add3, w.ld3, P + n->off_b3(), w.lg, w.ld3, (int)n->out, rows,
+                                      "adapt_out", s);
+    return rc ? rc : control_run(ctl, c, s);
+}
+
 int gather_rows(Adapters* a, const float* x, uint32_t rows, float dropout, uint64_t seed, uint64_t counter0, uint8_t* live, hipStream_t s)
 {
     ProfScope prof("prep", s);
@@ -234,6 +332,17 @@ Controls from_row(const Controls& c, uint64_t r0)
     Controls d = c;
     if (d.set_of_row) d.set_of_row += r0;
     return d;
+}
+
+// one pass of a forward or vote call
+int infer_rows(Net* n, Adapters* a, const float* x, const int32_t* slots_dev, uint32_t rows, const Controls& ctl, ControlRun c, hipStream_t s)
+{
+    if (few_rows(n, rows)) return forward_few(n, a, x, n->in, slots_dev, rows, ctl, c, nullptr, nullptr, s);
+    int rc = group_rows(a, slots_dev, rows, s);
+    if (!rc) rc = gather_rows(a, x, rows, 0.0f, 0, 0, nullptr, s);
+    if (!rc) rc = forward_rows(n, a, rows, s);
+    c.order = a->ws.order;
+    return rc ? rc : control_run(ctl, c, s);
 }
 
 }  // namespace
@@ -313,16 +422,11 @@ int adapters_forward(Net* n, Adapters* a, const float* x, const int32_t* slots_d
     if (int rc = ensure(a, rows, false, s)) return rc;
     for (uint64_t r0 = 0; r0 < rows; r0 += kAdaptRows) {
         const uint32_t R = (uint32_t)std::min<uint64_t>(kAdaptRows, rows - r0);
-        int rc = group_rows(a, slots_dev ? slots_dev + r0 : nullptr, R, s);
-        if (!rc) rc = gather_rows(a, x + r0 * n->in, R, 0.0f, 0, 0, nullptr, s);
-        if (!rc) rc = forward_rows(n, a, R, s);
-        if (rc) return rc;
         ControlRun c{};
-        c.in = a->ws.lg; c.ld_in = a->ws.ld3; c.rows = R; c.classes = n->out; c.order = a->ws.order;
+        c.in = a->ws.lg; c.ld_in = a->ws.ld3; c.rows = R; c.classes = n->out;
         c.raw = logits ? logits + r0 * n->out : nullptr; c.ld_raw = n->out;
         c.out = probs ? probs + r0 * n->out : nullptr; c.ld_out = n->out; c.probs = true;
-        rc = control_run(from_row(ctl, r0), c, s);
-        if (rc) return rc;
+        if (int rc = infer_rows(n, a, x + r0 * n->in, slots_dev + r0, R, from_row(ctl, r0), c, s)) return rc;
     }
     return SZH_OK;
 }
@@ -335,15 +439,10 @@ int adapters_vote(Net* n, Adapters* a, const float* x, const int32_t* slots_dev,
     if (int rc = ensure(a, rows, false, s)) return rc;
     for (uint64_t r0 = 0; r0 < rows; r0 += kAdaptRows) {
         const uint32_t R = (uint32_t)std::min<uint64_t>(kAdaptRows, rows - r0);
-        int rc = group_rows(a, slots_dev ? slots_dev + r0 : nullptr, R, s);
-        if (!rc) rc = gather_rows(a, x + r0 * n->in, R, 0.0f, 0, 0, nullptr, s);
-        if (!rc) rc = forward_rows(n, a, R, s);
-        if (rc) return rc;
         ControlRun c{};
-        c.in = a->ws.lg; c.ld_in = a->ws.ld3; c.rows = R; c.classes = n->out; c.order = a->ws.order;
+        c.in = a->ws.lg; c.ld_in = a->ws.ld3; c.rows = R; c.classes = n->out;
         c.threshold = threshold; c.group = group ? group + r0 : nullptr; c.groups = groups; c.votes = counts;
-        rc = control_run(from_row(ctl, r0), c, s);
-        if (rc) return rc;
+        if (int rc = infer_rows(n, a, x + r0 * n->in, slots_dev + r0, R, from_row(ctl, r0), c, s)) return rc;
     }
     return SZH_OK;
 }
@@ -356,30 +455,32 @@ int adapters_accumulate(Net* n, Adapters* a, const float* x, const int32_t* labe
     if (int rc = ensure(a, rows, true, s)) return rc;
     AdaptWorkspace& w = a->ws;
     const float* F = a->d_params;
-    const int r = (int)a->rank, h1 = (int)n->h1, h2 = (int)n->h2, out = (int)n->out;
+    const int r = (int)a->rank, h2 = (int)n->h2, out = (int)n->out;
     for (uint64_t r0 = 0; r0 < rows; r0 += kAdaptRows) {
         const uint32_t R = (uint32_t)std::min<uint64_t>(kAdaptRows, rows - r0);
         int rc = group_rows(a, slots_dev + r0, R, s);
         if (!rc) rc = gather_rows(a, x + r0 * n->in, R, dropout, seed, r0, w.live0, s);
-        if (!rc) rc = forward_rows(n, a, R, s);
-        if (rc) return rc;
         ControlRun c{};
         c.in = w.lg; c.ld_in = w.ld3; c.rows = R; c.classes = n->out; c.order = w.order;
         c.out = w.lg; c.ld_out = w.ld3; c.labels = labels + r0; c.row_live = w.live0; c.row_slot = w.row_slot; c.loss = w.loss; c.live = w.live;
-        rc = control_run(from_row(ctl, r0), c, s);   // lg now holds d3
+        const Controls ctl_r = from_row(ctl, r0);
+        const bool few = few_rows(n, R);
+        if (!rc && few) rc = forward_few(n, a, w.xs, w.ldx, w.row_slot, R, ctl_r, c, w.u2, w.u3, s);
+        if (!rc && !few) rc = forward_rows(n, a, R, s);
+        if (!rc && !few) rc = control_run(ctl_r, c, s);   // lg now holds d3
         if (rc) return rc;
-        rc = low_product(a, w.lg, w.ld3, out, F + a->off_b3(), 1, out, R, w.g3, s);
-        if (rc) return rc;
-        GemmArgs g{};
-        g.A = w.lg; g.lda = w.ld3; g.B = n->d_params + n->off_w3(); g.ldb = out; g.C = w.d2; g.ldc = w.ld2;
-        g.M = (int)R; g.N = h2; g.K = g.k_chunk = out; g.aux = w.h2; g.ldaux = w.ld2;
-        adapt_args(g, a, w.g3, F + a->off_a3(), 1, r);
-        rc = launch_gemm<A_ROWS, B_ROWS, EPI_ADAPT_DTANH, T_ADAPT_D2>(g, 1, s);
-        if (!rc) rc = low_product(a, w.d2, w.ld2, h2, F + a->off_b2(), 1, h2, R, w.g2, s);
-        if (!rc) rc = factor_gradient(a, w.h1, w.ld1, h1, w.g2, R, a->off_a2(), r, 1, s);
-        if (!rc) rc = factor_gradient(a, w.d2, w.ld2, h2, w.u2, R, a->off_b2(), 1, h2, s);
-        if (!rc) rc = factor_gradient(a, w.h2, w.ld2, h2, w.g3, R, a->off_a3(), r, 1, s);
-        if (!rc) rc = factor_gradient(a, w.lg, w.ld3, out, w.u3, R, a->off_b3(), 1, out, s);
+        if (!few || (uint64_t)n->h2 * n->out > kRowOutFloats) {
+            rc = low_product(a, w.lg, w.ld3, out, F + a->off_b3(), 1, out, R, w.g3, s);
+            if (rc) return rc;
+            GemmArgs g{};
+            g.A = w.lg; g.lda = w.ld3; g.B = n->d_params + n->off_w3(); g.ldb = out; g.C = w.d2; g.ldc = w.ld2;
+            g.M = (int)R; g.N = h2; g.K = g.k_chunk = out; g.aux = w.h2; g.ldaux = w.ld2;
+            adapt_args(g, a, w.g3, F + a->off_a3(), 1, r);
+            rc = launch_gemm<A_ROWS, B_ROWS, EPI_ADAPT_DTANH, T_ADAPT_D2>(g, 1, s);
+            if (!rc) rc = low_product(a, w.d2, w.ld2, h2, F + a->off_b2(), 1, h2, R, w.g2, s);
+            if (rc) return rc;
+        }
+        rc = factor_gradients(a, R, s);
         if (rc) return rc;
         hipLaunchKernelGGL(slot_stats_kernel, dim3(a->slots), dim3(256), 0, s, w.loss, w.live, w.begin, a->d_sums,
                            a->d_grad + a->per_slot() * a->slots);

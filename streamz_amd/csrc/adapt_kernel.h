@@ -46,13 +46,7 @@ __global__ __launch_bounds__(64) void group_count_kernel(const int32_t* __restri
     for (int k = threadIdx.x; k <= slots; k += 64) hist[k] = 0;
     __syncthreads();
     const uint32_t r0 = blockIdx.x * kGroupRows, r1 = min(rows, r0 + kGroupRows);
-    for (uint32_t r = r0; r < r1; r += 64) {
-        const bool in = r + threadIdx.x < r1;
-        const int key = in ? group_key(slot, r + threadIdx.x, slots) : 0;
-        each_key(key, in, [&](int k, unsigned long long member) {
-            if (threadIdx.x == 0) hist[k] += (uint32_t)__popcll(member);
-        });
-    }
+    for (uint32_t r = r0 + threadIdx.x; r < r1; r += 64) atomicAdd(&hist[group_key(slot, r, slots)], 1u);  // (integers: any order)
     __syncthreads();
     for (int k = threadIdx.x; k <= slots; k += 64) count[(size_t)k * blocks + blockIdx.x] = hist[k];
 }
@@ -97,15 +91,10 @@ __global__ __launch_bounds__(64) void group_begin_kernel(const uint32_t* __restr
     if (threadIdx.x == 0) begin[slots + 1] = rows;
 }
 
-// order[place] = row, row_slot[place] = its slot or -1
-__global__ __launch_bounds__(64) void group_place_kernel(const int32_t* __restrict__ slot, uint32_t rows, int slots, int blocks,
-                                                         const uint32_t* __restrict__ count, const uint32_t* __restrict__ begin,
-                                                         uint32_t* __restrict__ order, int32_t* __restrict__ row_slot)
+// order[place] = row, row_slot[place] = its slot or -1, for rows r0 .. r1 - 1; next[key]: where the key's next row goes
+__device__ __forceinline__ void place_rows(const int32_t* __restrict__ slot, uint32_t r0, uint32_t r1, int slots, uint32_t* next,
+                                           uint32_t* __restrict__ order, int32_t* __restrict__ row_slot)
 {
-    extern __shared__ uint32_t next[];
-    for (int k = threadIdx.x; k <= slots; k += 64) next[k] = begin[k] + count[(size_t)k * blocks + blockIdx.x];
-    __syncthreads();
-    const uint32_t r0 = blockIdx.x * kGroupRows, r1 = min(rows, r0 + kGroupRows);
     for (uint32_t r = r0; r < r1; r += 64) {
         const bool in = r + threadIdx.x < r1;
         const int key = in ? group_key(slot, r + threadIdx.x, slots) : 0;
@@ -122,6 +111,39 @@ __global__ __launch_bounds__(64) void group_place_kernel(const int32_t* __restri
             row_slot[place] = key < slots ? key : -1;
         }
     }
+}
+__global__ __launch_bounds__(64) void group_place_kernel(const int32_t* __restrict__ slot, uint32_t rows, int slots, int blocks,
+                                                         const uint32_t* __restrict__ count, const uint32_t* __restrict__ begin,
+                                                         uint32_t* __restrict__ order, int32_t* __restrict__ row_slot)
+{
+    extern __shared__ uint32_t next[];
+    for (int k = threadIdx.x; k <= slots; k += 64) next[k] = begin[k] + count[(size_t)k * blocks + blockIdx.x];
+    __syncthreads();
+    const uint32_t r0 = blockIdx.x * kGroupRows;
+    place_rows(slot, r0, min(rows, r0 + kGroupRows), slots, next, order, row_slot);
+}
+
+// all of it for one block of rows, in one wave
+__global__ __launch_bounds__(64) void group_few_kernel(const int32_t* __restrict__ slot, uint32_t rows, int slots,
+                                                       uint32_t* __restrict__ begin, uint32_t* __restrict__ order,
+                                                       int32_t* __restrict__ row_slot)
+{
+    extern __shared__ uint32_t next[];
+    for (int k = threadIdx.x; k <= slots; k += 64) next[k] = 0;
+    __syncthreads();
+    for (uint32_t r = threadIdx.x; r < rows; r += 64) atomicAdd(&next[group_key(slot, r, slots)], 1u);
+    __syncthreads();
+    uint32_t run = 0;
+    for (int b = 0; b <= slots; b += 64) {
+        const int i = b + (int)threadIdx.x;
+        const uint32_t v = i <= slots ? next[i] : 0;
+        const uint32_t inc = wave_scan(v);
+        if (i <= slots) begin[i] = next[i] = run + inc - v;
+        run += __shfl(inc, 63);
+    }
+    if (threadIdx.x == 0) begin[slots + 1] = rows;
+    __syncthreads();
+    place_rows(slot, 0, rows, slots, next, order, row_slot);
 }
 
 // ---- rows in that order -------------------------------------------------------------------------
@@ -235,17 +257,25 @@ __global__ __launch_bounds__(256) void low_kernel(LowArgs a)
 }
 
 // ---- factor gradients -----------------------------------------------------------------------------
-// slab[chunk + slot][m][j] = sum over the slot's rows i in the chunk of p[i][m] w[i][j].  Rows are sorted by
-// slot, so (chunk, slot) pairs that hold rows lie on a staircase and chunk + slot numbers them without a gap
-// table; factor_reduce_kernel adds a slot's chunks in order.
+// The four factors' gradients are four contractions over rows, grad[slot][m][j] = sum over the slot's rows of
+// p[i][m] w[i][j], m up to a layer's width and j the rank columns; one launch does all four.
+// slab[chunk + slot][m][j] takes the part of a chunk of rows: rows are sorted by slot, so (chunk, slot) pairs that
+// hold rows lie on a staircase and chunk + slot numbers them without a table; factor_reduce_kernel adds a slot's chunks.
 constexpr int kFactorRows = 512;
-struct FactorArgs {
+struct FactorJob {
     const float* p;        // [rows][ldp], 16-byte aligned rows
     const float* w;        // [rows][ldw], the rank columns
+    float* slab;
+    uint64_t off;          // the factor's place in a slot's gradient: element (m, j) at off + m * g_m + j * g_j
+    int ldp, M, g_m, g_j;
+    int first;             // first tile of 64 columns of this job
+    int first_out;         // first block of 256 elements of this job in factor_reduce_kernel
+};
+struct FactorArgs {
+    FactorJob job[4];
     const uint32_t* begin; // [slots + 2]
     const int32_t* row_slot;
-    float* slab;
-    int ldp, M, ldw, rank, slots;
+    int ldw, rank, slots;
 };
 
 // 64 columns of p per workgroup; its four waves take rows in turn and are joined in LDS.  A lane reads 16
@@ -254,9 +284,11 @@ template <int NT>
 __global__ __launch_bounds__(256) void factor_grad_kernel(FactorArgs a)
 {
     __shared__ __attribute__((aligned(16))) float part[4][64][NT * 16];
+    const int which = ((int)blockIdx.x >= a.job[1].first) + ((int)blockIdx.x >= a.job[2].first) + ((int)blockIdx.x >= a.job[3].first);
+    const FactorJob g = a.job[which];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int c16 = lane & 15, q = lane >> 4;
-    const int m0 = blockIdx.x * 64;
+    const int m0 = ((int)blockIdx.x - g.first) * 64;
     const uint32_t end = min(a.begin[a.slots], (blockIdx.y + 1) * (uint32_t)kFactorRows);
     uint32_t r = blockIdx.y * (uint32_t)kFactorRows;
     while (r < end) {
@@ -271,13 +303,13 @@ __global__ __launch_bounds__(256) void factor_grad_kernel(FactorArgs a)
             const bool in = i + q < stop;
             const size_t row = in ? i + q : stop - 1;
             const int col = m0 + 4 * c16;
-            f32x4 pv = *reinterpret_cast<const f32x4*>(a.p + row * a.ldp + min(col, a.ldp - 4));
+            f32x4 pv = *reinterpret_cast<const f32x4*>(g.p + row * g.ldp + min(col, g.ldp - 4));
 #pragma unroll
-            for (int t = 0; t < 4; ++t) pv[t] = in && col + t < a.M ? pv[t] : 0.0f;
+            for (int t = 0; t < 4; ++t) pv[t] = in && col + t < g.M ? pv[t] : 0.0f;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const int j = 16 * n + c16;
-                float v = a.w[row * a.ldw + min(j, a.rank - 1)];
+                float v = g.w[row * a.ldw + min(j, a.rank - 1)];
                 v = in && j < a.rank ? v : 0.0f;
 #pragma unroll
                 for (int t = 0; t < 4; ++t) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[t], v, acc[t][n], 0, 0, 0);
@@ -290,10 +322,10 @@ __global__ __launch_bounds__(256) void factor_grad_kernel(FactorArgs a)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) part[wave][4 * (4 * q + i) + t][16 * n + c16] = acc[t][n][i];
         __syncthreads();
-        float* slab = a.slab + ((size_t)blockIdx.y + slot) * a.M * a.rank;
+        float* slab = g.slab + ((size_t)blockIdx.y + slot) * g.M * a.rank;
         for (int e = threadIdx.x; e < 64 * a.rank; e += 256) {
             const int m = e / a.rank, j = e % a.rank;
-            if (m0 + m < a.M)
+            if (m0 + m < g.M)
                 slab[(size_t)(m0 + m) * a.rank + j] = (part[0][m][j] + part[1][m][j]) + (part[2][m][j] + part[3][m][j]);
         }
         __syncthreads();
@@ -301,20 +333,20 @@ __global__ __launch_bounds__(256) void factor_grad_kernel(FactorArgs a)
     }
 }
 
-// grad[slot][m * g_m + j * g_j] += the slot's chunks of the slab; 64-bit sums, in chunk order
-__global__ __launch_bounds__(256) void factor_reduce_kernel(const float* __restrict__ slab, const uint32_t* __restrict__ begin, int M,
-                                                            int rank, int g_m, int g_j, float* __restrict__ grad,
-                                                            uint64_t grad_slot)
+// grad[slot] += the slot's chunks of the slabs; 64-bit sums, in chunk order
+__global__ __launch_bounds__(256) void factor_reduce_kernel(FactorArgs a, float* __restrict__ grad, uint64_t grad_slot)
 {
     const int slot = blockIdx.y;
-    const uint32_t b = begin[slot], e = begin[slot + 1];
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (b == e || i >= M * rank) return;
+    const uint32_t b = a.begin[slot], e = a.begin[slot + 1];
+    if (b == e) return;
+    const int which = ((int)blockIdx.x >= a.job[1].first_out) + ((int)blockIdx.x >= a.job[2].first_out) + ((int)blockIdx.x >= a.job[3].first_out);
+    const FactorJob g = a.job[which];
+    const int i = ((int)blockIdx.x - g.first_out) * 256 + threadIdx.x;
+    if (i >= g.M * a.rank) return;
     const uint32_t c0 = b / kFactorRows, c1 = (e - 1) / kFactorRows;
     double t = 0.0;
-    for (uint32_t c = c0; c <= c1; ++c) t += (double)slab[(size_t)(c + slot) * M * rank + i];
-    float* g = grad + (size_t)slot * grad_slot + (size_t)(i / rank) * g_m + (size_t)(i % rank) * g_j;
-    *g += (float)t;
+    for (uint32_t c = c0; c <= c1; ++c) t += (double)g.slab[(size_t)(c + slot) * g.M * a.rank + i];
+    grad[(size_t)slot * grad_slot + g.off + (size_t)(i / a.rank) * g.g_m + (size_t)(i % a.rank) * g.g_j] += (float)t;
 }
 
 // sums[slot] += {loss, live rows} of the slot's rows (64 bits, fixed order); tail = the same as floats

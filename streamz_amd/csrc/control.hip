@@ -12,6 +12,7 @@
 // wave per row up to 1024 classes (control_rows_kernel), a workgroup per row beyond (control_row_kernel).
 #include <algorithm>
 
+#include "control_kernel.h"
 #include "internal.h"
 #include "prof.h"
 #include "streamz_hip.h"
@@ -20,106 +21,7 @@ namespace sz {
 
 namespace {
 
-enum Mode { M_INFER = 0, M_TRAIN = 1, M_VOTE = 2 };
-
-struct RowControl {
-    const float* bias;
-    const uint32_t* allow;
-    const uint32_t* counts;
-    float repetition, inverse, presence, frequency;
-};
-
-__device__ __forceinline__ int32_t row_set(const Controls& c, uint64_t row)
-{
-    return c.sets == 0 ? -1 : c.set_of_row ? c.set_of_row[row] : 0;
-}
-
-__device__ __forceinline__ RowControl row_control(const Controls& c, int C, int32_t set)
-{
-    RowControl r{nullptr, nullptr, nullptr, 1.0f, 1.0f, 0.0f, 0.0f};
-    if (set < 0 || (uint32_t)set >= c.sets) return r;
-    if (c.bias) r.bias = c.bias + (uint64_t)set * C;
-    if (c.allow) r.allow = c.allow + (uint64_t)set * ((C + 31) / 32);
-    if (c.counts) {
-        r.counts = c.counts + (uint64_t)set * C;
-        if (c.repetition) { r.repetition = c.repetition[set]; r.inverse = 1.0f / r.repetition; }
-        if (c.presence) r.presence = c.presence[set];
-        if (c.frequency) r.frequency = c.frequency[set];
-    }
-    return r;
-}
-
-__device__ __forceinline__ bool allowed(const RowControl& r, int c) { return !r.allow || ((r.allow[c >> 5] >> (c & 31)) & 1u); }
-
-// (the division by the repetition penalty is a product with its reciprocal: two roundings instead of one)
-__device__ __forceinline__ float penalised(const RowControl& r, float z, uint32_t count)
-{
-    const float n = (float)count;
-    const float seen = (z > 0.0f ? z * r.inverse : z * r.repetition) - r.presence;
-    return (n > 0.0f ? seen : z) - r.frequency * n;
-}
-
-__device__ __forceinline__ float controlled(const RowControl& r, float z, int c)
-{
-    if (r.counts) z = penalised(r, z, r.counts[c]);
-    if (r.bias) z += r.bias[c];
-    return allowed(r, c) ? z : -INFINITY;
-}
-
-// e^x for x <= 0 (or NaN): 2^(x log2 e) by the hardware instruction with the rounding of the product, which would
-// cost |x| 2^-24, put back to first order.  0 below -200.
-__device__ __forceinline__ float exp_low(float x)
-{
-    const float kL = 1.44269502f, kR = 1.92596299e-8f, kLn2 = 0.693147182f;  // log2 e in two parts
-    const float y = x < -200.0f ? -200.0f : x;
-    const float t = y * kL;
-    const float r = __builtin_fmaf(y, kR, __builtin_fmaf(y, kL, -t));
-    const float e = __builtin_amdgcn_exp2f(t);
-    return __builtin_fmaf(e, r * kLn2, e);
-}
-
-template <int LANES>
-__device__ __forceinline__ float lanes_max(float v)
-{
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
-template <int LANES>
-__device__ __forceinline__ float lanes_sum(float v)
-{
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-// the last of the largest values over the lanes: (p, c) pairs, c = -1 for none
-template <int LANES>
-__device__ __forceinline__ void lanes_best(float& p, int& c)
-{
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) {
-        const float q = __shfl_xor(p, o);
-        const int b = __shfl_xor(c, o);
-        if (q > p || (q == p && b > c)) { p = q; c = b; }
-    }
-}
-
-// the vote of identify_speaker_list (lib.rs:1391-1402): the last maximum wins; a row without a candidate has none.
-// Counts are integers: the order of the additions is of no matter.
-__device__ __forceinline__ void cast_vote(const ControlRun& a, uint64_t row, int C, bool some, float p, int best)
-{
-    const int32_t g = a.group ? a.group[row] : 0;
-    if (some && best >= 0 && p >= a.threshold && g >= 0 && (uint32_t)g < a.groups) atomicAdd(&a.votes[(uint64_t)g * C + best], 1ull);
-}
-
-struct TrainRow { int label; bool live; };
-__device__ __forceinline__ TrainRow train_row(const ControlRun& a, const RowControl& rc, uint64_t i, uint64_t row, int C, bool some)
-{
-    TrainRow t;
-    t.label = a.labels[row];
-    t.live = a.row_live[i] && a.row_slot[i] >= 0 && t.label >= 0 && t.label < C && some && allowed(rc, t.label);
-    return t;
-}
+using namespace control;
 
 // LANES lanes of a wave per row, Q groups of four classes per lane: class 4 (l + LANES q) + e.  A row's logits
 // and the number of its set are asked for while the row before is worked on.

@@ -305,7 +305,7 @@ struct AdaptWorkspace {
     uint32_t *order = nullptr, *begin = nullptr, *count = nullptr, *total = nullptr, *w2s = nullptr;
     int32_t* row_slot = nullptr;
     float *xs = nullptr, *h1 = nullptr, *h2 = nullptr, *lg = nullptr, *u2 = nullptr, *u3 = nullptr, *w1t = nullptr, *w2t = nullptr,
-          *w3t = nullptr, *d2 = nullptr, *g2 = nullptr, *g3 = nullptr, *loss = nullptr, *slab = nullptr;
+          *w3t = nullptr, *add2 = nullptr, *add3 = nullptr, *d2 = nullptr, *g2 = nullptr, *g3 = nullptr, *loss = nullptr, *slab = nullptr;
     uint8_t *live0 = nullptr, *live = nullptr;
 };
 struct Adapters {
