@@ -38,7 +38,7 @@ using namespace adapt;
 constexpr uint64_t kAdaptRows = 131072;
 
 // Calls of up to this many rows go row by row (adapt_rows.h).
-constexpr uint64_t kFewRows = 512;
+constexpr uint64_t kFewRows = 1024;
 
 inline int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
@@ -60,14 +60,14 @@ size_t lay_out(const Adapters* a, uint64_t rows, bool training, char* base, Adap
     AdaptWorkspace& o = w ? *w : t;
     const uint64_t blocks = (rows + kGroupRows - 1) / kGroupRows, S = a->slots;
     o.ldx = a->in + 1 <= 64 ? 64 : round_up((int)a->in + 1, 128);
-    o.ld1 = round_up((int)a->h1, 4); o.ld2 = round_up((int)a->h2, 4); o.ld3 = round_up((int)std::max(a->out, 1u), 4);
+    o.ld1 = round_up((int)a->h1, 32); o.ld2 = round_up((int)a->h2, 32); o.ld3 = round_up((int)std::max(a->out, 1u), 4);
     o.ldu = round_up((int)a->rank, 8);
     take(o.order, rows); take(o.row_slot, rows); take(o.begin, S + 2); take(o.count, (S + 1) * blocks); take(o.total, S + 1);
     take(o.xs, rows * o.ldx); take(o.live0, rows); take(o.live, rows);
     take(o.h1, (rows + 32) * o.ld1); take(o.h2, (rows + 32) * o.ld2); take(o.lg, (rows + 32) * o.ld3);
     take(o.u2, rows * o.ldu); take(o.u3, rows * o.ldu);
     take(o.add2, kFewRows * o.ld2); take(o.add3, kFewRows * o.ld3);
-    take(o.w1t, (uint64_t)a->h1 * o.ldx); take(o.w2t, (uint64_t)a->h1 * a->h2); take(o.w3t, (uint64_t)a->h2 * a->out + 1);
+    take(o.w1t, (uint64_t)a->h1 * o.ldx); take(o.w2t, (uint64_t)o.ld1 * a->h2); take(o.w3t, (uint64_t)o.ld2 * std::max(a->out, 1u));
     take(o.w2s, 3 * ((uint64_t)a->h1 * a->h2 + 1) / 2 + 4);
     if (training) {
         const uint64_t chunks = (rows + kFactorRows - 1) / kFactorRows;
@@ -86,8 +86,11 @@ int ensure(Adapters* a, uint64_t rows, bool training, hipStream_t s)
     rows = (rows + 255) / 256 * 256;
     training = training || a->ws_training;
     char* p = nullptr;
-    SZ_HIP(hipMalloc((void**)&p, lay_out(a, rows, training, nullptr, nullptr)));
+    const size_t bytes = lay_out(a, rows, training, nullptr, nullptr);
+    SZ_HIP(hipMalloc((void**)&p, bytes));
     try { a->arenas.push_back(p); } catch (...) { (void)hipFree(p); throw; }
+    SZ_HIP(hipMemset(p, 0, bytes));  // the columns between a row's end and its stride are read as zeros
+    SZ_HIP(hipDeviceSynchronize());
     // the old workspace stays until the handle goes: a captured graph may still work in it
     lay_out(a, rows, training, p, &a->ws);
     a->ws_rows = rows;
@@ -125,6 +128,18 @@ int group_rows(Adapters* a, const int32_t* slots_dev, uint32_t rows, hipStream_t
     return SZH_OK;
 }
 
+template <int NT, int OT, int WAVES, int UNR>
+int launch_low(LowArgs g, hipStream_t s)
+{
+    constexpr size_t lds = (size_t)WAVES * 32 * NT * 16 * sizeof(float);
+    if (int rc = allow_dynamic_lds((const void*)low_kernel<NT, OT, WAVES, UNR>, lds)) return rc;
+    const unsigned tiles = (g.rows + 31) / 32;
+    g.parts = tiles >= 512 ? 1 : (int)std::min<unsigned>(32, 1024 / tiles);
+    hipLaunchKernelGGL((low_kernel<NT, OT, WAVES, UNR>), dim3(tiles, g.parts), dim3(64 * WAVES), lds, s, g);
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
+}
+
 // u = scale * x F[slot]
 int low_product(const Adapters* a, const float* x, int ldx, int K, const float* factor, int f_k, int f_j, uint32_t rows, float* u,
                 hipStream_t s)
@@ -132,16 +147,39 @@ int low_product(const Adapters* a, const float* x, int ldx, int K, const float* 
     LowArgs g{};
     g.x = x; g.ldx = ldx; g.K = K; g.factor = factor; g.factor_slot = a->per_slot(); g.f_k = f_k; g.f_j = f_j;
     g.rank = (int)a->rank; g.row_slot = a->ws.row_slot; g.rows = rows; g.u = u; g.ldu = a->ws.ldu; g.scale = a->scale;
-    const dim3 grid((rows + 31) / 32), block(256);
     ProfScope prof("adapt_low", s);
     switch ((a->rank + 15) / 16) {
-    case 1: hipLaunchKernelGGL((low_kernel<1>), grid, block, 0, s, g); break;
-    case 2: hipLaunchKernelGGL((low_kernel<2>), grid, block, 0, s, g); break;
-    case 3: hipLaunchKernelGGL((low_kernel<3>), grid, block, 0, s, g); break;
-    default: hipLaunchKernelGGL((low_kernel<4>), grid, block, 0, s, g); break;
+    case 1: return launch_low<1, 0, 8, 4>(g, s);
+    case 2: return launch_low<2, 0, 8, 2>(g, s);
+    case 3: return launch_low<3, 0, 8, 2>(g, s);
+    default: return launch_low<4, 0, 4, 2>(g, s);
     }
-    SZ_HIP(hipGetLastError());
-    return SZH_OK;
+}
+
+// Output layers of up to 64 classes: u3 and the logits in one pass over h2
+bool low_out_applies(const Adapters* a) { return a->out <= 64; }
+int low_out(const Net* n, const Adapters* a, uint32_t rows, hipStream_t s)
+{
+    const AdaptWorkspace& w = a->ws;
+    LowArgs g{};
+    g.x = w.h2; g.ldx = w.ld2; g.K = (int)n->h2; g.factor = a->d_params + a->off_a3(); g.factor_slot = a->per_slot();
+    g.f_k = (int)a->rank; g.f_j = 1; g.rank = (int)a->rank; g.row_slot = w.row_slot; g.rows = rows; g.u = w.u3; g.ldu = w.ldu; g.scale = a->scale;
+    g.W = n->d_params + n->off_w3(); g.bias = n->d_params + n->off_b3(); g.up = a->d_params + a->off_b3(); g.up_slot = a->per_slot();
+    g.y = w.lg; g.out = (int)n->out; g.ldy = w.ld3;
+    ProfScope prof("adapt_out", s);
+    const int rt = (int)(a->rank + 15) / 16, ot = (int)(n->out + 15) / 16;
+    // (three tiles are taken as four: a column tile without columns repeats the last one's)
+    switch ((ot > 2 ? 4 : ot) * 8 + (rt > 2 ? 4 : rt)) {
+    case 1 * 8 + 1: return launch_low<2, 1, 8, 2>(g, s);
+    case 1 * 8 + 2: return launch_low<3, 1, 8, 2>(g, s);
+    case 1 * 8 + 4: return launch_low<5, 1, 4, 1>(g, s);
+    case 2 * 8 + 1: return launch_low<3, 2, 8, 2>(g, s);
+    case 2 * 8 + 2: return launch_low<4, 2, 4, 2>(g, s);
+    case 2 * 8 + 4: return launch_low<6, 2, 4, 1>(g, s);
+    case 4 * 8 + 1: return launch_low<5, 4, 4, 1>(g, s);
+    case 4 * 8 + 2: return launch_low<6, 4, 4, 1>(g, s);
+    default: return launch_low<8, 4, 4, 1>(g, s);
+    }
 }
 
 // the gradients of a pass's four factors, added to the bank's
@@ -180,7 +218,89 @@ int factor_gradients(Adapters* a, uint32_t rows, hipStream_t s)
 void adapt_args(GemmArgs& g, const Adapters* a, const float* low, const float* up, int up_k, int up_n)
 {
     g.low = low; g.ld_low = a->ws.ldu; g.up = up; g.up_slot = a->per_slot(); g.up_k = up_k; g.up_n = up_n; g.rank = (int)a->rank;
-    g.row_slot = a->ws.row_slot;
+    g.row_slot = a->ws.row_slot; g.row_begin = a->ws.begin;
+}
+
+template <bool TANH>
+int thin_product(const float* A, int lda, int K, const float* W, const float* add, int ldadd, const float* bias, float* C, int ldc, int N,
+                 uint32_t rows, const char* tag, hipStream_t s)
+{
+    ThinArgs g{};
+    g.A = A; g.lda = lda; g.W = W; g.add = add; g.ldadd = ldadd; g.bias = bias; g.C = C; g.ldc = ldc; g.M = (int)rows; g.N = N; g.K = K;
+    ProfScope prof(tag, s);
+    hipLaunchKernelGGL((thin_kernel<TANH>), dim3((N + 31) / 32, (rows + 31) / 32), dim3(64 * kThinWaves), 0, s, g);
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
+}
+
+// Which kernels a shared product of `rows` rows goes to.  The 256 x 256 tiles of gemm_f32w_kernel are the fastest
+// (137 TFLOP/s) but run one per compute unit, so only whole rounds of them pay: the first rows go there, the rest to
+// what is quickest for so many.  Times in us of a product [rows][K] x [K][N], fitted to measurements over K 512 .. 2048,
+// N 256 .. 2048, 256 to 66140 rows (66140 x 512 x 256: 182 us on 64-row tiles, 283 on 256-row tiles, 145 split;
+// 26456 x 2048 x 2048: 1849, 2051, 1660):
+//   256-row tiles: 0.232 K + 18 for every round of one tile per compute unit
+//   128-row tiles: two per unit 0.122 K + 17, one 0.071 K + 12        64-row tiles: 0.0337 K + 4 each, once 0.0085 K
+//   32 x 32 thin tiles: 5 + 0.001 K, and 3.55e-5 K each
+struct ProductPlan { uint32_t wide_rows; int rest; };  // rest: 0 thin, 64, 128
+double rest_time(uint32_t rows, int N, int K, double cus, int* how)
+{
+    auto ceil_div = [](uint64_t a, uint64_t b) { return (double)((a + b - 1) / b); };
+    const double t32 = ceil_div(rows, 32) * ceil_div(N, 32);
+    const double c64 = std::ceil(ceil_div(rows, 64) * ceil_div(N, 128) / cus), c128 = std::ceil(ceil_div(rows, 128) * ceil_div(N, 128) / cus);
+    const double thin = 5 + 0.001 * K + t32 * 3.55e-5 * K;
+    const double g64 = c64 * (0.0337 * K + 4) + 0.0085 * K;
+    const double g128 = std::floor(c128 / 2) * (0.122 * K + 17) + (std::fmod(c128, 2.0) != 0 ? 0.071 * K + 12 : 0);
+    *how = thin <= g64 && thin <= g128 ? 0 : g64 <= g128 ? 64 : 128;
+    return std::min(thin, std::min(g64, g128));
+}
+ProductPlan plan_product(uint32_t rows, int N, int K)
+{
+    const double cus = compute_units();
+    ProductPlan best{0, 64};
+    double time = rest_time(rows, N, K, cus, &best.rest);
+    const uint32_t across = (N + 255) / 256, down = (rows + 255) / 256;
+    const uint32_t rounds = (uint32_t)((uint64_t)across * down / (uint64_t)cus);
+    // whole rounds of wide tiles (and one more, partly filled); the transposed weights cost a launch
+    for (uint32_t q = rounds ? rounds : 1; q <= rounds + 1; ++q) {
+        const uint32_t m = (uint32_t)std::min<uint64_t>((uint64_t)q * (uint64_t)cus / across, down);
+        if (m == 0) continue;
+        ProductPlan p{std::min(rows, m * 256), 64};
+        double t = std::ceil((double)m * across / cus) * (0.232 * K + 18) + 6;
+        if (p.wide_rows < rows) t += rest_time(rows - p.wide_rows, N, K, cus, &p.rest) + 2;
+        if (t < time) { time = t; best = p; }
+    }
+    return best;
+}
+
+// C = epilogue(A W + low part), rows sorted by slot, as planned.  g: the whole product with B = W [K][N]; Kp: A's
+// columns with the zeros behind them, a multiple of 32; wt: room for W transposed and padded, [N][Kp].
+template <int EPI, int TAG>
+int shared_product(const GemmArgs& g, int Kp, float* wt, hipStream_t s)
+{
+    const ProductPlan p = plan_product((uint32_t)g.M, g.N, g.K);
+    if (p.wide_rows) {
+        {
+            ProfScope prof("w2t", s);
+            hipLaunchKernelGGL(pad_transpose_kernel, dim3((unsigned)(((uint64_t)g.N * Kp + 255) / 256)), dim3(256), 0, s, g.B, g.K, g.N, Kp, wt);
+            SZ_HIP(hipGetLastError());
+        }
+        GemmArgs h = g;
+        h.M = (int)p.wide_rows; h.B = wt; h.ldb = Kp; h.K = h.k_chunk = Kp;
+        if (int rc = launch_gemm_f32w<EPI, TAG>(h, s)) return rc;
+        if ((int)p.wide_rows == g.M) return SZH_OK;
+    }
+    GemmArgs h = g;
+    h.M -= (int)p.wide_rows;
+    h.A += (size_t)p.wide_rows * g.lda; h.C += (size_t)p.wide_rows * g.ldc; h.low += (size_t)p.wide_rows * g.ld_low; h.row_slot += p.wide_rows;
+    if (p.rest == 64) return launch_gemm_rows<A_ROWS, B_KROWS, EPI, TAG, 64>(h, s);
+    if (p.rest == 128) return launch_gemm_rows<A_ROWS, B_KROWS, EPI, TAG, 128>(h, s);
+    ThinArgs t{};
+    t.A = h.A; t.lda = h.lda; t.W = h.B; t.bias = h.bias; t.C = h.C; t.ldc = h.ldc; t.M = h.M; t.N = h.N; t.K = h.K;
+    t.low = h.low; t.up = h.up; t.row_slot = h.row_slot; t.up_slot = h.up_slot; t.ld_low = h.ld_low; t.rank = h.rank;
+    ProfScope prof(kGemmTagName[TAG], s);
+    hipLaunchKernelGGL((thin_kernel<EPI == EPI_ADAPT_TANH>), dim3((t.N + 31) / 32, (t.M + 31) / 32), dim3(64 * kThinWaves), 0, s, t);
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
 }
 
 // logits of `rows` grouped rows in the workspace's lg, activations in h1, h2, rank columns in u2, u3
@@ -190,56 +310,41 @@ int forward_rows(Net* n, Adapters* a, uint32_t rows, hipStream_t s)
     const float* P = n->d_params;
     const float* F = a->d_params;
     const int r = (int)a->rank;
-    const bool x3 = use_x3(n, rows), wide1 = use_wide_f32(n, rows), wide = !x3 && wide1;
     int rc;
-    if (x3 || wide) {
-        ProfScope prof("w2t", s);
-        hipLaunchKernelGGL(transpose_kernel, dim3((n->h2 + 31) / 32, (n->h1 + 31) / 32), dim3(256), 0, s, P + n->off_w2(), (int)n->h1,
-                           (int)n->h2, w.w2t);
-        const uint64_t count = (uint64_t)n->h1 * n->h2;
-        if (x3)
-            hipLaunchKernelGGL(split_planes_kernel, dim3((unsigned)((count / 2 + 255) / 256)), dim3(256), 0, s, w.w2t, count, w.w2s, count / 2);
-    }
-    if (wide1) {
-        ProfScope prof("w2t", s);
-        hipLaunchKernelGGL(pad_transpose_kernel, dim3((n->h1 * w.ldx + 255) / 256), dim3(256), 0, s, P + n->off_w1(), (int)n->in, (int)n->h1,
-                           w.ldx, w.w1t);
-    }
-    SZ_HIP(hipGetLastError());
     GemmArgs g{};
-    g.A = w.xs; g.lda = w.ldx; g.a_pad = 0; g.C = w.h1; g.ldc = w.ld1; g.M = (int)rows; g.N = (int)n->h1; g.bias = P + n->off_b1();
-    if (wide1) {
-        g.B = w.w1t; g.ldb = w.ldx; g.K = g.k_chunk = w.ldx;
-        rc = launch_gemm_f32w<EPI_BIAS_RELU, T_ADAPT1>(g, s);
-    } else {
-        g.B = P + n->off_w1(); g.ldb = (int)n->h1; g.K = g.k_chunk = (int)n->in;
-        rc = launch_gemm<A_ROWS, B_KROWS, EPI_BIAS_RELU, T_ADAPT1>(g, 1, s);
-    }
-    if (rc) return rc;
-    rc = low_product(a, w.h1, w.ld1, (int)n->h1, F + a->off_a2(), r, 1, rows, w.u2, s);
+    g.A = w.xs; g.lda = w.ldx; g.C = w.h1; g.ldc = w.ld1; g.M = (int)rows; g.N = (int)n->h1; g.bias = P + n->off_b1();
+    g.B = P + n->off_w1(); g.ldb = (int)n->h1; g.K = g.k_chunk = (int)n->in;
+    // (a short k: 64-row tiles are never behind, 57 us against 61 on 128 and 70 on 256 rows at 66140 x 60 x 512)
+    rc = launch_gemm_rows<A_ROWS, B_KROWS, EPI_BIAS_RELU, T_ADAPT1, 64>(g, s);
+    if (!rc) rc = low_product(a, w.h1, w.ld1, (int)n->h1, F + a->off_a2(), r, 1, rows, w.u2, s);
     if (rc) return rc;
     g = GemmArgs{};
     g.A = w.h1; g.lda = w.ld1; g.C = w.h2; g.ldc = w.ld2; g.M = (int)rows; g.N = (int)n->h2; g.K = g.k_chunk = (int)n->h1;
-    g.bias = P + n->off_b2();
+    g.B = P + n->off_w2(); g.ldb = (int)n->h2; g.bias = P + n->off_b2();
     adapt_args(g, a, w.u2, F + a->off_b2(), (int)n->h2, 1);
-    if (x3) {
+    if (use_x3(n, rows)) {
+        {
+            ProfScope prof("w2split", s);
+            const uint64_t count = (uint64_t)n->h1 * n->h2;
+            hipLaunchKernelGGL(transpose_kernel, dim3((n->h2 + 31) / 32, (n->h1 + 31) / 32), dim3(256), 0, s, P + n->off_w2(), (int)n->h1,
+                               (int)n->h2, w.w2t);
+            hipLaunchKernelGGL(split_planes_kernel, dim3((unsigned)((count / 2 + 255) / 256)), dim3(256), 0, s, w.w2t, count, w.w2s, count / 2);
+            SZ_HIP(hipGetLastError());
+        }
         g.B = (const float*)w.w2s; g.ldb = (int)n->h1; g.b_plane = (uint64_t)n->h1 * n->h2;
         rc = launch_gemm_x3<X3_ROWS_F32, X3_ROWS_SPLIT, EPI_ADAPT_TANH, T_ADAPT2>(g, 1, s);
-    } else if (wide) {
-        g.B = w.w2t; g.ldb = (int)n->h1;
-        rc = launch_gemm_f32w<EPI_ADAPT_TANH, T_ADAPT2>(g, s);
     } else {
-        g.B = P + n->off_w2(); g.ldb = (int)n->h2;
-        rc = launch_gemm<A_ROWS, B_KROWS, EPI_ADAPT_TANH, T_ADAPT2>(g, 1, s);
+        rc = shared_product<EPI_ADAPT_TANH, T_ADAPT2>(g, w.ld1, w.w2t, s);
     }
     if (rc || n->out == 0) return rc;
+    if (low_out_applies(a)) return low_out(n, a, rows, s);
     rc = low_product(a, w.h2, w.ld2, (int)n->h2, F + a->off_a3(), r, 1, rows, w.u3, s);
     if (rc) return rc;
     g = GemmArgs{};
     g.A = w.h2; g.lda = w.ld2; g.C = w.lg; g.ldc = w.ld3; g.M = (int)rows; g.N = (int)n->out; g.K = g.k_chunk = (int)n->h2;
     g.B = P + n->off_w3(); g.ldb = (int)n->out; g.bias = P + n->off_b3();
     adapt_args(g, a, w.u3, F + a->off_b3(), (int)n->out, 1);
-    return launch_gemm<A_ROWS, B_KROWS, EPI_ADAPT_BIAS, T_ADAPT3>(g, 1, s);
+    return shared_product<EPI_ADAPT_BIAS, T_ADAPT3>(g, w.ld2, w.w3t, s);
 }
 
 // Whether a call takes the few-row path: its row kernels hold a row's activations in LDS.
@@ -263,18 +368,6 @@ RowArgs row_args(const Net* n, Adapters* a, const float* x, uint64_t ldx, const 
     g.rank = (int)a->rank; g.ldu = w.ldu; g.ld1 = w.ld1; g.ld2 = w.ld2; g.ld3 = w.ld3; g.scale = a->scale;
     g.h1 = w.h1; g.h2 = w.h2; g.add2 = w.add2; g.add3 = w.add3;
     return g;
-}
-
-template <bool TANH>
-int thin_product(const float* A, int lda, int K, const float* W, const float* add, int ldadd, const float* bias, float* C, int ldc, int N,
-                 uint32_t rows, const char* tag, hipStream_t s)
-{
-    ThinArgs g{};
-    g.A = A; g.lda = lda; g.W = W; g.add = add; g.ldadd = ldadd; g.bias = bias; g.C = C; g.ldc = ldc; g.M = (int)rows; g.N = N; g.K = K;
-    ProfScope prof(tag, s);
-    hipLaunchKernelGGL((thin_kernel<TANH>), dim3((N + 31) / 32, (rows + 31) / 32), dim3(64 * kThinWaves), 0, s, g);
-    SZ_HIP(hipGetLastError());
-    return SZH_OK;
 }
 
 template <int OUT>
@@ -476,7 +569,7 @@ int adapters_accumulate(Net* n, Adapters* a, const float* x, const int32_t* labe
             g.A = w.lg; g.lda = w.ld3; g.B = n->d_params + n->off_w3(); g.ldb = out; g.C = w.d2; g.ldc = w.ld2;
             g.M = (int)R; g.N = h2; g.K = g.k_chunk = out; g.aux = w.h2; g.ldaux = w.ld2;
             adapt_args(g, a, w.g3, F + a->off_a3(), 1, r);
-            rc = launch_gemm<A_ROWS, B_ROWS, EPI_ADAPT_DTANH, T_ADAPT_D2>(g, 1, s);
+            rc = launch_gemm_rows<A_ROWS, B_ROWS, EPI_ADAPT_DTANH, T_ADAPT_D2, 64>(g, s);  // (a short k, as above)
             if (!rc) rc = low_product(a, w.d2, w.ld2, h2, F + a->off_b2(), 1, h2, R, w.g2, s);
             if (rc) return rc;
         }

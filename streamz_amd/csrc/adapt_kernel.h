@@ -175,7 +175,8 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const float* __restric
 
 // ---- products with the rank columns ----------------------------------------------------------------
 // u[i][j] = scale * sum_k x[i][k] F[k][j],  F = the [K][rank] matrix of row i's slot with element (k, j) at
-// k * f_k + j * f_j.  Columns from rank to ldu, and rows without a slot, are zero.
+// k * f_k + j * f_j.  Columns from rank to ldu, and rows without a slot, are zero.  With W (the output layer of few
+// classes) one pass over x gives the logits too: y = x W + bias + u B, B the slot's [rank][out] matrix.
 struct LowArgs {
     const float* x;      // [rows][ldx], 16-byte aligned rows
     const float* factor; // slot 0's matrix
@@ -185,55 +186,95 @@ struct LowArgs {
     uint32_t rows;
     int ldx, K, f_k, f_j, rank, ldu;
     float scale;
+    int parts;           // the slots of a tile are dealt to this many workgroups (few tiles of many slots)
+    // the output layer
+    const float *W, *bias, *up;
+    uint64_t up_slot;
+    float* y;
+    int out, ldy;
 };
 
-// 32 rows per workgroup on v_mfma_f32_16x16x4_f32, the K range split over its four waves and joined in LDS.
-// A step pairs lane group q's k with k0 + 4 q + t, so that a lane reads 16 bytes of its row for four steps.
-template <int NT>
-__global__ __launch_bounds__(256) void low_kernel(LowArgs a)
+// 32 rows per workgroup on v_mfma_f32_16x16x4_f32, the K range split over its waves and joined in LDS.  A step
+// pairs lane group q's k with k0 + 4 q + t, so that a lane reads 16 bytes of its row for four steps.  UNR blocks of
+// 16 k are requested at once: with as many rows as there are, what a wave does is wait.  NT tiles of 16
+// columns: OT of the output layer, then the rank's.  A column beyond the matrix takes another's values and is dropped.
+template <int NT, int OT, int WAVES, int UNR>
+__global__ __launch_bounds__(64 * WAVES) void low_kernel(LowArgs a)
 {
-    __shared__ __attribute__((aligned(16))) float part[4][32][NT * 16];
+    extern __shared__ __attribute__((aligned(16))) float low_lds[];
+    float (*part)[32][NT * 16] = reinterpret_cast<float (*)[32][NT * 16]>(low_lds);
+    constexpr int RT = NT - OT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r16 = lane & 15, q = lane >> 4;
     const uint32_t row0 = blockIdx.x * 32;
     const uint32_t my_row = row0 + (lane & 31);
     const int mine = my_row < a.rows ? a.row_slot[my_row] : -1;
-    uint32_t left = (uint32_t)__ballot(mine >= 0);
-    const int blocks = (a.K + 15) / 16, per = (blocks + 3) / 4;
-    const int b0 = wave * per, b1 = min(blocks, b0 + per);
+    // rows without an adapter are a group of their own (slot -1), which the output layer computes with u = 0
+    uint32_t left = (uint32_t)__ballot(my_row < a.rows && (OT > 0 || mine >= 0));
+    const int blocks = (a.K + 15) / 16, per = (blocks + WAVES - 1) / WAVES;
+    const int b0 = wave * per, b1 = min(blocks, b0 + per), full = min(b1, a.K / 16);
     const float* x[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) x[t] = a.x + (size_t)min(row0 + 16 * t + r16, a.rows - 1) * a.ldx + 4 * q;
-    // rows without an adapter
-    const uint32_t none = ~left;
-    for (int e = threadIdx.x; e < 32 * a.ldu; e += 256) {
-        const int r = e / a.ldu;
-        if (row0 + r < a.rows && ((none >> r) & 1u)) a.u[(size_t)(row0 + r) * a.ldu + e % a.ldu] = 0.0f;
+    if (OT == 0 && blockIdx.y == 0) {
+        const uint32_t none = ~left;
+        for (int e = threadIdx.x; e < 32 * a.ldu; e += 64 * WAVES) {
+            const int r = e / a.ldu;
+            if (row0 + r < a.rows && ((none >> r) & 1u)) a.u[(size_t)(row0 + r) * a.ldu + e % a.ldu] = 0.0f;
+        }
     }
-    while (left) {
+    for (int turn = 0; left; ++turn) {
         const int slot = __builtin_amdgcn_readlane(mine, __builtin_ctz(left));
-        const uint32_t member = (uint32_t)__ballot(mine == slot);
+        const uint32_t member = (uint32_t)__ballot(mine == slot) & left;
         left &= ~member;
-        const float* f = a.factor + (size_t)slot * a.factor_slot;
+        if (turn % a.parts != (int)blockIdx.y) continue;
+        const float* f = a.factor + (size_t)max(slot, 0) * a.factor_slot;
+        const float* col[NT];
+        uint32_t step[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if (n < OT) { col[n] = a.W + min(16 * n + r16, a.out - 1); step[n] = (uint32_t)a.out; }
+            else { col[n] = f + (size_t)min(16 * (n - OT) + r16, a.rank - 1) * a.f_j; step[n] = (uint32_t)a.f_k; }
+        }
         f32x4 acc[2][NT];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int b = b0; b < b1; ++b) {
+        int b = b0;
+        for (; b + UNR <= full; b += UNR) {
+            f32x4 xv[UNR][2];
+            float w[UNR][4][NT];
+#pragma unroll
+            for (int i = 0; i < UNR; ++i) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) xv[i][t] = *reinterpret_cast<const f32x4*>(x[t] + 16 * (b + i));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) w[i][e][n] = col[n][(uint32_t)(16 * (b + i) + 4 * q + e) * step[n]];
+            }
+#pragma unroll
+            for (int i = 0; i < UNR; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[i][t][e], w[i][e][n], acc[t][n], 0, 0, 0);
+        }
+        for (; b < b1; ++b) {
             f32x4 xv[2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) xv[t] = *reinterpret_cast<const f32x4*>(x[t] + 16 * b);
-            const int k0 = 16 * b + 4 * q;
+            for (int t = 0; t < 2; ++t) xv[t] = *reinterpret_cast<const f32x4*>(x[t] + min(16 * b, a.ldx - 4 - 4 * q));
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const bool in_k = k0 + e < a.K;
-                const float* fk = f + (size_t)min(k0 + e, a.K - 1) * a.f_k;
+                const int k = 16 * b + 4 * q + e;
+                const bool in_k = k < a.K;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const int j = 16 * n + r16;
-                    float v = fk[(size_t)min(j, a.rank - 1) * a.f_j];
-                    v = in_k && j < a.rank ? v : 0.0f;
+                    float v = col[n][(uint32_t)min(k, a.K - 1) * step[n]];
+                    v = in_k ? v : 0.0f;
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
                         acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(in_k ? xv[t][e] : 0.0f, v, acc[t][n], 0, 0, 0);
@@ -247,10 +288,30 @@ __global__ __launch_bounds__(256) void low_kernel(LowArgs a)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) part[wave][16 * t + 4 * q + i][16 * n + r16] = acc[t][n][i];
         __syncthreads();
-        for (int e = threadIdx.x; e < 32 * NT * 16; e += 256) {
-            const int r = e / (NT * 16), j = e % (NT * 16);
-            if (j < a.ldu && row0 + r < a.rows && ((member >> r) & 1u))
-                a.u[(size_t)(row0 + r) * a.ldu + j] = a.scale * ((part[0][r][j] + part[1][r][j]) + (part[2][r][j] + part[3][r][j]));
+        for (int e = threadIdx.x; e < 32 * RT * 16; e += 64 * WAVES) {
+            const int r = e / (RT * 16), j = e % (RT * 16);
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) s += part[w][r][OT * 16 + j];
+            s = slot >= 0 && j < a.rank ? a.scale * s : 0.0f;
+            if (j < a.ldu && row0 + r < a.rows && ((member >> r) & 1u)) a.u[(size_t)(row0 + r) * a.ldu + j] = s;
+            if (OT > 0) part[0][r][OT * 16 + j] = s;  // (read by this thread alone before)
+        }
+        if (OT > 0) {
+            __syncthreads();
+            const float* up = a.up + (size_t)max(slot, 0) * a.up_slot;
+            for (int e = threadIdx.x; e < 32 * OT * 16; e += 64 * WAVES) {
+                const int r = e / (OT * 16), c = e % (OT * 16);
+                if (c >= a.out || row0 + r >= a.rows || !((member >> r) & 1u)) continue;
+                float s = 0.0f, v = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) s += part[w][r][c];
+                if (slot >= 0) {
+#pragma unroll 4
+                    for (int j = 0; j < a.rank; ++j) v = __builtin_fmaf(part[0][r][OT * 16 + j], up[(size_t)j * a.out + c], v);
+                }
+                a.y[(size_t)(row0 + r) * a.ldy + c] = s + v + a.bias[c];
+            }
         }
         __syncthreads();
     }

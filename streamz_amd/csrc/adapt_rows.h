@@ -277,6 +277,8 @@ __global__ __launch_bounds__(kRowT) void row_out_kernel(RowArgs a, Controls ctl,
 
 // C = act(A W + add + bias) for few rows: a workgroup computes a 32 x 32 tile, its eight waves a part of k each
 // (v_mfma_f32_32x32x2_f32, operands straight from memory), joined in LDS.  A step pairs k = e with k = 4 + e of eight.
+// add: a matrix (few rows: row_hidden_kernel made it), or the rows' low-rank part as in adapt_add, the tile's slots
+// dealt to the waves.
 struct ThinArgs {
     const float* A; uint64_t lda;   // [M][K], 16-byte aligned rows
     const float* W;                 // [K][N]
@@ -284,19 +286,62 @@ struct ThinArgs {
     const float* bias;
     float* C; uint64_t ldc;
     int M, N, K;
+    const float *low, *up;          // add == nullptr
+    const int32_t* row_slot;
+    uint64_t up_slot;
+    int ld_low, rank;
 };
 constexpr int kThinWaves = 8;
 template <bool TANH>
 __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(ThinArgs g)
 {
-    __shared__ __attribute__((aligned(16))) float part[kThinWaves][32][32];
+    __shared__ __attribute__((aligned(16))) float part[kThinWaves + 1][32][32];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l31 = lane & 31, half = lane >> 5;
     const int n0 = blockIdx.x * 32, m0 = blockIdx.y * 32;
     const int blocks = (g.K + 7) / 8, per = (blocks + kThinWaves - 1) / kThinWaves;
     const int b0 = wave * per, b1 = min(blocks, b0 + per);
-    const float* a = g.A + (uint64_t)min(m0 + l31, g.M - 1) * g.lda + 4 * half;
-    const float* w = g.W + (uint64_t)(4 * half) * g.N + min(n0 + l31, g.N - 1);
+    const int row = min(m0 + l31, g.M - 1), col = min(n0 + l31, g.N - 1);
+    const float* a = g.A + (uint64_t)row * g.lda + 4 * half;
+    const float* w = g.W + (uint64_t)(4 * half) * g.N + col;
     gemm::f32x16 acc;
+    if (!g.add) {
+        const int mine = m0 + l31 < g.M ? g.row_slot[m0 + l31] : -1;
+        uint32_t left = (uint32_t)__ballot(mine >= 0);
+        if (wave == 0) {
+            for (int r = half; r < 32; r += 2)
+                if (!((left >> r) & 1u)) part[kThinWaves][r][l31] = 0.0f;
+        }
+        const int steps = g.ld_low >> 1;  // a multiple of 4; a step pairs k = st with k = st + steps
+        const float* low = g.low + (uint64_t)row * g.ld_low + half * steps;
+        for (int turn = 0; left; ++turn) {
+            const int slot = __builtin_amdgcn_readlane(mine, __builtin_ctz(left));
+            const uint32_t member = (uint32_t)__ballot(mine == slot);
+            left &= ~member;
+            if (turn % kThinWaves != wave) continue;
+            const float* up = g.up + (uint64_t)slot * g.up_slot + col;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+#pragma unroll 2
+            for (int st = 0; st < steps; st += 4) {
+                const float4 a4 = *reinterpret_cast<const float4*>(low + st);
+                const float av[4] = {a4.x, a4.y, a4.z, a4.w};
+                float bv[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int k = half * steps + st + j;
+                    bv[j] = up[(uint64_t)min(k, g.rank - 1) * g.N];
+                    bv[j] = k < g.rank ? bv[j] : 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(av[j], bv[j], acc, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int m = (r & 3) + 8 * (r >> 2) + 4 * half;
+                if ((member >> m) & 1u) part[kThinWaves][m][l31] = acc[r];
+            }
+        }
+    }
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
     const int full = min(b1, g.K / 8);   // blocks that lie inside K
@@ -336,7 +381,7 @@ __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(ThinArgs g)
         float s = 0.0f;
 #pragma unroll
         for (int p = 0; p < kThinWaves; ++p) s += part[p][m][n];
-        s += g.add[(uint64_t)(m0 + m) * g.ldadd + n0 + n];
+        s += g.add ? g.add[(uint64_t)(m0 + m) * g.ldadd + n0 + n] : part[kThinWaves][m][n];
         s += g.bias[n0 + n];
         g.C[(uint64_t)(m0 + m) * g.ldc + n0 + n] = TANH ? gemm::fast_tanh(s) : s;
     }

@@ -276,7 +276,7 @@ __global__ __launch_bounds__(XW_THREADS) void gemm_x3w_kernel(GemmArgs g)
             multiply(L + XW_STAGE, 2);
             __syncthreads();
         }
-        if constexpr (EPI >= EPI_ADAPT_TANH) adapt_add<TN, WN>(g, acc, cur.m0, cur.n0, wm, wn, l31, half);
+        if constexpr (EPI >= EPI_ADAPT_TANH) adapt_add<TN, WN, 1>(g, acc, cur.m0, cur.n0, wm, wn, l31, half);
         finish_tile<plain_epi(EPI), XW_TM, TN, WN>(g, C, acc, cur.m0, cur.n0, wm, wn, l31, half);
         if (!has_next) break;
         tile = next;
@@ -459,7 +459,7 @@ __global__ __launch_bounds__(XW_THREADS) void gemm_f32w_kernel(GemmArgs g)
             fa.template stash<1>(L + FW_STAGE);
             fb.template stash<1>(L + FW_STAGE + FW_OPER);
         }
-        if constexpr (EPI >= EPI_ADAPT_TANH) adapt_add<TN, WN>(g, acc, cur.m0, cur.n0, wm, wn, l31, half);
+        if constexpr (EPI >= EPI_ADAPT_TANH) adapt_add_lds<TN, WN>(g, acc, L + 2 * FW_STAGE, cur.m0, cur.n0, wm, wn, l31, half);
         finish_tile<plain_epi(EPI), XW_TM, TN, WN>(g, C, acc, cur.m0, cur.n0, wm, wn, l31, half);
         if (!has_next) break;
         tile = next;

@@ -71,6 +71,7 @@ struct GemmArgs {
     const float* low = nullptr;
     const float* up = nullptr;
     const int32_t* row_slot = nullptr;
+    const uint32_t* row_begin = nullptr;  // [slot] first row of the slot, [slot + 1] the row behind its last (adapt_add_lds)
     uint64_t up_slot = 0;
     int ld_low = 0, rank = 0, up_k = 0, up_n = 0;
 };
@@ -320,7 +321,8 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& g, float* C, f32x16 
 // that slot's rows alone: zero factors for the other rows instead would let an inf or NaN in one request's
 // adapter reach its neighbours, and a row's sum would be rounded by the company it is in.
 // A step pairs k = st with st + ld_low / 2, so a lane's values of `low` are contiguous.
-template <int TN, int WN>
+// GROUP: column tiles whose sums are formed side by side (their operands are requested together).
+template <int TN, int WN, int GROUP>
 __device__ __forceinline__ void adapt_add(const GemmArgs& g, f32x16 (&acc)[2][TN], int m0, int n0, int wm, int wn, int l31,
                                           int half)
 {
@@ -338,28 +340,103 @@ __device__ __forceinline__ void adapt_add(const GemmArgs& g, f32x16 (&acc)[2][TN
             const uint32_t rows = member >> (4 * half);
             const float* up = g.up + (size_t)slot * g.up_slot;
 #pragma unroll
-            for (int tn = 0; tn < TN; ++tn) {
-                const int col = min(n0 + wn * WN + tn * 32 + l31, g.N - 1);
-                const float* u = up + (size_t)col * g.up_n;
-                f32x16 c;
+            for (int tn = 0; tn < TN; tn += GROUP) {
+                f32x16 c[GROUP];
+                uint32_t at[GROUP];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) c[r] = 0.0f;
+                for (int t = 0; t < GROUP; ++t) {
+                    at[t] = (uint32_t)min(n0 + wn * WN + (tn + t) * 32 + l31, g.N - 1) * (uint32_t)g.up_n;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) c[t][r] = 0.0f;
+                }
+#pragma unroll 2
                 for (int st = 0; st < steps; st += 4) {
                     const float4 a4 = *reinterpret_cast<const float4*>(low + st);
                     const float av[4] = {a4.x, a4.y, a4.z, a4.w};
+                    float b[4][GROUP];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int k = half * steps + st + j;
-                        float b = u[(size_t)min(k, g.rank - 1) * g.up_k];
-                        b = k < g.rank ? b : 0.0f;
-                        c = __builtin_amdgcn_mfma_f32_32x32x2f32(av[j], b, c, 0, 0, 0);
+#pragma unroll
+                        for (int t = 0; t < GROUP; ++t) {
+                            b[j][t] = up[at[t] + (uint32_t)min(k, g.rank - 1) * (uint32_t)g.up_k];
+                            b[j][t] = k < g.rank ? b[j][t] : 0.0f;
+                        }
                     }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int t = 0; t < GROUP; ++t) c[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(av[j], b[j][t], c[t], 0, 0, 0);
                 }
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if ((rows >> ((r & 3) + 8 * (r >> 2))) & 1u) acc[tm][tn][r] += c[r];
+                for (int t = 0; t < GROUP; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if ((rows >> ((r & 3) + 8 * (r >> 2))) & 1u) acc[tm][tn + t][r] += c[t][r];
             }
         }
+    }
+}
+
+// The same for the 256 x 256 tiles, whose one workgroup per compute unit has nothing else to run while it waits
+// for the factors: the tile's rank columns and the slot's factor go through LDS, 32 of rank at a time, in one
+// request each.  Slots are taken from the sorted rows, so all waves walk them together.
+constexpr int AL_LDA = 36, AL_LDB = 260;
+constexpr size_t AL_BYTES = (256 * AL_LDA + 32 * AL_LDB) * sizeof(float);
+template <int TN, int WN>
+__device__ __forceinline__ void adapt_add_lds(const GemmArgs& g, f32x16 (&acc)[2][TN], float* lds, int m0, int n0, int wm, int wn, int l31,
+                                              int half)
+{
+    float* As = lds;
+    float* Bs = lds + 256 * AL_LDA;
+    const int t = threadIdx.x;
+    const int end = min(g.M, m0 + 256);
+    const int steps_all = g.ld_low;
+    for (int r = m0; r < end;) {
+        const int slot = __builtin_amdgcn_readfirstlane(g.row_slot[r]);
+        if (slot < 0) break;  // rows without an adapter are the last
+        const int stop = min(end, (int)g.row_begin[slot + 1]);
+        const float* up = g.up + (size_t)slot * g.up_slot;
+        for (int k0 = 0; k0 < steps_all; k0 += 32) {
+            const int kn = min(32, steps_all - k0), steps = kn >> 1;
+            {
+                const float* low = g.low + (size_t)min(m0 + (t >> 1), g.M - 1) * g.ld_low + k0 + (t & 1) * steps;
+                float* dst = As + (t >> 1) * AL_LDA + (t & 1) * steps;
+                for (int q = 0; q < steps; q += 4) *reinterpret_cast<float4*>(dst + q) = *reinterpret_cast<const float4*>(low + q);
+                const int c = t & 255;
+                const float* u = up + (size_t)min(n0 + c, g.N - 1) * g.up_n;
+#pragma unroll 4
+                for (int k = t >> 8; k < kn; k += 2) Bs[k * AL_LDB + c] = k0 + k < g.rank ? u[(size_t)(k0 + k) * g.up_k] : 0.0f;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int tm = 0; tm < 2; ++tm) {
+                const int base = m0 + wm * 64 + tm * 32;
+                const int lo = max(r - base, 0), hi = min(stop - base, 32);
+                if (lo >= hi) continue;
+                const uint32_t member = (hi >= 32 ? 0xffffffffu : (1u << hi) - 1u) & ~((1u << lo) - 1u);
+                const uint32_t rows = member >> (4 * half);
+                const float* a = As + (wm * 64 + tm * 32 + l31) * AL_LDA + half * steps;
+#pragma unroll
+                for (int tn = 0; tn < TN; ++tn) {
+                    const float* b = Bs + half * steps * AL_LDB + wn * WN + tn * 32 + l31;
+                    f32x16 c;
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) c[q] = 0.0f;
+                    for (int st = 0; st < steps; st += 4) {
+                        const float4 a4 = *reinterpret_cast<const float4*>(a + st);
+                        const float av[4] = {a4.x, a4.y, a4.z, a4.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(av[j], b[(st + j) * AL_LDB], c, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int q = 0; q < 16; ++q)
+                        if ((rows >> ((q & 3) + 8 * (q >> 2))) & 1u) acc[tm][tn][q] += c[q];
+                }
+            }
+            __syncthreads();
+        }
+        r = stop;
     }
 }
 
@@ -522,7 +599,7 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_kernel(GemmArgs g)
         }
     }
 
-    if constexpr (EPI >= EPI_ADAPT_TANH) adapt_add<TN, WN>(g, acc, m0, n0, wm, wn, l31, half);
+    if constexpr (EPI >= EPI_ADAPT_TANH) adapt_add<TN, WN, 1>(g, acc, m0, n0, wm, wn, l31, half);
     finish_tile<plain_epi(EPI), TM, TN, WN>(g, C, acc, m0, n0, wm, wn, l31, half);
 }
 

@@ -49,6 +49,20 @@ int launch_gemm(GemmArgs g, int splits, hipStream_t s)
     return SZH_OK;
 }
 
+// the same with the row tile chosen by the caller
+template <int AM, int BMd, int EPI, int TAG, int TM>
+int launch_gemm_rows(GemmArgs g, hipStream_t s)
+{
+    if (g.M <= 0 || g.N <= 0) return SZH_OK;
+    g.a_vec = vec_ok(g.A, g.lda);
+    g.b_vec = vec_ok(g.B, g.ldb);
+    ProfScope prof(kGemmTagName[TAG], s);
+    hipLaunchKernelGGL((gemm_kernel<AM, BMd, EPI, TAG, TM, kGemmKT, kGemmDB>), dim3((g.N + BN - 1) / BN, (g.M + TM - 1) / TM),
+                       dim3(kGemmThreads), 0, s, g);
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
+}
+
 int compute_units()
 {
     static int cus[64] = {};
@@ -84,12 +98,13 @@ template <int EPI, int TAG, int SRC = X3_ROWS_F32>
 int launch_gemm_f32w(GemmArgs g, hipStream_t s, int splits = 1)
 {
     if (g.M <= 0 || g.N <= 0) return SZH_OK;
-    if (int rc = allow_dynamic_lds((const void*)gemm_f32w_kernel<SRC, SRC, EPI, TAG>, FW_LDS_BYTES)) return rc;
+    constexpr size_t lds = FW_LDS_BYTES + (EPI >= EPI_ADAPT_TANH ? AL_BYTES : 0);
+    if (int rc = allow_dynamic_lds((const void*)gemm_f32w_kernel<SRC, SRC, EPI, TAG>, lds)) return rc;
     ProfScope prof(kGemmTagName[TAG], s);
     g.tiles_x = (g.N + XW_TN - 1) / XW_TN; g.tiles_y = (g.M + XW_TM - 1) / XW_TM; g.tiles_z = splits;
     const int tiles = g.tiles_x * g.tiles_y * g.tiles_z;
     const int blocks = std::min((tiles + 7) / 8 * 8, compute_units() / 8 * 8);
-    hipLaunchKernelGGL((gemm_f32w_kernel<SRC, SRC, EPI, TAG>), dim3(blocks), dim3(XW_THREADS), FW_LDS_BYTES, s, g);
+    hipLaunchKernelGGL((gemm_f32w_kernel<SRC, SRC, EPI, TAG>), dim3(blocks), dim3(XW_THREADS), lds, s, g);
     SZ_HIP(hipGetLastError());
     return SZH_OK;
 }
