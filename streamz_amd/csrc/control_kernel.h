@@ -66,19 +66,33 @@ __device__ __forceinline__ float exp_low(float x)
     return __builtin_fmaf(e, r * kLn2, e);
 }
 
+// Joins a value over LANES neighbouring lanes: within 16 by the register file's own lane exchanges (pairs, pairs of
+// pairs, mirrored halves, mirrored rows: after each step all lanes of the smaller group hold the same), beyond by shuffles.
+template <int CTRL>
+__device__ __forceinline__ float lane_move(float v)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
+template <int LANES, class F>
+__device__ __forceinline__ float lanes_join(float v, F f)
+{
+    if (LANES > 1) v = f(v, lane_move<0xB1>(v));
+    if (LANES > 2) v = f(v, lane_move<0x4E>(v));
+    if (LANES > 4) v = f(v, lane_move<0x141>(v));
+    if (LANES > 8) v = f(v, lane_move<0x140>(v));
+    if (LANES > 16) v = f(v, __shfl_xor(v, 16));
+    if (LANES > 32) v = f(v, __shfl_xor(v, 32));
+    return v;
+}
 template <int LANES>
 __device__ __forceinline__ float lanes_max(float v)
 {
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    return lanes_join<LANES>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 template <int LANES>
 __device__ __forceinline__ float lanes_sum(float v)
 {
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    return lanes_join<LANES>(v, [](float a, float b) { return a + b; });
 }
 // the last of the largest values over the lanes: (p, c) pairs, c = -1 for none
 template <int LANES>

@@ -249,13 +249,14 @@ int identify_tiled(Net* n, Extractor* e, const int16_t* pcm, bool pcm_on_device,
 
 // ---- gradient clipping (clip.hip) ------------------------------------------------------
 struct ClipTensor { const float* src; float* dst; uint64_t len; uint32_t group; };
-struct ClipPiece { const float* src; float* dst; uint32_t len, group; };
+struct ClipPiece { const float* src; float* dst; uint32_t len, group, vec; };  // vec: both addresses are multiples of 16
 struct Clip {
     ClipPiece* d_pieces = nullptr;  // ordered by group
     double* d_part = nullptr;       // each piece's sum of squares
     uint32_t* d_first = nullptr;    // [groups + 1] first piece of each group
     uint32_t n_pieces = 0, groups = 0;
     bool has_empty = false;         // a group without elements
+    bool fold = false;              // a group of more pieces than every workgroup should add for itself
     const float* live = nullptr;    // the group's norm is that of its tensors divided by live[group * live_step]
     uint32_t live_step = 1;
     int device = 0;
