@@ -37,8 +37,11 @@ using namespace adapt;
 // Rows per pass: a call with more is walked in pieces, whose workspace does not grow with it.
 constexpr uint64_t kAdaptRows = 131072;
 
-// Calls of up to this many rows go row by row (adapt_rows.h).
-constexpr uint64_t kFewRows = 1024;
+// Calls of up to this many rows go row by row (adapt_rows.h); of half as many in training, whose row kernels do more.
+// Forward, on rows and on tiles: 23 and 36 us at 256 rows of 60-512-256-16, 38 and 40 at 512, 65 and 47 at 1024; 58 and
+// 87 us at 64 rows of 60-2048-2048-256, 124 and 149 at 512, 222 and 178 at 1024.  Training: 61 and 80 us at 256 rows of the
+// small network, 93 and 92 at 512.
+constexpr uint64_t kFewRows = 512;
 
 inline int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
@@ -47,6 +50,17 @@ bool capturing(hipStream_t s)
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     return hipStreamIsCapturing(s, &st) == hipSuccess && st == hipStreamCaptureStatusActive;
 }
+
+// Rows per chunk of the factor gradients: enough workgroups (tiles x chunks) to fill the chip twice, no more than 512
+// rows (the sums of a chunk's rows are joined by a second launch), no less than 64.
+int factor_tiles(const Adapters* a) { return (int)((a->h1 + 63) / 64 + 2 * ((a->h2 + 63) / 64) + (a->out + 63) / 64); }
+uint32_t factor_chunk(const Adapters* a, uint64_t rows)
+{
+    const uint64_t want = std::max<uint64_t>(1, 1024 / factor_tiles(a));
+    return (uint32_t)std::min<uint64_t>(512, std::max<uint64_t>(64, (rows / want + 63) / 64 * 64));
+}
+// most chunks that a call of up to `rows` rows makes
+uint64_t factor_chunks_most(const Adapters* a, uint64_t rows) { return std::max<uint64_t>(rows / 512, 1024 / factor_tiles(a)) + 2; }
 
 // How the arrays of a pass lie in the workspace; `base` null: only the size.
 size_t lay_out(const Adapters* a, uint64_t rows, bool training, char* base, AdaptWorkspace* w)
@@ -70,9 +84,8 @@ size_t lay_out(const Adapters* a, uint64_t rows, bool training, char* base, Adap
     take(o.w1t, (uint64_t)a->h1 * o.ldx); take(o.w2t, (uint64_t)o.ld1 * a->h2); take(o.w3t, (uint64_t)o.ld2 * std::max(a->out, 1u));
     take(o.w2s, 3 * ((uint64_t)a->h1 * a->h2 + 1) / 2 + 4);
     if (training) {
-        const uint64_t chunks = (rows + kFactorRows - 1) / kFactorRows;
         take(o.d2, (rows + 32) * o.ld2); take(o.g2, rows * o.ldu); take(o.g3, rows * o.ldu); take(o.loss, rows);
-        take(o.slab, (chunks + S) * a->per_slot());
+        take(o.slab, (factor_chunks_most(a, rows) + S) * a->per_slot());
     }
     return at;
 }
@@ -117,6 +130,13 @@ int group_rows(Adapters* a, const int32_t* slots_dev, uint32_t rows, hipStream_t
     ProfScope prof("adapt_group", s);
     if (blocks == 1) {
         hipLaunchKernelGGL(group_few_kernel, dim3(1), dim3(64), lds, s, slots_dev, rows, S, w.begin, w.order, w.row_slot);
+        SZ_HIP(hipGetLastError());
+        return SZH_OK;
+    }
+    if (blocks <= kGroupWaves && S <= kGroupMidSlots) {
+        const size_t mid = (size_t)kGroupWaves * (S + 1) * sizeof(uint32_t);
+        if (int rc = allow_dynamic_lds((const void*)group_mid_kernel, mid)) return rc;
+        hipLaunchKernelGGL(group_mid_kernel, dim3(1), dim3(64 * kGroupWaves), mid, s, slots_dev, rows, S, w.begin, w.order, w.row_slot);
         SZ_HIP(hipGetLastError());
         return SZH_OK;
     }
@@ -193,7 +213,9 @@ int factor_gradients(Adapters* a, uint32_t rows, hipStream_t s)
     g.job[1] = {w.d2, w.u2, nullptr, a->off_b2(), w.ld2, h2, 1, h2, 0, 0};
     g.job[2] = {w.h2, w.g3, nullptr, a->off_a3(), w.ld2, h2, r, 1, 0, 0};
     g.job[3] = {w.lg, w.u3, nullptr, a->off_b3(), w.ld3, out, 1, out, 0, 0};
-    const uint64_t chunks = (rows + kFactorRows - 1) / kFactorRows;
+    g.chunk = factor_chunk(a, rows);
+    const uint64_t chunks = (rows + g.chunk - 1) / g.chunk;
+    if (chunks > factor_chunks_most(a, a->ws_rows)) { set_error("adapters: more chunks than the workspace holds"); return SZH_EINVAL; }
     float* slab = w.slab;
     int tiles = 0, blocks = 0;
     for (FactorJob& j : g.job) {
@@ -211,6 +233,28 @@ int factor_gradients(Adapters* a, uint32_t rows, hipStream_t s)
     default: hipLaunchKernelGGL((factor_grad_kernel<4>), grid, block, 0, s, g); break;
     }
     hipLaunchKernelGGL(factor_reduce_kernel, dim3(blocks, a->slots), block, 0, s, g, a->d_grad, a->per_slot());
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
+}
+
+// d3 -> g3, d2, g2 in one launch; up to 64 classes (beyond them the product with w3 wants larger tiles)
+bool back_applies(const Adapters* a) { return a->out <= 64; }
+int back_rows(const Net* n, const Adapters* a, uint32_t rows, hipStream_t s)
+{
+    const AdaptWorkspace& w = a->ws;
+    const float* F = a->d_params;
+    BackArgs g{};
+    g.d3 = w.lg; g.h2 = w.h2; g.w3 = n->d_params + n->off_w3(); g.a3 = F + a->off_a3(); g.b3 = F + a->off_b3(); g.b2 = F + a->off_b2();
+    g.per_slot = a->per_slot(); g.row_slot = w.row_slot; g.d2 = w.d2; g.g2 = w.g2; g.g3 = w.g3; g.rows = rows;
+    g.n2 = (int)n->h2; g.out = (int)n->out; g.rank = (int)a->rank; g.ld2 = w.ld2; g.ld3 = w.ld3; g.ldu = w.ldu; g.scale = a->scale;
+    const dim3 grid((rows + 31) / 32);
+    ProfScope prof("adapt_back", s);
+    switch ((a->rank + 15) / 16) {
+    case 1: hipLaunchKernelGGL((back_kernel<1, 8>), grid, dim3(512), 0, s, g); break;
+    case 2: hipLaunchKernelGGL((back_kernel<2, 8>), grid, dim3(512), 0, s, g); break;
+    case 3: hipLaunchKernelGGL((back_kernel<3, 4>), grid, dim3(256), 0, s, g); break;
+    default: hipLaunchKernelGGL((back_kernel<4, 4>), grid, dim3(256), 0, s, g); break;
+    }
     SZ_HIP(hipGetLastError());
     return SZH_OK;
 }
@@ -348,9 +392,9 @@ int forward_rows(Net* n, Adapters* a, uint32_t rows, hipStream_t s)
 }
 
 // Whether a call takes the few-row path: its row kernels hold a row's activations in LDS.
-bool few_rows(const Net* n, uint64_t rows)
+bool few_rows(const Net* n, uint64_t rows, bool training)
 {
-    return rows <= kFewRows && n->in + n->h1 + 2 * n->h2 + n->out <= 24576;
+    return rows <= (training ? kFewRows / 2 : kFewRows) && n->in + n->h1 + 2 * n->h2 + n->out <= 24576;
 }
 
 // w3 beyond this is not streamed by every row: the logits become a product of their own
@@ -430,7 +474,7 @@ Controls from_row(const Controls& c, uint64_t r0)
 // one pass of a forward or vote call
 int infer_rows(Net* n, Adapters* a, const float* x, const int32_t* slots_dev, uint32_t rows, const Controls& ctl, ControlRun c, hipStream_t s)
 {
-    if (few_rows(n, rows)) return forward_few(n, a, x, n->in, slots_dev, rows, ctl, c, nullptr, nullptr, s);
+    if (few_rows(n, rows, false)) return forward_few(n, a, x, n->in, slots_dev, rows, ctl, c, nullptr, nullptr, s);
     int rc = group_rows(a, slots_dev, rows, s);
     if (!rc) rc = gather_rows(a, x, rows, 0.0f, 0, 0, nullptr, s);
     if (!rc) rc = forward_rows(n, a, rows, s);
@@ -557,12 +601,16 @@ int adapters_accumulate(Net* n, Adapters* a, const float* x, const int32_t* labe
         c.in = w.lg; c.ld_in = w.ld3; c.rows = R; c.classes = n->out; c.order = w.order;
         c.out = w.lg; c.ld_out = w.ld3; c.labels = labels + r0; c.row_live = w.live0; c.row_slot = w.row_slot; c.loss = w.loss; c.live = w.live;
         const Controls ctl_r = from_row(ctl, r0);
-        const bool few = few_rows(n, R);
+        const bool few = few_rows(n, R, true);
         if (!rc && few) rc = forward_few(n, a, w.xs, w.ldx, w.row_slot, R, ctl_r, c, w.u2, w.u3, s);
         if (!rc && !few) rc = forward_rows(n, a, R, s);
         if (!rc && !few) rc = control_run(ctl_r, c, s);   // lg now holds d3
         if (rc) return rc;
-        if (!few || (uint64_t)n->h2 * n->out > kRowOutFloats) {
+        const bool back_done = few && (uint64_t)n->h2 * n->out <= kRowOutFloats;  // (by the row kernel)
+        if (!back_done && back_applies(a)) {
+            rc = back_rows(n, a, R, s);
+            if (rc) return rc;
+        } else if (!back_done) {
             rc = low_product(a, w.lg, w.ld3, out, F + a->off_b3(), 1, out, R, w.g3, s);
             if (rc) return rc;
             GemmArgs g{};

@@ -146,6 +146,59 @@ __global__ __launch_bounds__(64) void group_few_kernel(const int32_t* __restrict
     place_rows(slot, 0, rows, slots, next, order, row_slot);
 }
 
+// ... and for up to kGroupWaves blocks, a wave each
+constexpr int kGroupWaves = 16, kGroupMidSlots = 1000;
+__global__ __launch_bounds__(64 * kGroupWaves) void group_mid_kernel(const int32_t* __restrict__ slot, uint32_t rows, int slots,
+                                                                     uint32_t* __restrict__ begin, uint32_t* __restrict__ order,
+                                                                     int32_t* __restrict__ row_slot)
+{
+    extern __shared__ uint32_t hist[];  // [kGroupWaves][slots + 1]
+    __shared__ uint32_t carry[kGroupWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, keys = slots + 1;
+    for (int e = threadIdx.x; e < kGroupWaves * keys; e += 64 * kGroupWaves) hist[e] = 0;
+    __syncthreads();
+    uint32_t* mine = hist + wave * keys;
+    const uint32_t per = ((rows + kGroupWaves - 1) / kGroupWaves + 63) & ~63u;
+    const uint32_t r0 = min(rows, wave * per), r1 = min(rows, r0 + per);
+    for (uint32_t r = r0 + lane; r < r1; r += 64) atomicAdd(&mine[group_key(slot, r, slots)], 1u);
+    __syncthreads();
+    // keys in order, the waves of a key in order: a thread per key (keys <= 64 kGroupWaves) adds its waves up
+    uint32_t sum = 0;
+    const int k = threadIdx.x;
+    if (k < keys)
+        for (int w = 0; w < kGroupWaves; ++w) { const uint32_t v = hist[w * keys + k]; hist[w * keys + k] = sum; sum += v; }
+    const uint32_t inc = wave_scan(sum);
+    if (lane == 63) carry[wave] = inc;
+    __syncthreads();
+    uint32_t base = inc - sum;
+    for (int w = 0; w < wave; ++w) base += carry[w];
+    if (k < keys) {
+        begin[k] = base;
+        for (int w = 0; w < kGroupWaves; ++w) hist[w * keys + k] += base;
+    }
+    if (threadIdx.x == 0) begin[slots + 1] = rows;
+    __syncthreads();
+    // as place_rows, the wave's lanes in step by themselves: their LDS accesses are in program order
+    for (uint32_t r = r0; r < r1; r += 64) {
+        const bool in = r + lane < r1;
+        const int key = in ? group_key(slot, r + lane, slots) : 0;
+        uint32_t place = 0;
+        each_key(key, in, [&](int kk, unsigned long long member) {
+            const uint32_t at = mine[kk];
+            __builtin_amdgcn_wave_barrier();
+            if (in && key == kk) place = at + (uint32_t)__popcll(member & ((1ull << lane) - 1));
+            if (lane == 0) mine[kk] = at + (uint32_t)__popcll(member);
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+        });
+        if (in) {
+            order[place] = r + lane;
+            row_slot[place] = key < slots ? key : -1;
+        }
+    }
+}
+
 // ---- rows in that order -------------------------------------------------------------------------
 // xs[i] = [x[order[i]] | 1 | 0 ...] with input dropout (element j of row r zeroed where uniform01(seed,
 // counter0 + r, j) < dropout: the draws of szh_net_accumulate_dev), live[i] = any element left.  One wave per row.
@@ -288,6 +341,15 @@ __global__ __launch_bounds__(64 * WAVES) void low_kernel(LowArgs a)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) part[wave][16 * t + 4 * q + i][16 * n + r16] = acc[t][n][i];
         __syncthreads();
+        // the output layer's second product: its 2 OT tiles of 16 x 16 are dealt to the waves, their factors asked for ahead
+        constexpr int TILES = (2 * OT + WAVES - 1) / WAVES;
+        float up[TILES ? TILES : 1][RT * 4];
+#pragma unroll
+        for (int y = 0; y < TILES; ++y) {
+            const float* B = a.up + (size_t)max(slot, 0) * a.up_slot + min(16 * ((wave + y * WAVES) >> 1) + r16, a.out - 1);
+#pragma unroll
+            for (int k = 0; k < RT * 4; ++k) up[y][k] = B[(size_t)min(4 * k + q, a.rank - 1) * a.out];
+        }
         for (int e = threadIdx.x; e < 32 * RT * 16; e += 64 * WAVES) {
             const int r = e / (RT * 16), j = e % (RT * 16);
             float s = 0.0f;
@@ -299,19 +361,190 @@ __global__ __launch_bounds__(64 * WAVES) void low_kernel(LowArgs a)
         }
         if (OT > 0) {
             __syncthreads();
-            const float* up = a.up + (size_t)max(slot, 0) * a.up_slot;
-            for (int e = threadIdx.x; e < 32 * OT * 16; e += 64 * WAVES) {
-                const int r = e / (OT * 16), c = e % (OT * 16);
-                if (c >= a.out || row0 + r >= a.rows || !((member >> r) & 1u)) continue;
-                float s = 0.0f, v = 0.0f;
 #pragma unroll
-                for (int w = 0; w < WAVES; ++w) s += part[w][r][c];
-                if (slot >= 0) {
-#pragma unroll 4
-                    for (int j = 0; j < a.rank; ++j) v = __builtin_fmaf(part[0][r][OT * 16 + j], up[(size_t)j * a.out + c], v);
+            for (int y = 0; y < TILES; ++y) {
+                const int tile = wave + y * WAVES, yt = tile & 1, c = 16 * (tile >> 1) + r16;
+                if (tile >= 2 * OT) break;
+                f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < RT * 4; ++k) {
+                    const float w = slot >= 0 && 4 * k + q < a.rank ? up[y][k] : 0.0f;
+                    v = __builtin_amdgcn_mfma_f32_16x16x4f32(part[0][16 * yt + r16][OT * 16 + 4 * k + q], w, v, 0, 0, 0);
                 }
-                a.y[(size_t)(row0 + r) * a.ldy + c] = s + v + a.bias[c];
+                const float bias = a.bias[min(c, a.out - 1)];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 16 * yt + 4 * q + i;
+                    float s = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < WAVES; ++w) s += part[w][r][c];
+                    if (c < a.out && row0 + r < a.rows && ((member >> r) & 1u)) a.y[(size_t)(row0 + r) * a.ldy + c] = s + v[i] + bias;
+                }
             }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- backward through the output layer ---------------------------------------------------------------
+// g3 = scale d3 B3^T, d2 = (d3 W3^T + g3 A3^T)(1 - h2^2), g2 = scale d2 B2^T for 32 rows per workgroup, d3 and h2 read
+// and d2, g2, g3 written once.  Everything is computed transposed (rows of the batch along the matrix instruction's
+// columns): a result's four registers then are four neighbouring units of one row, which is what the next product's
+// operand and 16-byte loads and stores want.  The waves deal the hidden units among themselves; g2, a sum over all
+// of them, is joined in LDS.  Bound by memory: at 66140 x 256 x 16 it moves 140 MB.
+struct BackArgs {
+    const float *d3, *h2, *w3;        // [rows][ld3], [rows][ld2], [n2][out]
+    const float *a3, *b3, *b2;        // slot 0's factors [n2][rank], [rank][out], [rank][n2]
+    uint64_t per_slot;
+    const int32_t* row_slot;
+    float *d2, *g2, *g3;              // [rows][ld2], [rows][ldu]
+    uint32_t rows;
+    int n2, out, rank, ld2, ld3, ldu;
+    float scale;
+};
+template <int RT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void back_kernel(BackArgs a)
+{
+    __shared__ float part[WAVES][2][RT * 16][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r16 = lane & 15, q = lane >> 4;
+    const uint32_t row0 = blockIdx.x * 32;
+    const uint32_t my_row = row0 + (lane & 31);
+    const int mine = my_row < a.rows ? a.row_slot[my_row] : -1;
+    uint32_t left = (uint32_t)__ballot(my_row < a.rows);
+    size_t row[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) row[t] = min(row0 + 16 * t + r16, a.rows - 1);
+    const int tiles = (a.n2 + 15) / 16;
+    const int out4 = (a.out + 3) & ~3;  // (ld3 is a multiple of 4: whole 16-byte pieces lie inside a row of d3)
+    while (left) {
+        const int slot = __builtin_amdgcn_readlane(mine, __builtin_ctz(left));
+        const uint32_t member = (uint32_t)__ballot(mine == slot) & left;
+        left &= ~member;
+        if (slot < 0) {  // rows without an adapter: d3 is zero there
+            for (int e = threadIdx.x; e < 32 * a.n2; e += 64 * WAVES)
+                if ((member >> (e / a.n2)) & 1u) a.d2[(size_t)(row0 + e / a.n2) * a.ld2 + e % a.n2] = 0.0f;
+            for (int e = threadIdx.x; e < 32 * a.ldu; e += 64 * WAVES)
+                if ((member >> (e / a.ldu)) & 1u) a.g2[(size_t)(row0 + e / a.ldu) * a.ldu + e % a.ldu] = a.g3[(size_t)(row0 + e / a.ldu) * a.ldu + e % a.ldu] = 0.0f;
+            continue;
+        }
+        const float* a3 = a.a3 + (size_t)slot * a.per_slot;
+        const float* b3 = a.b3 + (size_t)slot * a.per_slot;
+        const float* b2 = a.b2 + (size_t)slot * a.per_slot;
+        const bool mem[2] = {((member >> r16) & 1u) != 0, ((member >> (16 + r16)) & 1u) != 0};
+        // g3^T: registers j = 16 n + 4 q + i of row r16 (every wave has all of it)
+        f32x4 g3[2][RT], g2[2][RT];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < RT; ++n) g3[t][n] = g2[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c0 = 0; c0 < out4; c0 += 16) {
+            const int c = c0 + 4 * q;
+            f32x4 d[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) d[t] = *reinterpret_cast<const f32x4*>(a.d3 + row[t] * a.ld3 + min(c, a.ld3 - 4));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool in = c + e < a.out;
+#pragma unroll
+                for (int n = 0; n < RT; ++n) {
+                    float w = b3[(size_t)min(16 * n + r16, a.rank - 1) * a.out + min(c + e, a.out - 1)];
+                    w = in && 16 * n + r16 < a.rank ? w : 0.0f;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) g3[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, in ? d[t][e] : 0.0f, g3[t][n], 0, 0, 0);
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < RT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    g3[t][n][i] *= a.scale;
+                    const int j = 16 * n + 4 * q + i;
+                    if (wave == 0 && mem[t] && j < a.ldu) a.g3[row[t] * a.ldu + j] = g3[t][n][i];
+                }
+        for (int tile = wave; tile < tiles; tile += WAVES) {
+            const int n0 = 16 * tile, u = min(n0 + r16, a.n2 - 1);  // the unit whose weights this lane holds
+            f32x4 h[2], d2[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                h[t] = *reinterpret_cast<const f32x4*>(a.h2 + row[t] * a.ld2 + n0 + 4 * q);
+                d2[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            float wb[4][RT];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int n = 0; n < RT; ++n) {
+                    const int j = 16 * n + r16, k = n0 + 4 * q + e;
+                    wb[e][n] = b2[(size_t)min(j, a.rank - 1) * a.n2 + min(k, a.n2 - 1)];
+                    wb[e][n] = j < a.rank && k < a.n2 ? wb[e][n] : 0.0f;
+                }
+            for (int c0 = 0; c0 < out4; c0 += 16) {
+                const int c = c0 + 4 * q;
+                f32x4 d[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) d[t] = *reinterpret_cast<const f32x4*>(a.d3 + row[t] * a.ld3 + min(c, a.ld3 - 4));
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = a.w3[(size_t)u * a.out + min(c + e, a.out - 1)];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool in = c + e < a.out;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) d2[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? w[e] : 0.0f, in ? d[t][e] : 0.0f, d2[t], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < RT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int j = 16 * n + 4 * q + e;
+                    float w = a3[(size_t)u * a.rank + min(j, a.rank - 1)];
+                    w = j < a.rank ? w : 0.0f;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) d2[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, g3[t][n][e], d2[t], 0, 0, 0);
+                }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d2[t][i] *= 1.0f - h[t][i] * h[t][i];
+                // (columns between n2 and ld2 take products with zeros, or zeros: the padding of h2 and the clamped unit's
+                // weights are finite or theirs alone; only whole pieces inside ld2 are stored)
+                if (mem[t]) {
+                    float* dst = a.d2 + row[t] * a.ld2 + n0 + 4 * q;
+                    if (n0 + 4 * q + 3 < a.n2) *reinterpret_cast<f32x4*>(dst) = d2[t];
+                    else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (n0 + 4 * q + i < a.n2) dst[i] = d2[t][i];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d2[t][i] = n0 + 4 * q + i < a.n2 ? d2[t][i] : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int n = 0; n < RT; ++n)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) g2[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(wb[e][n], d2[t][e], g2[t][n], 0, 0, 0);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < RT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[wave][t][16 * n + 4 * q + i][r16] = g2[t][n][i];
+        __syncthreads();
+        for (int e = threadIdx.x; e < 32 * a.ldu; e += 64 * WAVES) {
+            const int r = e / a.ldu, j = e % a.ldu;
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) s += part[w][r >> 4][j][r & 15];
+            if ((member >> r) & 1u) a.g2[(size_t)(row0 + r) * a.ldu + j] = j < a.rank ? a.scale * s : 0.0f;
         }
         __syncthreads();
     }
@@ -322,7 +555,6 @@ __global__ __launch_bounds__(64 * WAVES) void low_kernel(LowArgs a)
 // p[i][m] w[i][j], m up to a layer's width and j the rank columns; one launch does all four.
 // slab[chunk + slot][m][j] takes the part of a chunk of rows: rows are sorted by slot, so (chunk, slot) pairs that
 // hold rows lie on a staircase and chunk + slot numbers them without a table; factor_reduce_kernel adds a slot's chunks.
-constexpr int kFactorRows = 512;
 struct FactorJob {
     const float* p;        // [rows][ldp], 16-byte aligned rows
     const float* w;        // [rows][ldw], the rank columns
@@ -337,6 +569,7 @@ struct FactorArgs {
     const uint32_t* begin; // [slots + 2]
     const int32_t* row_slot;
     int ldw, rank, slots;
+    uint32_t chunk;        // rows per chunk
 };
 
 // 64 columns of p per workgroup; its four waves take rows in turn and are joined in LDS.  A lane reads 16
@@ -350,8 +583,8 @@ __global__ __launch_bounds__(256) void factor_grad_kernel(FactorArgs a)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int c16 = lane & 15, q = lane >> 4;
     const int m0 = ((int)blockIdx.x - g.first) * 64;
-    const uint32_t end = min(a.begin[a.slots], (blockIdx.y + 1) * (uint32_t)kFactorRows);
-    uint32_t r = blockIdx.y * (uint32_t)kFactorRows;
+    const uint32_t end = min(a.begin[a.slots], (blockIdx.y + 1) * a.chunk);
+    uint32_t r = blockIdx.y * a.chunk;
     while (r < end) {
         const int slot = a.row_slot[r];
         const uint32_t stop = min(end, a.begin[slot + 1]);
@@ -360,20 +593,29 @@ __global__ __launch_bounds__(256) void factor_grad_kernel(FactorArgs a)
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t i = r + 4 * wave; i < stop; i += 16) {
-            const bool in = i + q < stop;
-            const size_t row = in ? i + q : stop - 1;
+        // (two groups of four rows at a time: the loads of both are in flight)
+        for (uint32_t i = r + 4 * wave; i < stop; i += 32) {
+            f32x4 pv[2];
+            float wv[2][NT];
             const int col = m0 + 4 * c16;
-            f32x4 pv = *reinterpret_cast<const f32x4*>(g.p + row * g.ldp + min(col, g.ldp - 4));
 #pragma unroll
-            for (int t = 0; t < 4; ++t) pv[t] = in && col + t < g.M ? pv[t] : 0.0f;
+            for (int g2 = 0; g2 < 2; ++g2) {
+                const size_t row = min(i + 16 * g2 + q, stop - 1);
+                pv[g2] = *reinterpret_cast<const f32x4*>(g.p + row * g.ldp + min(col, g.ldp - 4));
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int j = 16 * n + c16;
-                float v = g.w[row * a.ldw + min(j, a.rank - 1)];
-                v = in && j < a.rank ? v : 0.0f;
+                for (int n = 0; n < NT; ++n) wv[g2][n] = g.w[row * a.ldw + min(16 * n + c16, a.rank - 1)];
+            }
 #pragma unroll
-                for (int t = 0; t < 4; ++t) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[t], v, acc[t][n], 0, 0, 0);
+            for (int g2 = 0; g2 < 2; ++g2) {
+                const bool in = i + 16 * g2 + q < stop;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) pv[g2][t] = in && col + t < g.M ? pv[g2][t] : 0.0f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float v = in && 16 * n + c16 < a.rank ? wv[g2][n] : 0.0f;
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[g2][t], v, acc[t][n], 0, 0, 0);
+                }
             }
         }
 #pragma unroll
@@ -404,7 +646,7 @@ __global__ __launch_bounds__(256) void factor_reduce_kernel(FactorArgs a, float*
     const FactorJob g = a.job[which];
     const int i = ((int)blockIdx.x - g.first_out) * 256 + threadIdx.x;
     if (i >= g.M * a.rank) return;
-    const uint32_t c0 = b / kFactorRows, c1 = (e - 1) / kFactorRows;
+    const uint32_t c0 = b / a.chunk, c1 = (e - 1) / a.chunk;
     double t = 0.0;
     for (uint32_t c = c0; c <= c1; ++c) t += (double)g.slab[(size_t)(c + slot) * g.M * a.rank + i];
     grad[(size_t)slot * grad_slot + g.off + (size_t)(i / a.rank) * g.g_m + (size_t)(i % a.rank) * g.g_j] += (float)t;

@@ -49,11 +49,22 @@ __device__ __forceinline__ void row_product(const float* x, int K, const float* 
                         a2 = __builtin_fmaf(xv, w[i].z, a2); a3 = __builtin_fmaf(xv, w[i].w, a3);
                     }
                 }
-                for (; k < n_k; k += slices) {
-                    const float4 w = *reinterpret_cast<const float4*>(M + (size_t)k * N + c);
-                    const float xv = v[k];
-                    a0 = __builtin_fmaf(xv, w.x, a0); a1 = __builtin_fmaf(xv, w.y, a1);
-                    a2 = __builtin_fmaf(xv, w.z, a2); a3 = __builtin_fmaf(xv, w.w, a3);
+                // what is left of k, four pieces in flight, those behind it as zeros
+                for (; k < n_k; k += 4 * slices) {
+                    float4 w[4];
+                    float xv[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int kk = min(k + i * slices, n_k - 1);
+                        w[i] = *reinterpret_cast<const float4*>(M + (size_t)kk * N + c);
+                        xv[i] = v[kk];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool on = k + i * slices < n_k;
+                        a0 = __builtin_fmaf(xv[i], on ? w[i].x : 0.0f, a0); a1 = __builtin_fmaf(xv[i], on ? w[i].y : 0.0f, a1);
+                        a2 = __builtin_fmaf(xv[i], on ? w[i].z : 0.0f, a2); a3 = __builtin_fmaf(xv[i], on ? w[i].w : 0.0f, a3);
+                    }
                 }
             } else {
                 const int c1 = min(c + 1, N - 1), c2 = min(c + 2, N - 1), c3 = min(c + 3, N - 1);

