@@ -169,11 +169,35 @@ int low_product(const Adapters* a, const float* x, int ldx, int K, const float* 
     g.rank = (int)a->rank; g.row_slot = a->ws.row_slot; g.rows = rows; g.u = u; g.ldu = a->ws.ldu; g.scale = a->scale;
     ProfScope prof("adapt_low", s);
     switch ((a->rank + 15) / 16) {
-    case 1: return launch_low<1, 0, 8, 4>(g, s);
-    case 2: return launch_low<2, 0, 8, 2>(g, s);
+    case 1: return launch_low<1, 0, 4, 4>(g, s);
+    case 2: return launch_low<2, 0, 4, 2>(g, s);
     case 3: return launch_low<3, 0, 8, 2>(g, s);
     default: return launch_low<4, 0, 4, 2>(g, s);
     }
+}
+
+// whether rows of `width` values, `apart` values from one to the next, can be read in aligned pieces of 16 bytes
+bool in_fours(const float* p, uint64_t width, uint64_t apart) { return width % 4 == 0 && apart % 4 == 0 && ((uintptr_t)p & 15) == 0; }
+
+// h1 and u2 in one pass over x, straight from the caller's rows where `order` is given.  At rank 32 a wave's W1 and A2 leave
+// no registers for the rows to come, and the pass takes as long as the gather and the two products it replaces.
+bool front_applies(const Net* n, const Adapters* a) { return n->in <= kFrontIn && n->h1 <= 64 * kFrontWaves && a->rank <= 16; }
+int front_rows(const Net* n, const Adapters* a, const float* x, int ldx, const uint32_t* order, uint8_t* live, uint32_t rows, hipStream_t s)
+{
+    const AdaptWorkspace& w = a->ws;
+    FrontArgs g{};
+    g.x = x; g.order = order; g.w1 = n->d_params + n->off_w1(); g.b1 = n->d_params + n->off_b1(); g.a2 = a->d_params + a->off_a2();
+    g.per_slot = a->per_slot(); g.row_slot = w.row_slot; g.h1 = w.h1; g.u2 = w.u2; g.live = live; g.rows = rows;
+    g.in = (int)n->in; g.ldx = ldx; g.n1 = (int)n->h1; g.ld1 = w.ld1; g.rank = (int)a->rank; g.ldu = w.ldu; g.scale = a->scale;
+    const bool fours = in_fours(x, n->in, ldx) && in_fours(g.w1, n->h1, n->h1) && in_fours(g.b1, n->h1, 0);
+    const int waves = (g.n1 + 63) / 64;
+    const size_t lds = (size_t)2 * waves * 16 * 17 * sizeof(float);
+    const dim3 grid(std::min<unsigned>((rows + 15) / 16, (unsigned)compute_units() * (kFrontWaves / waves))), block(64 * waves);
+    ProfScope prof("adapt_h1", s);
+    if (fours) hipLaunchKernelGGL((front_kernel<true>), grid, block, lds, s, g);
+    else hipLaunchKernelGGL((front_kernel<false>), grid, block, lds, s, g);
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
 }
 
 // Output layers of up to 64 classes: u3 and the logits in one pass over h2
@@ -190,7 +214,7 @@ int low_out(const Net* n, const Adapters* a, uint32_t rows, hipStream_t s)
     const int rt = (int)(a->rank + 15) / 16, ot = (int)(n->out + 15) / 16;
     // (three tiles are taken as four: a column tile without columns repeats the last one's)
     switch ((ot > 2 ? 4 : ot) * 8 + (rt > 2 ? 4 : rt)) {
-    case 1 * 8 + 1: return launch_low<2, 1, 8, 2>(g, s);
+    case 1 * 8 + 1: return launch_low<2, 1, 4, 2>(g, s);
     case 1 * 8 + 2: return launch_low<3, 1, 8, 2>(g, s);
     case 1 * 8 + 4: return launch_low<5, 1, 4, 1>(g, s);
     case 2 * 8 + 1: return launch_low<3, 2, 8, 2>(g, s);
@@ -247,13 +271,18 @@ int back_rows(const Net* n, const Adapters* a, uint32_t rows, hipStream_t s)
     g.d3 = w.lg; g.h2 = w.h2; g.w3 = n->d_params + n->off_w3(); g.a3 = F + a->off_a3(); g.b3 = F + a->off_b3(); g.b2 = F + a->off_b2();
     g.per_slot = a->per_slot(); g.row_slot = w.row_slot; g.d2 = w.d2; g.g2 = w.g2; g.g3 = w.g3; g.rows = rows;
     g.n2 = (int)n->h2; g.out = (int)n->out; g.rank = (int)a->rank; g.ld2 = w.ld2; g.ld3 = w.ld3; g.ldu = w.ldu; g.scale = a->scale;
+    const bool fours = in_fours(g.w3, n->out, n->out) && in_fours(g.a3, a->rank, g.per_slot) && in_fours(g.b2, n->h2, g.per_slot);
     const dim3 grid((rows + 31) / 32);
     ProfScope prof("adapt_back", s);
-    switch ((a->rank + 15) / 16) {
-    case 1: hipLaunchKernelGGL((back_kernel<1, 8>), grid, dim3(512), 0, s, g); break;
-    case 2: hipLaunchKernelGGL((back_kernel<2, 8>), grid, dim3(512), 0, s, g); break;
-    case 3: hipLaunchKernelGGL((back_kernel<3, 4>), grid, dim3(256), 0, s, g); break;
-    default: hipLaunchKernelGGL((back_kernel<4, 4>), grid, dim3(256), 0, s, g); break;
+    switch ((a->rank + 15) / 16 * 2 + fours) {
+    case 2: hipLaunchKernelGGL((back_kernel<1, 4, 2, false>), grid, dim3(256), 0, s, g); break;
+    case 3: hipLaunchKernelGGL((back_kernel<1, 4, 2, true>), grid, dim3(256), 0, s, g); break;
+    case 4: hipLaunchKernelGGL((back_kernel<2, 8, 2, false>), grid, dim3(512), 0, s, g); break;
+    case 5: hipLaunchKernelGGL((back_kernel<2, 8, 2, true>), grid, dim3(512), 0, s, g); break;
+    case 6: hipLaunchKernelGGL((back_kernel<3, 4, 2, false>), grid, dim3(256), 0, s, g); break;
+    case 7: hipLaunchKernelGGL((back_kernel<3, 4, 2, true>), grid, dim3(256), 0, s, g); break;
+    case 8: hipLaunchKernelGGL((back_kernel<4, 4, 2, false>), grid, dim3(256), 0, s, g); break;
+    default: hipLaunchKernelGGL((back_kernel<4, 4, 2, true>), grid, dim3(256), 0, s, g); break;
     }
     SZ_HIP(hipGetLastError());
     return SZH_OK;
@@ -347,8 +376,9 @@ int shared_product(const GemmArgs& g, int Kp, float* wt, hipStream_t s)
     return SZH_OK;
 }
 
-// logits of `rows` grouped rows in the workspace's lg, activations in h1, h2, rank columns in u2, u3
-int forward_rows(Net* n, Adapters* a, uint32_t rows, hipStream_t s)
+// logits of `rows` grouped rows in the workspace's lg, activations in h1, h2, rank columns in u2, u3; x, in the caller's
+// order, unless gather_rows has put its rows into xs already (null)
+int forward_rows(Net* n, Adapters* a, const float* x, uint8_t* live, uint32_t rows, hipStream_t s)
 {
     AdaptWorkspace& w = a->ws;
     const float* P = n->d_params;
@@ -356,11 +386,15 @@ int forward_rows(Net* n, Adapters* a, uint32_t rows, hipStream_t s)
     const int r = (int)a->rank;
     int rc;
     GemmArgs g{};
-    g.A = w.xs; g.lda = w.ldx; g.C = w.h1; g.ldc = w.ld1; g.M = (int)rows; g.N = (int)n->h1; g.bias = P + n->off_b1();
-    g.B = P + n->off_w1(); g.ldb = (int)n->h1; g.K = g.k_chunk = (int)n->in;
-    // (a short k: 64-row tiles are never behind, 57 us against 61 on 128 and 70 on 256 rows at 66140 x 60 x 512)
-    rc = launch_gemm_rows<A_ROWS, B_KROWS, EPI_BIAS_RELU, T_ADAPT1, 64>(g, s);
-    if (!rc) rc = low_product(a, w.h1, w.ld1, (int)n->h1, F + a->off_a2(), r, 1, rows, w.u2, s);
+    if (front_applies(n, a)) {
+        rc = x ? front_rows(n, a, x, (int)n->in, w.order, live, rows, s) : front_rows(n, a, w.xs, w.ldx, nullptr, nullptr, rows, s);
+    } else {
+        g.A = w.xs; g.lda = w.ldx; g.C = w.h1; g.ldc = w.ld1; g.M = (int)rows; g.N = (int)n->h1; g.bias = P + n->off_b1();
+        g.B = P + n->off_w1(); g.ldb = (int)n->h1; g.K = g.k_chunk = (int)n->in;
+        // (a short k: 64-row tiles are never behind, 57 us against 61 on 128 and 70 on 256 rows at 66140 x 60 x 512)
+        rc = launch_gemm_rows<A_ROWS, B_KROWS, EPI_BIAS_RELU, T_ADAPT1, 64>(g, s);
+        if (!rc) rc = low_product(a, w.h1, w.ld1, (int)n->h1, F + a->off_a2(), r, 1, rows, w.u2, s);
+    }
     if (rc) return rc;
     g = GemmArgs{};
     g.A = w.h1; g.lda = w.ld1; g.C = w.h2; g.ldc = w.ld2; g.M = (int)rows; g.N = (int)n->h2; g.K = g.k_chunk = (int)n->h1;
@@ -476,8 +510,9 @@ int infer_rows(Net* n, Adapters* a, const float* x, const int32_t* slots_dev, ui
 {
     if (few_rows(n, rows, false)) return forward_few(n, a, x, n->in, slots_dev, rows, ctl, c, nullptr, nullptr, s);
     int rc = group_rows(a, slots_dev, rows, s);
-    if (!rc) rc = gather_rows(a, x, rows, 0.0f, 0, 0, nullptr, s);
-    if (!rc) rc = forward_rows(n, a, rows, s);
+    const bool front = front_applies(n, a);
+    if (!rc && !front) rc = gather_rows(a, x, rows, 0.0f, 0, 0, nullptr, s);
+    if (!rc) rc = forward_rows(n, a, front ? x : nullptr, nullptr, rows, s);
     c.order = a->ws.order;
     return rc ? rc : control_run(ctl, c, s);
 }
@@ -596,14 +631,14 @@ int adapters_accumulate(Net* n, Adapters* a, const float* x, const int32_t* labe
     for (uint64_t r0 = 0; r0 < rows; r0 += kAdaptRows) {
         const uint32_t R = (uint32_t)std::min<uint64_t>(kAdaptRows, rows - r0);
         int rc = group_rows(a, slots_dev + r0, R, s);
-        if (!rc) rc = gather_rows(a, x + r0 * n->in, R, dropout, seed, r0, w.live0, s);
+        const bool few = few_rows(n, R, true), front = !few && front_applies(n, a) && dropout <= 0.0f;
+        if (!rc && !front) rc = gather_rows(a, x + r0 * n->in, R, dropout, seed, r0, w.live0, s);
         ControlRun c{};
         c.in = w.lg; c.ld_in = w.ld3; c.rows = R; c.classes = n->out; c.order = w.order;
         c.out = w.lg; c.ld_out = w.ld3; c.labels = labels + r0; c.row_live = w.live0; c.row_slot = w.row_slot; c.loss = w.loss; c.live = w.live;
         const Controls ctl_r = from_row(ctl, r0);
-        const bool few = few_rows(n, R, true);
         if (!rc && few) rc = forward_few(n, a, w.xs, w.ldx, w.row_slot, R, ctl_r, c, w.u2, w.u3, s);
-        if (!rc && !few) rc = forward_rows(n, a, R, s);
+        if (!rc && !few) rc = forward_rows(n, a, front ? x + r0 * n->in : nullptr, w.live0, R, s);
         if (!rc && !few) rc = control_run(ctl_r, c, s);   // lg now holds d3
         if (rc) return rc;
         const bool back_done = few && (uint64_t)n->h2 * n->out <= kRowOutFloats;  // (by the row kernel)

@@ -25,19 +25,6 @@ __device__ __forceinline__ int group_key(const int32_t* slot, uint64_t r, int sl
     return s >= 0 && s < slots ? s : slots;
 }
 
-// Visits the distinct keys of the wave's active lanes: f(key, mask of the lanes that hold it).
-template <class F>
-__device__ __forceinline__ void each_key(int key, bool active, F f)
-{
-    unsigned long long left = __ballot(active);
-    while (left) {
-        const int k = __builtin_amdgcn_readlane(key, __ffsll(left) - 1);
-        const unsigned long long member = __ballot(active && key == k);
-        left &= ~member;
-        f(k, member);
-    }
-}
-
 // count[key][block] of a block of rows
 __global__ __launch_bounds__(64) void group_count_kernel(const int32_t* __restrict__ slot, uint32_t rows, int slots, int blocks,
                                                          uint32_t* __restrict__ count)
@@ -91,23 +78,32 @@ __global__ __launch_bounds__(64) void group_begin_kernel(const uint32_t* __restr
     if (threadIdx.x == 0) begin[slots + 1] = rows;
 }
 
-// order[place] = row, row_slot[place] = its slot or -1, for rows r0 .. r1 - 1; next[key]: where the key's next row goes
+// order[place] = row, row_slot[place] = its slot or -1, for rows r0 .. r1 - 1, by one wave; next[key]: where the key's next
+// row goes.  The lanes of a lane's key are found bit by bit of the key, whatever keys there are (a turn for each key
+// took 50 us more at 8000 rows of 200 slots).
 __device__ __forceinline__ void place_rows(const int32_t* __restrict__ slot, uint32_t r0, uint32_t r1, int slots, uint32_t* next,
                                            uint32_t* __restrict__ order, int32_t* __restrict__ row_slot)
 {
+    const int lane = threadIdx.x & 63, bits = 32 - __clz(slots);
     for (uint32_t r = r0; r < r1; r += 64) {
-        const bool in = r + threadIdx.x < r1;
-        const int key = in ? group_key(slot, r + threadIdx.x, slots) : 0;
-        uint32_t place = 0;
-        each_key(key, in, [&](int k, unsigned long long member) {
-            const uint32_t base = next[k];
-            if (in && key == k) place = base + (uint32_t)__popcll(member & ((1ull << threadIdx.x) - 1));
-            __syncthreads();  // (one wave: every lane has read next[k])
-            if (threadIdx.x == 0) next[k] = base + (uint32_t)__popcll(member);
-            __syncthreads();
-        });
+        const bool in = r + lane < r1;
+        const int key = in ? group_key(slot, r + lane, slots) : 0;
+        unsigned long long same = __ballot(in);
+        for (int b = 0; b < bits; ++b) {
+            const bool one = (key >> b) & 1;
+            const unsigned long long ones = __ballot(one);
+            same &= one ? ones : ~ones;
+        }
+        const unsigned long long before = same & ((1ull << lane) - 1);
+        const uint32_t base = next[key];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();  // (every lane has read next[key])
+        if (in && before == 0) next[key] = base + (uint32_t)__popcll(same);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
         if (in) {
-            order[place] = r + threadIdx.x;
+            const uint32_t place = base + (uint32_t)__popcll(before);
+            order[place] = r + lane;
             row_slot[place] = key < slots ? key : -1;
         }
     }
@@ -178,25 +174,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void group_mid_kernel(const int32
     }
     if (threadIdx.x == 0) begin[slots + 1] = rows;
     __syncthreads();
-    // as place_rows, the wave's lanes in step by themselves: their LDS accesses are in program order
-    for (uint32_t r = r0; r < r1; r += 64) {
-        const bool in = r + lane < r1;
-        const int key = in ? group_key(slot, r + lane, slots) : 0;
-        uint32_t place = 0;
-        each_key(key, in, [&](int kk, unsigned long long member) {
-            const uint32_t at = mine[kk];
-            __builtin_amdgcn_wave_barrier();
-            if (in && key == kk) place = at + (uint32_t)__popcll(member & ((1ull << lane) - 1));
-            if (lane == 0) mine[kk] = at + (uint32_t)__popcll(member);
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-        });
-        if (in) {
-            order[place] = r + lane;
-            row_slot[place] = key < slots ? key : -1;
-        }
-    }
+    place_rows(slot, r0, r1, slots, mine, order, row_slot);
 }
 
 // ---- rows in that order -------------------------------------------------------------------------
@@ -224,6 +202,187 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const float* __restric
         const bool some = __any(any);
         if (lane == 0) live[i] = some ? 1 : 0;
     }
+}
+
+// ---- the first layer and its rank columns ------------------------------------------------------------
+// use ? v : 0 for a loaded v.  Of a plain select the compiler may make a branch with the load in it, where it is waited for
+// before the next is asked for (sixteen such loads in a row took 16 us).
+__device__ __forceinline__ float keep_if(bool use, float v)
+{
+    asm("" : "+v"(v));
+    return use ? v : 0.0f;
+}
+// Four neighbouring values p[at .. at + 3], those from `end` on as zeros, in two steps: what is asked for first and what is
+// waited for later.  FOURS: p is 16-byte aligned, at and end in fours (a template's choice for the same reason).
+template <bool FOURS>
+__device__ __forceinline__ f32x4 ask_four(const float* __restrict__ p, int at, int end)
+{
+    if (FOURS) return *reinterpret_cast<const f32x4*>(p + min(at, end - 4));
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = p[min(at + e, end - 1)];
+    return v;
+}
+__device__ __forceinline__ f32x4 cut_four(f32x4 v, int at, int end)
+{
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = keep_if(at + e < end, v[e]);
+    return v;
+}
+
+// h1 = relu(x W1 + b1) and u2 = scale h1 A2[slot] of up to 64 inputs, 512 units and rank 16 in one pass: x is read where the
+// caller has it (row i is x[order[i]]), h1 is written once and not read again.  Workgroups walk along the rows, 16 at a time,
+// and keep W1 in registers: a wave has 64 units, and the A2 of those for the slot it saw last (rows come sorted by
+// slot).  The next rows' x is asked for while this one's is computed.  All is transposed (rows of the batch along the
+// matrix instruction's columns), with unit n0 + 4 (4 (m % 4) + m / 4) + c in row m of the instruction's tile c: a result's
+// register i of the four tiles is units n0 + 16 i + 4 q + 0 .. 3 of one row, a 16-byte store and the next product's operand
+// as it is.  u2, a sum over all units, is joined in LDS, in the order of the waves.  Rows of another slot than the one at
+// hand keep their sums: what a row gets does not depend on its neighbours.  Bound by matrix instructions.
+constexpr int kFrontWaves = 8, kFrontIn = 64;
+struct FrontArgs {
+    const float* x;
+    const uint32_t* order;   // null: x's rows are in order
+    const float *w1, *b1, *a2;  // [in][n1], [n1], slot 0's [n1][rank]
+    uint64_t per_slot;
+    const int32_t* row_slot;
+    float *h1, *u2;
+    uint8_t* live;           // null, or any element of x but 0
+    uint32_t rows;
+    int in, ldx, n1, ld1, rank, ldu;
+    float scale;
+};
+// FOURS: the rows of x, W1 and b1 are 16-byte aligned and in fours
+template <bool FOURS>
+__global__ __launch_bounds__(64 * kFrontWaves) void front_kernel(FrontArgs a)
+{
+    extern __shared__ __attribute__((aligned(16))) float front_lds[];  // [2][waves][16][17]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int r16 = lane & 15, q = lane >> 4;
+    const uint32_t tiles = (a.rows + 15) / 16;
+    const uint32_t first = (uint32_t)((uint64_t)tiles * blockIdx.x / gridDim.x), last = (uint32_t)((uint64_t)tiles * (blockIdx.x + 1) / gridDim.x);
+    if (first >= last) return;
+    const int n0 = 64 * wave, unit4 = n0 + 4 * (4 * (r16 & 3) + (r16 >> 2));
+    f32x4 w[4][4], bias[4];  // (zeros beyond the inputs and units: relu makes 0 of those units whatever x holds)
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int k = 16 * b + 4 * q + e;
+            w[b][e] = ask_four<FOURS>(a.w1 + (uint32_t)min(k, a.in - 1) * (uint32_t)a.n1, unit4, a.n1);
+        }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bias[i] = ask_four<FOURS>(a.b1, n0 + 16 * i + 4 * q, a.n1);
+    // rows of a tile, x's row for each, its slot; tiles behind the last one are the last one
+    auto at = [&](uint32_t tile) { return min(16 * min(tile, last - 1) + r16, a.rows - 1); };
+    auto source = [&](uint32_t tile) { return a.order ? a.order[at(tile)] : at(tile); };
+    f32x4 x[4], next[4];
+    uint32_t ahead = source(first + 1);
+    int slot_of = a.row_slot[at(first)];
+    {
+        const float* p = a.x + (size_t)source(first) * a.ldx;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) x[b] = ask_four<FOURS>(p, 16 * b + 4 * q, a.in);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[b][e] = cut_four(w[b][e], unit4, 16 * b + 4 * q + e < a.in ? a.n1 : 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bias[i] = cut_four(bias[i], n0 + 16 * i + 4 * q, a.n1);
+#pragma unroll
+    for (int b = 0; b < 4; ++b) x[b] = cut_four(x[b], 16 * b + 4 * q, a.in);
+    // Every lane stores at every tile, those without a row into the rows behind the last one, those without a unit into
+    // one of those: behind a store that may not have happened the wait for the next x would be for the store as well.
+    float* spare = a.h1 + (size_t)(a.rows + 31) * a.ld1 + 4 * (lane & 7);
+    int r_out = threadIdx.x / a.ldu, j_out = threadIdx.x % a.ldu;
+    auto part_of = [&](uint32_t tile) { return reinterpret_cast<float (*)[16][17]>(front_lds) + ((tile - first) & 1) * waves; };
+    auto join = [&](uint32_t tile) {
+        const float (*part)[16][17] = part_of(tile);
+        for (int e = threadIdx.x, r = r_out, j = j_out; e < 16 * a.ldu; e += blockDim.x, r = e / a.ldu, j = e % a.ldu) {
+            float s = 0.0f;
+#pragma unroll
+            for (int v = 0; v < kFrontWaves; ++v) s += keep_if(v < waves, part[min(v, waves - 1)][j][r]);
+            if (16 * tile + r < a.rows) a.u2[(size_t)(16 * tile + r) * a.ldu + j] = j < a.rank ? a.scale * s : 0.0f;
+        }
+    };
+    int have = -1;      // the slot that f belongs to
+    float f[4][4];      // A2 of unit n0 + 16 i + 4 q + c, rank column r16
+    for (uint32_t tile = first; tile < last; ++tile) {
+        const float* p = a.x + (size_t)ahead * a.ldx;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) next[b] = ask_four<FOURS>(p, 16 * b + 4 * q, a.in);
+        ahead = source(tile + 2);
+        const int slot_next = a.row_slot[at(tile + 1)];
+        const uint32_t row = 16 * tile + r16;
+        const bool in = row < a.rows;
+        if (a.live && wave == 0) {
+            bool any = false;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) any = any || x[b][e] != 0.0f;
+            const unsigned long long some = __ballot(any);
+            if (q == 0 && in) a.live[row] = ((some >> r16) & 0x0001000100010001ull) != 0;
+        }
+        f32x4 h[4];  // [tile of the instruction]
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[c][i] = bias[i][c];
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) h[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[b][e][c], x[b][e], h[c], 0, 0, 0);
+        if (tile > first) join(tile - 1);  // (beside the matrix instructions)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = n0 + 16 * i + 4 * q;
+            f32x4 v;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) h[c][i] = v[c] = h[c][i] > 0.0f ? h[c][i] : 0.0f;
+            *reinterpret_cast<f32x4*>(n < a.ld1 ? a.h1 + (size_t)row * a.ld1 + n : spare) = v;
+        }
+        f32x4 u = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t left = (uint32_t)__ballot(in && slot_of >= 0) & 0xffffu;
+        while (left) {
+            const int slot = __builtin_amdgcn_readlane(slot_of, __builtin_ctz(left));
+            const bool mem = slot_of == slot;
+            left &= ~(uint32_t)__ballot(mem);
+            if (slot != have) {
+                have = slot;
+                const float* a2 = a.a2 + (size_t)slot * a.per_slot;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) f[i][c] = a2[(uint32_t)min(n0 + 16 * i + 4 * q + c, a.n1 - 1) * (uint32_t)a.rank + min(r16, a.rank - 1)];
+                __builtin_amdgcn_sched_barrier(0);
+                int unit = n0 + 4 * q, col = r16;
+                asm("" : "+v"(unit), "+v"(col));  // (or thirty-two masks are kept in scalar registers all along)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) f[i][c] = keep_if(unit + 16 * i + c < a.n1 && col < a.rank, f[i][c]);
+            }
+            f32x4 v[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) v[c & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(f[i][c], h[c][i], v[c & 1], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = mem ? v[0][i] + v[1][i] : u[i];
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) x[b] = cut_four(next[b], 16 * b + 4 * q, a.in);
+        slot_of = slot_next;
+        // (two buffers: who writes the next but one has passed the next barrier, and with it everyone's reads of this one)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part_of(tile)[wave][4 * q + i][r16] = u[i];
+        __syncthreads();
+    }
+    join(last - 1);
 }
 
 // ---- products with the rank columns ----------------------------------------------------------------
@@ -307,6 +466,7 @@ __global__ __launch_bounds__(64 * WAVES) void low_kernel(LowArgs a)
 #pragma unroll
                     for (int n = 0; n < NT; ++n) w[i][e][n] = col[n][(uint32_t)(16 * (b + i) + 4 * q + e) * step[n]];
             }
+            __builtin_amdgcn_sched_barrier(0);  // every load is asked for before the first is waited for
 #pragma unroll
             for (int i = 0; i < UNR; ++i)
 #pragma unroll
@@ -320,14 +480,18 @@ __global__ __launch_bounds__(64 * WAVES) void low_kernel(LowArgs a)
             f32x4 xv[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) xv[t] = *reinterpret_cast<const f32x4*>(x[t] + min(16 * b, a.ldx - 4 - 4 * q));
+            float w[4][NT];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) w[e][n] = col[n][(uint32_t)min(16 * b + 4 * q + e, a.K - 1) * step[n]];
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int k = 16 * b + 4 * q + e;
-                const bool in_k = k < a.K;
+                const bool in_k = 16 * b + 4 * q + e < a.K;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    float v = col[n][(uint32_t)min(k, a.K - 1) * step[n]];
-                    v = in_k ? v : 0.0f;
+                    const float v = keep_if(in_k, w[e][n]);
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
                         acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(in_k ? xv[t][e] : 0.0f, v, acc[t][n], 0, 0, 0);
@@ -350,6 +514,7 @@ __global__ __launch_bounds__(64 * WAVES) void low_kernel(LowArgs a)
 #pragma unroll
             for (int k = 0; k < RT * 4; ++k) up[y][k] = B[(size_t)min(4 * k + q, a.rank - 1) * a.out];
         }
+        __builtin_amdgcn_sched_barrier(0);
         for (int e = threadIdx.x; e < 32 * RT * 16; e += 64 * WAVES) {
             const int r = e / (RT * 16), j = e % (RT * 16);
             float s = 0.0f;
@@ -368,7 +533,7 @@ __global__ __launch_bounds__(64 * WAVES) void low_kernel(LowArgs a)
                 f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < RT * 4; ++k) {
-                    const float w = slot >= 0 && 4 * k + q < a.rank ? up[y][k] : 0.0f;
+                    const float w = keep_if(slot >= 0 && 4 * k + q < a.rank, up[y][k]);
                     v = __builtin_amdgcn_mfma_f32_16x16x4f32(part[0][16 * yt + r16][OT * 16 + 4 * k + q], w, v, 0, 0, 0);
                 }
                 const float bias = a.bias[min(c, a.out - 1)];
@@ -387,7 +552,7 @@ __global__ __launch_bounds__(64 * WAVES) void low_kernel(LowArgs a)
 }
 
 // ---- backward through the output layer ---------------------------------------------------------------
-// g3 = scale d3 B3^T, d2 = (d3 W3^T + g3 A3^T)(1 - h2^2), g2 = scale d2 B2^T for 32 rows per workgroup, d3 and h2 read
+// g3 = scale d3 B3^T, d2 = (d3 W3^T + g3 A3^T)(1 - h2^2), g2 = scale d2 B2^T for 16 T rows per workgroup, d3 and h2 read
 // and d2, g2, g3 written once.  Everything is computed transposed (rows of the batch along the matrix instruction's
 // columns): a result's four registers then are four neighbouring units of one row, which is what the next product's
 // operand and 16-byte loads and stores want.  The waves deal the hidden units among themselves; g2, a sum over all
@@ -402,19 +567,21 @@ struct BackArgs {
     int n2, out, rank, ld2, ld3, ldu;
     float scale;
 };
-template <int RT, int WAVES>
+// FOURS: the rows of W3, A3 and B2 are 16-byte aligned and in fours
+template <int RT, int WAVES, int T, bool FOURS>
 __global__ __launch_bounds__(64 * WAVES) void back_kernel(BackArgs a)
 {
-    __shared__ float part[WAVES][2][RT * 16][17];
+    __shared__ float part[WAVES][T][RT * 16][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r16 = lane & 15, q = lane >> 4;
-    const uint32_t row0 = blockIdx.x * 32;
-    const uint32_t my_row = row0 + (lane & 31);
+    const uint32_t row0 = blockIdx.x * (16 * T);
+    const uint32_t my_row = row0 + (lane & (16 * T - 1));
     const int mine = my_row < a.rows ? a.row_slot[my_row] : -1;
-    uint32_t left = (uint32_t)__ballot(my_row < a.rows);
-    size_t row[2];
+    constexpr uint32_t MASK = T == 2 ? 0xffffffffu : 0xffffu;
+    uint32_t left = (uint32_t)__ballot(my_row < a.rows) & MASK;
+    size_t row[T];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) row[t] = min(row0 + 16 * t + r16, a.rows - 1);
+    for (int t = 0; t < T; ++t) row[t] = min(row0 + 16 * t + r16, a.rows - 1);
     const int tiles = (a.n2 + 15) / 16;
     const int out4 = (a.out + 3) & ~3;  // (ld3 is a multiple of 4: whole 16-byte pieces lie inside a row of d3)
     while (left) {
@@ -422,41 +589,48 @@ __global__ __launch_bounds__(64 * WAVES) void back_kernel(BackArgs a)
         const uint32_t member = (uint32_t)__ballot(mine == slot) & left;
         left &= ~member;
         if (slot < 0) {  // rows without an adapter: d3 is zero there
-            for (int e = threadIdx.x; e < 32 * a.n2; e += 64 * WAVES)
+            for (int e = threadIdx.x; e < 16 * T * a.n2; e += 64 * WAVES)
                 if ((member >> (e / a.n2)) & 1u) a.d2[(size_t)(row0 + e / a.n2) * a.ld2 + e % a.n2] = 0.0f;
-            for (int e = threadIdx.x; e < 32 * a.ldu; e += 64 * WAVES)
+            for (int e = threadIdx.x; e < 16 * T * a.ldu; e += 64 * WAVES)
                 if ((member >> (e / a.ldu)) & 1u) a.g2[(size_t)(row0 + e / a.ldu) * a.ldu + e % a.ldu] = a.g3[(size_t)(row0 + e / a.ldu) * a.ldu + e % a.ldu] = 0.0f;
             continue;
         }
         const float* a3 = a.a3 + (size_t)slot * a.per_slot;
         const float* b3 = a.b3 + (size_t)slot * a.per_slot;
         const float* b2 = a.b2 + (size_t)slot * a.per_slot;
-        const bool mem[2] = {((member >> r16) & 1u) != 0, ((member >> (16 + r16)) & 1u) != 0};
-        // g3^T: registers j = 16 n + 4 q + i of row r16 (every wave has all of it)
-        f32x4 g3[2][RT], g2[2][RT];
+        bool mem[T];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < T; ++t) mem[t] = ((member >> (16 * t + r16)) & 1u) != 0;
+        // g3^T: registers j = 16 n + 4 q + i of row r16 (every wave has all of it)
+        f32x4 g3[T][RT], g2[T][RT];
+#pragma unroll
+        for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int n = 0; n < RT; ++n) g3[t][n] = g2[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         for (int c0 = 0; c0 < out4; c0 += 16) {
             const int c = c0 + 4 * q;
-            f32x4 d[2];
+            f32x4 d[T];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) d[t] = *reinterpret_cast<const f32x4*>(a.d3 + row[t] * a.ld3 + min(c, a.ld3 - 4));
+            for (int t = 0; t < T; ++t) d[t] = *reinterpret_cast<const f32x4*>(a.d3 + row[t] * a.ld3 + min(c, a.ld3 - 4));
+            float b[4][RT];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int n = 0; n < RT; ++n) b[e][n] = b3[(size_t)min(16 * n + r16, a.rank - 1) * a.out + min(c + e, a.out - 1)];
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const bool in = c + e < a.out;
 #pragma unroll
                 for (int n = 0; n < RT; ++n) {
-                    float w = b3[(size_t)min(16 * n + r16, a.rank - 1) * a.out + min(c + e, a.out - 1)];
-                    w = in && 16 * n + r16 < a.rank ? w : 0.0f;
+                    const float w = keep_if(in && 16 * n + r16 < a.rank, b[e][n]);
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) g3[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, in ? d[t][e] : 0.0f, g3[t][n], 0, 0, 0);
+                    for (int t = 0; t < T; ++t) g3[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, in ? d[t][e] : 0.0f, g3[t][n], 0, 0, 0);
                 }
             }
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int n = 0; n < RT; ++n)
 #pragma unroll
@@ -465,50 +639,49 @@ __global__ __launch_bounds__(64 * WAVES) void back_kernel(BackArgs a)
                     const int j = 16 * n + 4 * q + i;
                     if (wave == 0 && mem[t] && j < a.ldu) a.g3[row[t] * a.ldu + j] = g3[t][n][i];
                 }
+#pragma unroll 2
         for (int tile = wave; tile < tiles; tile += WAVES) {
             const int n0 = 16 * tile, u = min(n0 + r16, a.n2 - 1);  // the unit whose weights this lane holds
-            f32x4 h[2], d2[2];
+            f32x4 h[T], d2[T];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < T; ++t) {
                 h[t] = *reinterpret_cast<const f32x4*>(a.h2 + row[t] * a.ld2 + n0 + 4 * q);
                 d2[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
-            float wb[4][RT];
+            f32x4 wb[RT], wa[RT];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int n = 0; n < RT; ++n) {
-                    const int j = 16 * n + r16, k = n0 + 4 * q + e;
-                    wb[e][n] = b2[(size_t)min(j, a.rank - 1) * a.n2 + min(k, a.n2 - 1)];
-                    wb[e][n] = j < a.rank && k < a.n2 ? wb[e][n] : 0.0f;
-                }
+            for (int n = 0; n < RT; ++n) {
+                wb[n] = ask_four<FOURS>(b2 + (size_t)min(16 * n + r16, a.rank - 1) * a.n2, n0 + 4 * q, a.n2);
+                wa[n] = ask_four<FOURS>(a3 + (size_t)u * a.rank, 16 * n + 4 * q, a.rank);
+            }
             for (int c0 = 0; c0 < out4; c0 += 16) {
                 const int c = c0 + 4 * q;
-                f32x4 d[2];
+                f32x4 d[T];
 #pragma unroll
-                for (int t = 0; t < 2; ++t) d[t] = *reinterpret_cast<const f32x4*>(a.d3 + row[t] * a.ld3 + min(c, a.ld3 - 4));
-                float w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = a.w3[(size_t)u * a.out + min(c + e, a.out - 1)];
+                for (int t = 0; t < T; ++t) d[t] = *reinterpret_cast<const f32x4*>(a.d3 + row[t] * a.ld3 + min(c, a.ld3 - 4));
+                f32x4 w = ask_four<FOURS>(a.w3 + (size_t)u * a.out, c, a.out);
+                __builtin_amdgcn_sched_barrier(0);
+                w = cut_four(w, c, a.out);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const bool in = c + e < a.out;
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) d2[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? w[e] : 0.0f, in ? d[t][e] : 0.0f, d2[t], 0, 0, 0);
+                    for (int t = 0; t < T; ++t) d2[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[e], in ? d[t][e] : 0.0f, d2[t], 0, 0, 0);
                 }
+            }
+#pragma unroll
+            for (int n = 0; n < RT; ++n) {
+                wb[n] = cut_four(wb[n], n0 + 4 * q, 16 * n + r16 < a.rank ? a.n2 : 0);
+                wa[n] = cut_four(wa[n], 16 * n + 4 * q, a.rank);
             }
 #pragma unroll
             for (int n = 0; n < RT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = 16 * n + 4 * q + e;
-                    float w = a3[(size_t)u * a.rank + min(j, a.rank - 1)];
-                    w = j < a.rank ? w : 0.0f;
+                for (int e = 0; e < 4; ++e)
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) d2[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, g3[t][n][e], d2[t], 0, 0, 0);
-                }
+                    for (int t = 0; t < T; ++t) d2[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(wa[n][e], g3[t][n][e], d2[t], 0, 0, 0);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < T; ++t) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) d2[t][i] *= 1.0f - h[t][i] * h[t][i];
                 // (columns between n2 and ld2 take products with zeros, or zeros: the padding of h2 and the clamped unit's
@@ -530,16 +703,16 @@ __global__ __launch_bounds__(64 * WAVES) void back_kernel(BackArgs a)
 #pragma unroll
                 for (int n = 0; n < RT; ++n)
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) g2[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(wb[e][n], d2[t][e], g2[t][n], 0, 0, 0);
+                    for (int t = 0; t < T; ++t) g2[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(wb[n][e], d2[t][e], g2[t][n], 0, 0, 0);
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int n = 0; n < RT; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) part[wave][t][16 * n + 4 * q + i][r16] = g2[t][n][i];
         __syncthreads();
-        for (int e = threadIdx.x; e < 32 * a.ldu; e += 64 * WAVES) {
+        for (int e = threadIdx.x; e < 16 * T * a.ldu; e += 64 * WAVES) {
             const int r = e / a.ldu, j = e % a.ldu;
             float s = 0.0f;
 #pragma unroll
