@@ -148,14 +148,17 @@ int group_rows(Adapters* a, const int32_t* slots_dev, uint32_t rows, hipStream_t
     return SZH_OK;
 }
 
-template <int NT, int OT, int WAVES, int UNR>
+// whether rows of `width` values, `apart` values from one to the next, can be read in aligned pieces of 16 bytes
+bool in_fours(const float* p, uint64_t width, uint64_t apart) { return width % 4 == 0 && apart % 4 == 0 && ((uintptr_t)p & 15) == 0; }
+
+template <int NT, int OT, int WAVES, int UNR, bool FOURS = false>
 int launch_low(LowArgs g, hipStream_t s)
 {
     constexpr size_t lds = (size_t)WAVES * 32 * NT * 16 * sizeof(float);
-    if (int rc = allow_dynamic_lds((const void*)low_kernel<NT, OT, WAVES, UNR>, lds)) return rc;
+    if (int rc = allow_dynamic_lds((const void*)low_kernel<NT, OT, WAVES, UNR, FOURS>, lds)) return rc;
     const unsigned tiles = (g.rows + 31) / 32;
     g.parts = tiles >= 512 ? 1 : (int)std::min<unsigned>(32, 1024 / tiles);
-    hipLaunchKernelGGL((low_kernel<NT, OT, WAVES, UNR>), dim3(tiles, g.parts), dim3(64 * WAVES), lds, s, g);
+    hipLaunchKernelGGL((low_kernel<NT, OT, WAVES, UNR, FOURS>), dim3(tiles, g.parts), dim3(64 * WAVES), lds, s, g);
     SZ_HIP(hipGetLastError());
     return SZH_OK;
 }
@@ -168,16 +171,18 @@ int low_product(const Adapters* a, const float* x, int ldx, int K, const float* 
     g.x = x; g.ldx = ldx; g.K = K; g.factor = factor; g.factor_slot = a->per_slot(); g.f_k = f_k; g.f_j = f_j;
     g.rank = (int)a->rank; g.row_slot = a->ws.row_slot; g.rows = rows; g.u = u; g.ldu = a->ws.ldu; g.scale = a->scale;
     ProfScope prof("adapt_low", s);
-    switch ((a->rank + 15) / 16) {
-    case 1: return launch_low<1, 0, 4, 4>(g, s);
-    case 2: return launch_low<2, 0, 4, 2>(g, s);
-    case 3: return launch_low<3, 0, 8, 2>(g, s);
-    default: return launch_low<4, 0, 4, 2>(g, s);
+    const bool fours = f_k == 1 && in_fours(factor, f_j, g.factor_slot);
+    switch ((a->rank + 15) / 16 * 2 + fours) {
+    case 2: return launch_low<1, 0, 4, 4>(g, s);
+    case 3: return launch_low<1, 0, 4, 4, true>(g, s);
+    case 4: return launch_low<2, 0, 4, 2>(g, s);
+    case 5: return launch_low<2, 0, 8, 4, true>(g, s);
+    case 6: return launch_low<3, 0, 4, 2>(g, s);
+    case 7: return launch_low<3, 0, 4, 2, true>(g, s);
+    case 8: return launch_low<4, 0, 4, 2>(g, s);
+    default: return launch_low<4, 0, 4, 2, true>(g, s);
     }
 }
-
-// whether rows of `width` values, `apart` values from one to the next, can be read in aligned pieces of 16 bytes
-bool in_fours(const float* p, uint64_t width, uint64_t apart) { return width % 4 == 0 && apart % 4 == 0 && ((uintptr_t)p & 15) == 0; }
 
 // h1 and u2 in one pass over x, straight from the caller's rows where `order` is given.  At rank 32 a wave's W1 and A2 leave
 // no registers for the rows to come, and the pass takes as long as the gather and the two products it replaces.
@@ -251,10 +256,10 @@ int factor_gradients(Adapters* a, uint32_t rows, hipStream_t s)
     const dim3 grid(tiles, (unsigned)chunks), block(256);
     ProfScope prof("adapt_grad", s);
     switch ((r + 15) / 16) {
-    case 1: hipLaunchKernelGGL((factor_grad_kernel<1>), grid, block, 0, s, g); break;
-    case 2: hipLaunchKernelGGL((factor_grad_kernel<2>), grid, block, 0, s, g); break;
-    case 3: hipLaunchKernelGGL((factor_grad_kernel<3>), grid, block, 0, s, g); break;
-    default: hipLaunchKernelGGL((factor_grad_kernel<4>), grid, block, 0, s, g); break;
+    case 1: hipLaunchKernelGGL((factor_grad_kernel<1, 4>), grid, block, 0, s, g); break;
+    case 2: hipLaunchKernelGGL((factor_grad_kernel<2, 4>), grid, block, 0, s, g); break;
+    case 3: hipLaunchKernelGGL((factor_grad_kernel<3, 2>), grid, block, 0, s, g); break;
+    default: hipLaunchKernelGGL((factor_grad_kernel<4, 2>), grid, block, 0, s, g); break;
     }
     hipLaunchKernelGGL(factor_reduce_kernel, dim3(blocks, a->slots), block, 0, s, g, a->d_grad, a->per_slot());
     SZ_HIP(hipGetLastError());

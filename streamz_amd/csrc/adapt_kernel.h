@@ -410,7 +410,8 @@ struct LowArgs {
 // pairs lane group q's k with k0 + 4 q + t, so that a lane reads 16 bytes of its row for four steps.  UNR blocks of
 // 16 k are requested at once: with as many rows as there are, what a wave does is wait.  NT tiles of 16
 // columns: OT of the output layer, then the rank's.  A column beyond the matrix takes another's values and is dropped.
-template <int NT, int OT, int WAVES, int UNR>
+// FOURS (OT = 0): f_k is 1 and the factor's columns are 16-byte aligned, in fours.
+template <int NT, int OT, int WAVES, int UNR, bool FOURS>
 __global__ __launch_bounds__(64 * WAVES) void low_kernel(LowArgs a)
 {
     extern __shared__ __attribute__((aligned(16))) float low_lds[];
@@ -462,9 +463,16 @@ __global__ __launch_bounds__(64 * WAVES) void low_kernel(LowArgs a)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) xv[i][t] = *reinterpret_cast<const f32x4*>(x[t] + 16 * (b + i));
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
+                for (int n = 0; n < NT; ++n) {
+                    if (FOURS) {
+                        const f32x4 v = *reinterpret_cast<const f32x4*>(col[n] + 16 * (b + i) + 4 * q);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) w[i][e][n] = col[n][(uint32_t)(16 * (b + i) + 4 * q + e) * step[n]];
+                        for (int e = 0; e < 4; ++e) w[i][e][n] = v[e];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[i][e][n] = col[n][(uint32_t)(16 * (b + i) + 4 * q + e) * step[n]];
+                    }
+                }
             }
             __builtin_amdgcn_sched_barrier(0);  // every load is asked for before the first is waited for
 #pragma unroll
@@ -747,7 +755,7 @@ struct FactorArgs {
 
 // 64 columns of p per workgroup; its four waves take rows in turn and are joined in LDS.  A lane reads 16
 // bytes of a row of p for four matrix instructions: step t's columns are 4 c + t.
-template <int NT>
+template <int NT, int G>
 __global__ __launch_bounds__(256) void factor_grad_kernel(FactorArgs a)
 {
     __shared__ __attribute__((aligned(16))) float part[4][64][NT * 16];
@@ -766,26 +774,26 @@ __global__ __launch_bounds__(256) void factor_grad_kernel(FactorArgs a)
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        // (two groups of four rows at a time: the loads of both are in flight)
-        for (uint32_t i = r + 4 * wave; i < stop; i += 32) {
-            f32x4 pv[2];
-            float wv[2][NT];
+        // (G groups of four rows at a time: the loads of all are asked for before the first is waited for)
+        for (uint32_t i = r + 4 * wave; i < stop; i += 16 * G) {
+            f32x4 pv[G];
+            float wv[G][NT];
             const int col = m0 + 4 * c16;
 #pragma unroll
-            for (int g2 = 0; g2 < 2; ++g2) {
+            for (int g2 = 0; g2 < G; ++g2) {
                 const size_t row = min(i + 16 * g2 + q, stop - 1);
                 pv[g2] = *reinterpret_cast<const f32x4*>(g.p + row * g.ldp + min(col, g.ldp - 4));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) wv[g2][n] = g.w[row * a.ldw + min(16 * n + c16, a.rank - 1)];
             }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int g2 = 0; g2 < 2; ++g2) {
+            for (int g2 = 0; g2 < G; ++g2) {
                 const bool in = i + 16 * g2 + q < stop;
-#pragma unroll
-                for (int t = 0; t < 4; ++t) pv[g2][t] = in && col + t < g.M ? pv[g2][t] : 0.0f;
+                pv[g2] = cut_four(pv[g2], col, in ? g.M : 0);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float v = in && 16 * n + c16 < a.rank ? wv[g2][n] : 0.0f;
+                    const float v = keep_if(in && 16 * n + c16 < a.rank, wv[g2][n]);
 #pragma unroll
                     for (int t = 0; t < 4; ++t) acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[g2][t], v, acc[t][n], 0, 0, 0);
                 }

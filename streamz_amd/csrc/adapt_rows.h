@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "adapt_kernel.h"
 #include "control_kernel.h"
 #include "gemm_kernel.h"
 
@@ -341,10 +342,11 @@ __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(ThinArgs g)
                 for (int j = 0; j < 4; ++j) {
                     const int k = half * steps + st + j;
                     bv[j] = up[(uint64_t)min(k, g.rank - 1) * g.N];
-                    bv[j] = k < g.rank ? bv[j] : 0.0f;
                 }
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(av[j], bv[j], acc, 0, 0, 0);
+                for (int j = 0; j < 4; ++j)
+                    acc = __builtin_amdgcn_mfma_f32_32x32x2f32(av[j], keep_if(half * steps + st + j < g.rank, bv[j]), acc, 0, 0, 0);
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -366,6 +368,7 @@ __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(ThinArgs g)
 #pragma unroll
             for (int e = 0; e < 4; ++e) wv[q][e] = w[(uint64_t)(8 * (b + q) + e) * g.N];
         }
+        __builtin_amdgcn_sched_barrier(0);  // every load is asked for before the first is waited for
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const float v[4] = {av[q].x, av[q].y, av[q].z, av[q].w};
@@ -374,13 +377,18 @@ __global__ __launch_bounds__(64 * kThinWaves) void thin_kernel(ThinArgs g)
         }
     }
     for (; b < b1; ++b) {
+        float av[4], wv[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int k = 8 * b + 4 * half + e;
-            const bool in = k < g.K;
-            const float av = in ? a[8 * b + e] : 0.0f;
-            const float wv = in ? w[(uint64_t)(8 * b + e) * g.N] : 0.0f;
-            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(av, wv, acc, 0, 0, 0);
+            const int k = min(8 * b + 4 * half + e, g.K - 1) - 4 * half;
+            av[e] = a[k];
+            wv[e] = w[(int64_t)k * g.N];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool in = 8 * b + 4 * half + e < g.K;
+            acc = __builtin_amdgcn_mfma_f32_32x32x2f32(keep_if(in, av[e]), keep_if(in, wv[e]), acc, 0, 0, 0);
         }
     }
 #pragma unroll
