@@ -91,9 +91,10 @@ def _split(flat, shapes):
 
 
 class _View:
-    """Device memory that the library owns, as torch takes it in."""
+    """Device memory that the library owns, as torch takes it in; the tensor keeps its owner."""
 
-    def __init__(self, ptr, shape, typestr="<f4"):
+    def __init__(self, ptr, shape, owner, typestr="<f4"):
+        self.owner = owner
         self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": typestr, "data": (ptr, False), "version": 2}
 
 
@@ -177,7 +178,7 @@ def prepare(case, seed):
         s["bank"].reserve(n, training=case["op"] == "train")
         s["handle"] = streamz_amd.LogitControls(**{k: v if k == "sets" else v.data_ptr() for k, v in s["controls"].items()}) if s["controls"] else None
         if case["op"] == "train":
-            grad = torch.as_tensor(_View(s["bank"].grad_ptr(), (s["bank"].grad_len(),)), device=dev)
+            grad = torch.as_tensor(_View(s["bank"].grad_ptr(), (s["bank"].grad_len(),), s["bank"]), device=dev)
             s["grad"] = grad[:case["slots"] * P].view(case["slots"], P)
             s["stats"] = grad[case["slots"] * P:].view(case["slots"], 2)
     return s
