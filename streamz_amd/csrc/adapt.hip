@@ -266,9 +266,7 @@ int factor_gradients(Adapters* a, uint32_t rows, hipStream_t s)
     return SZH_OK;
 }
 
-// d3 -> g3, d2, g2 in one launch; up to 64 classes (beyond them the product with w3 wants larger tiles)
-bool back_applies(const Adapters* a) { return a->out <= 64; }
-int back_rows(const Net* n, const Adapters* a, uint32_t rows, hipStream_t s)
+BackArgs back_args(const Net* n, const Adapters* a, uint32_t rows)
 {
     const AdaptWorkspace& w = a->ws;
     const float* F = a->d_params;
@@ -276,7 +274,41 @@ int back_rows(const Net* n, const Adapters* a, uint32_t rows, hipStream_t s)
     g.d3 = w.lg; g.h2 = w.h2; g.w3 = n->d_params + n->off_w3(); g.a3 = F + a->off_a3(); g.b3 = F + a->off_b3(); g.b2 = F + a->off_b2();
     g.per_slot = a->per_slot(); g.row_slot = w.row_slot; g.d2 = w.d2; g.g2 = w.g2; g.g3 = w.g3; g.rows = rows;
     g.n2 = (int)n->h2; g.out = (int)n->out; g.rank = (int)a->rank; g.ld2 = w.ld2; g.ld3 = w.ld3; g.ldu = w.ldu; g.scale = a->scale;
-    const bool fours = in_fours(g.w3, n->out, n->out) && in_fours(g.a3, a->rank, g.per_slot) && in_fours(g.b2, n->h2, g.per_slot);
+    return g;
+}
+bool back_fours(const Adapters* a, const BackArgs& g)
+{
+    return in_fours(g.w3, g.out, g.out) && in_fours(g.a3, a->rank, g.per_slot) && in_fours(g.b2, g.n2, g.per_slot);
+}
+
+// The output layer, the loss and back to d2 and the rank columns in one launch, lg taking d3
+bool tail_applies(const Adapters* a) { return a->out <= 64 && a->rank <= 16; }
+template <int OT>
+int launch_tail(const BackArgs& g, bool fours, const TailArgs& o, const Controls& ctl, const ControlRun& c, hipStream_t s)
+{
+    const dim3 grid((g.rows + 31) / 32), block(256);
+    ProfScope prof("adapt_tail", s);
+    if (fours) hipLaunchKernelGGL((tail_kernel<OT, true>), grid, block, 0, s, g, o, ctl, c);
+    else hipLaunchKernelGGL((tail_kernel<OT, false>), grid, block, 0, s, g, o, ctl, c);
+    SZ_HIP(hipGetLastError());
+    return SZH_OK;
+}
+int tail_rows(const Net* n, const Adapters* a, const Controls& ctl, const ControlRun& c, uint32_t rows, hipStream_t s)
+{
+    const BackArgs g = back_args(n, a, rows);
+    const TailArgs o{n->d_params + n->off_b3(), a->ws.u3, a->ws.lg};
+    const bool fours = back_fours(a, g);
+    if (n->out <= 16) return launch_tail<1>(g, fours, o, ctl, c, s);
+    if (n->out <= 32) return launch_tail<2>(g, fours, o, ctl, c, s);
+    return launch_tail<4>(g, fours, o, ctl, c, s);
+}
+
+// d3 -> g3, d2, g2 in one launch; up to 64 classes (beyond them the product with w3 wants larger tiles)
+bool back_applies(const Adapters* a) { return a->out <= 64; }
+int back_rows(const Net* n, const Adapters* a, uint32_t rows, hipStream_t s)
+{
+    const BackArgs g = back_args(n, a, rows);
+    const bool fours = back_fours(a, g);
     const dim3 grid((rows + 31) / 32);
     ProfScope prof("adapt_back", s);
     switch ((a->rank + 15) / 16 * 2 + fours) {
@@ -382,8 +414,8 @@ int shared_product(const GemmArgs& g, int Kp, float* wt, hipStream_t s)
 }
 
 // logits of `rows` grouped rows in the workspace's lg, activations in h1, h2, rank columns in u2, u3; x, in the caller's
-// order, unless gather_rows has put its rows into xs already (null)
-int forward_rows(Net* n, Adapters* a, const float* x, uint8_t* live, uint32_t rows, hipStream_t s)
+// order, unless gather_rows has put its rows into xs already (null); `tail`: as far as h2
+int forward_rows(Net* n, Adapters* a, const float* x, uint8_t* live, bool tail, uint32_t rows, hipStream_t s)
 {
     AdaptWorkspace& w = a->ws;
     const float* P = n->d_params;
@@ -419,7 +451,7 @@ int forward_rows(Net* n, Adapters* a, const float* x, uint8_t* live, uint32_t ro
     } else {
         rc = shared_product<EPI_ADAPT_TANH, T_ADAPT2>(g, w.ld1, w.w2t, s);
     }
-    if (rc || n->out == 0) return rc;
+    if (rc || n->out == 0 || tail) return rc;
     if (low_out_applies(a)) return low_out(n, a, rows, s);
     rc = low_product(a, w.h2, w.ld2, (int)n->h2, F + a->off_a3(), r, 1, rows, w.u3, s);
     if (rc) return rc;
@@ -517,7 +549,7 @@ int infer_rows(Net* n, Adapters* a, const float* x, const int32_t* slots_dev, ui
     int rc = group_rows(a, slots_dev, rows, s);
     const bool front = front_applies(n, a);
     if (!rc && !front) rc = gather_rows(a, x, rows, 0.0f, 0, 0, nullptr, s);
-    if (!rc) rc = forward_rows(n, a, front ? x : nullptr, nullptr, rows, s);
+    if (!rc) rc = forward_rows(n, a, front ? x : nullptr, nullptr, false, rows, s);
     c.order = a->ws.order;
     return rc ? rc : control_run(ctl, c, s);
 }
@@ -643,10 +675,12 @@ int adapters_accumulate(Net* n, Adapters* a, const float* x, const int32_t* labe
         c.out = w.lg; c.ld_out = w.ld3; c.labels = labels + r0; c.row_live = w.live0; c.row_slot = w.row_slot; c.loss = w.loss; c.live = w.live;
         const Controls ctl_r = from_row(ctl, r0);
         if (!rc && few) rc = forward_few(n, a, w.xs, w.ldx, w.row_slot, R, ctl_r, c, w.u2, w.u3, s);
-        if (!rc && !few) rc = forward_rows(n, a, front ? x + r0 * n->in : nullptr, w.live0, R, s);
-        if (!rc && !few) rc = control_run(ctl_r, c, s);   // lg now holds d3
+        const bool tail = !few && tail_applies(a);
+        if (!rc && !few) rc = forward_rows(n, a, front ? x + r0 * n->in : nullptr, w.live0, tail, R, s);
+        if (!rc && tail) rc = tail_rows(n, a, ctl_r, c, R, s);
+        if (!rc && !few && !tail) rc = control_run(ctl_r, c, s);   // lg now holds d3
         if (rc) return rc;
-        const bool back_done = few && (uint64_t)n->h2 * n->out <= kRowOutFloats;  // (by the row kernel)
+        const bool back_done = tail || (few && (uint64_t)n->h2 * n->out <= kRowOutFloats);  // (by the row kernel)
         if (!back_done && back_applies(a)) {
             rc = back_rows(n, a, R, s);
             if (rc) return rc;

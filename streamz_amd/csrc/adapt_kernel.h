@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "control_kernel.h"
 #include "rng.h"
 
 namespace sz {
@@ -575,11 +576,10 @@ struct BackArgs {
     int n2, out, rank, ld2, ld3, ldu;
     float scale;
 };
-// FOURS: the rows of W3, A3 and B2 are 16-byte aligned and in fours
-template <int RT, int WAVES, int T, bool FOURS>
-__global__ __launch_bounds__(64 * WAVES) void back_kernel(BackArgs a)
+// d3(t, row, c): four classes of a row of tile t.  FOURS: the rows of W3, A3 and B2 are 16-byte aligned and in fours.
+template <int RT, int WAVES, int T, bool FOURS, class D3>
+__device__ __forceinline__ void back_tiles(const BackArgs& a, float (*part)[T][RT * 16][17], D3 d3)
 {
-    __shared__ float part[WAVES][T][RT * 16][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r16 = lane & 15, q = lane >> 4;
     const uint32_t row0 = blockIdx.x * (16 * T);
@@ -619,7 +619,7 @@ __global__ __launch_bounds__(64 * WAVES) void back_kernel(BackArgs a)
             const int c = c0 + 4 * q;
             f32x4 d[T];
 #pragma unroll
-            for (int t = 0; t < T; ++t) d[t] = *reinterpret_cast<const f32x4*>(a.d3 + row[t] * a.ld3 + min(c, a.ld3 - 4));
+            for (int t = 0; t < T; ++t) d[t] = d3(t, row[t], c);
             float b[4][RT];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -666,7 +666,7 @@ __global__ __launch_bounds__(64 * WAVES) void back_kernel(BackArgs a)
                 const int c = c0 + 4 * q;
                 f32x4 d[T];
 #pragma unroll
-                for (int t = 0; t < T; ++t) d[t] = *reinterpret_cast<const f32x4*>(a.d3 + row[t] * a.ld3 + min(c, a.ld3 - 4));
+                for (int t = 0; t < T; ++t) d[t] = d3(t, row[t], c);
                 f32x4 w = ask_four<FOURS>(a.w3 + (size_t)u * a.out, c, a.out);
                 __builtin_amdgcn_sched_barrier(0);
                 w = cut_four(w, c, a.out);
@@ -688,10 +688,18 @@ __global__ __launch_bounds__(64 * WAVES) void back_kernel(BackArgs a)
                 for (int e = 0; e < 4; ++e)
 #pragma unroll
                     for (int t = 0; t < T; ++t) d2[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(wa[n][e], g3[t][n][e], d2[t], 0, 0, 0);
+            // Every matrix result is read before the first branch behind it: the compiler's count of wait states over several
+            // ways to one place can miss the shortest (seen: a result's last register read 3 states behind, where 10 are due).
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = d2[t][i] * (1.0f - h[t][i] * h[t][i]);
+                    asm volatile("" : "+v"(v));
+                    d2[t][i] = v;
+                }
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) d2[t][i] *= 1.0f - h[t][i] * h[t][i];
                 // (columns between n2 and ld2 take products with zeros, or zeros: the padding of h2 and the clamped unit's
                 // weights are finite or theirs alone; only whole pieces inside ld2 are stored)
                 if (mem[t]) {
@@ -729,6 +737,173 @@ __global__ __launch_bounds__(64 * WAVES) void back_kernel(BackArgs a)
         }
         __syncthreads();
     }
+}
+template <int RT, int WAVES, int T, bool FOURS>
+__global__ __launch_bounds__(64 * WAVES) void back_kernel(BackArgs a)
+{
+    __shared__ float part[WAVES][T][RT * 16][17];
+    back_tiles<RT, WAVES, T, FOURS>(a, part, [&](int, size_t row, int c) { return *reinterpret_cast<const f32x4*>(a.d3 + row * a.ld3 + min(c, a.ld3 - 4)); });
+}
+
+// The output layer and back in one launch, for up to 16 rank columns and 64 classes (OT tiles of 16): u3, the logits,
+// controls and softmax, the loss, d3, and what back_kernel makes of it.  A workgroup has 32 rows; their logits and
+// d3 stay in LDS, and what of h2 the second half reads is still in the cache.
+struct TailArgs {
+    const float* bias;
+    float *u3, *d3;   // [rows][ldu], [rows][ld3]
+};
+template <int OT, bool FOURS>
+__global__ __launch_bounds__(256) void tail_kernel(BackArgs a, TailArgs o, Controls ctl, ControlRun run)
+{
+    constexpr int WAVES = 4, T = 2, LD = 16 * OT + 4;
+    __shared__ __attribute__((aligned(16))) float sums[WAVES][T][(OT + 1) * 16][17];  // classes, then rank columns
+    __shared__ __attribute__((aligned(16))) float z[16 * T][LD];                       // logits, then d3
+    __shared__ float us[16 * T][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r16 = lane & 15, q = lane >> 4;
+    const uint32_t row0 = blockIdx.x * (16 * T);
+    const uint32_t my_row = row0 + (lane & 31);
+    const int mine = my_row < a.rows ? a.row_slot[my_row] : -1;
+    const uint32_t adapted = (uint32_t)__ballot(mine >= 0);
+    {
+        size_t row[T];
+#pragma unroll
+        for (int t = 0; t < T; ++t) row[t] = min(row0 + 16 * t + r16, a.rows - 1);
+        // transposed as in back_tiles: register i of a lane is class 16 y + 4 q + i, or that rank column, of row r16
+        f32x4 y[T][OT], u[T];
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+            u[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int n = 0; n < OT; ++n) y[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        const int tiles = (a.n2 + 15) / 16;
+        for (int tile = wave; tile < tiles; tile += WAVES) {
+            const int n0 = 16 * tile;
+            f32x4 h[T];
+            float w[4][OT], f[4];
+#pragma unroll
+            for (int t = 0; t < T; ++t) h[t] = *reinterpret_cast<const f32x4*>(a.h2 + row[t] * a.ld2 + n0 + 4 * q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int n = 0; n < OT; ++n) w[e][n] = a.w3[(size_t)min(n0 + 4 * q + e, a.n2 - 1) * a.out + min(16 * n + r16, a.out - 1)];
+            auto ask = [&](int slot) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[e] = a.a3[(size_t)slot * a.per_slot + (size_t)min(n0 + 4 * q + e, a.n2 - 1) * a.rank + min(r16, a.rank - 1)];
+            };
+            uint32_t left = adapted;
+            int slot = left ? __builtin_amdgcn_readlane(mine, __builtin_ctz(left)) : 0;
+            ask(slot);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool in = n0 + 4 * q + e < a.n2;
+#pragma unroll
+                for (int t = 0; t < T; ++t) h[t][e] = in ? h[t][e] : 0.0f;
+#pragma unroll
+                for (int n = 0; n < OT; ++n) {
+                    const float v = keep_if(in, w[e][n]);
+#pragma unroll
+                    for (int t = 0; t < T; ++t) y[t][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, h[t][e], y[t][n], 0, 0, 0);
+                }
+            }
+            while (left) {
+                left &= ~(uint32_t)__ballot(mine == slot);
+                f32x4 v[T];
+#pragma unroll
+                for (int t = 0; t < T; ++t) v[t] = u[t];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float g = keep_if(n0 + 4 * q + e < a.n2, f[e]);
+#pragma unroll
+                    for (int t = 0; t < T; ++t) v[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(g, h[t][e], v[t], 0, 0, 0);
+                }
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    const bool mem = __shfl(mine, 16 * t + r16) == slot;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) u[t][i] = mem ? v[t][i] : u[t][i];
+                }
+                if (left) {
+                    slot = __builtin_amdgcn_readlane(mine, __builtin_ctz(left));
+                    ask(slot);
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sums[wave][t][OT * 16 + 4 * q + i][r16] = u[t][i];
+#pragma unroll
+                for (int n = 0; n < OT; ++n) sums[wave][t][16 * n + 4 * q + i][r16] = y[t][n][i];
+            }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * T * 16; e += 64 * WAVES) {
+        const int r = e >> 4, j = e & 15;
+        const bool on = ((adapted >> r) & 1u) && j < a.rank;
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) s += sums[w][r >> 4][OT * 16 + j][r & 15];
+        s = on ? a.scale * s : 0.0f;
+        us[r][j] = s;
+        if (j < a.ldu && row0 + r < a.rows) o.u3[(size_t)(row0 + r) * a.ldu + j] = s;
+    }
+    __syncthreads();
+    // eight lanes have a row from here on, each every eighth class
+    const int r = threadIdx.x >> 3, l = threadIdx.x & 7;
+    const uint32_t i = min(row0 + r, a.rows - 1);
+    const bool real = row0 + r < a.rows;
+    const int slot = a.row_slot[i];
+    const float* b3 = a.b3 + (size_t)max(slot, 0) * a.per_slot;
+    const uint64_t row = run.order ? run.order[i] : i;
+    const control::RowControl rc = control::row_control(ctl, a.out, control::row_set(ctl, row));
+    float top = -INFINITY;
+    for (int c = l; c < a.out; c += 8) {
+        float b[16], v = 0.0f, low = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) b[j] = b3[(size_t)min(j, a.rank - 1) * a.out + c];
+        const float bias = o.bias[c];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) v += sums[w][r >> 4][c][r & 15];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) low = __builtin_fmaf(us[r][j], keep_if(slot >= 0 && j < a.rank, b[j]), low);
+        v = control::controlled(rc, v + low + bias, c);
+        z[r][c] = v;
+        top = fmaxf(top, v);
+    }
+    top = control::lanes_max<8>(top);
+    const float shift = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    for (int c = l; c < a.out; c += 8) {
+        const float e = control::exp_low(z[r][c] - shift);
+        z[r][c] = e;
+        sum += e;
+    }
+    sum = control::lanes_sum<8>(sum);
+    const bool some = !(sum <= 0.0f);  // (a NaN row stays one)
+    const float inv = some ? 1.0f / sum : 0.0f;
+    const control::TrainRow tr = control::train_row(run, rc, i, row, a.out, some);
+    for (int c = l; c < LD; c += 8) {
+        float v = 0.0f;
+        if (c < a.out && tr.live) {
+            const float p = z[r][c] * inv;
+            v = c == tr.label ? p - 1.0f : p;
+            if (real && c == tr.label) run.loss[i] = -logf(fmaxf(p, 1e-12f));
+        }
+        z[r][c] = v;
+        if (real && c < a.out) o.d3[(size_t)i * a.ld3 + c] = v;
+    }
+    if (real && l == 0) {
+        run.live[i] = tr.live ? 1 : 0;
+        if (!tr.live) run.loss[i] = 0.0f;
+    }
+    __syncthreads();
+    back_tiles<1, WAVES, T, FOURS>(a, reinterpret_cast<float (*)[T][16][17]>(&sums[0][0][0][0]),
+                                   [&](int t, size_t, int c) { return *reinterpret_cast<const f32x4*>(&z[16 * t + r16][min(c, 16 * OT)]); });
 }
 
 // ---- factor gradients -----------------------------------------------------------------------------
@@ -841,7 +1016,16 @@ __global__ __launch_bounds__(256) void slot_stats_kernel(const float* __restrict
     __shared__ double sl[256], sc[256];
     const int slot = blockIdx.x;
     double l = 0.0, c = 0.0;
-    for (uint32_t i = begin[slot] + threadIdx.x; i < begin[slot + 1]; i += 256) { l += (double)loss[i]; c += (double)live[i]; }
+    // (eight rows a thread in flight; those behind the last as zeros)
+    const uint32_t end = begin[slot + 1];
+    for (uint32_t i = begin[slot] + threadIdx.x; i < end; i += 8 * 256) {
+        float a[8], b[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { const uint32_t at = min(i + 256 * k, end - 1); a[k] = loss[at]; b[k] = (float)live[at]; }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { l += (double)keep_if(i + 256 * k < end, a[k]); c += (double)keep_if(i + 256 * k < end, b[k]); }
+    }
     sl[threadIdx.x] = l; sc[threadIdx.x] = c;
     __syncthreads();
     for (int o = 128; o > 0; o >>= 1) {

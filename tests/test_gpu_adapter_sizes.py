@@ -30,6 +30,13 @@ BORDERS = [
     ((60, 96, 72, 65), 4, 20, 600, "mixed"),
     ((60, 96, 72, 300), 4, 20, 200, "mixed"),
     ((60, 96, 300, 300), 4, 20, 40, "mixed"),
+    # the output layer and back in one launch, or not; w3 streamed by every row, or not
+    ((60, 70, 50, 16), 4, 16, 300, "mixed"),
+    ((60, 70, 50, 17), 4, 15, 300, "mixed"),
+    ((60, 70, 50, 33), 300, 16, 400, "mixed"),
+    ((60, 70, 50, 64), 4, 16, 290, "runs"),
+    ((60, 70, 1100, 64), 4, 9, 100, "mixed"),
+    ((60, 70, 1100, 63), 4, 20, 100, "mixed"),
     # rows put in the order of their slots by one workgroup, or by four launches
     ((60, 32, 16, 4), 5, 4, 8192, "mixed"),
     ((60, 32, 16, 4), 5, 4, 8193, "mixed"),
