@@ -96,6 +96,14 @@ __device__ __forceinline__ float relu_max(float v)
     asm("v_max_f32 %0, 0, %1" : "=v"(r) : "v"(v));
     return r;
 }
+// The same of a matrix instruction's own result: the median of v, 0 and infinity (0 for a NaN).  The compiler counts no wait
+// states before an instruction in asm, and of a known infinity it makes the maximum with its second instruction again.
+__device__ __forceinline__ float relu_of_product(float v)
+{
+    float inf = INFINITY;
+    asm("" : "+s"(inf));
+    return __builtin_amdgcn_fmed3f(v, 0.0f, inf);
+}
 
 __device__ __forceinline__ Frag4 load4(const float* base, int64_t row, int col, int ld, int row_max, int col_max,
                                        int vec)

@@ -268,7 +268,7 @@ __global__ __launch_bounds__(kThreads) void infer_vote_kernel(Args a)
                 for (int q = 0; q < 4; ++q) {
                     f32x4v o;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[i] = gemm::relu_max(acc[4 * q + i]);
+                    for (int i = 0; i < 4; ++i) o[i] = gemm::relu_of_product(acc[4 * q + i]);
                     *reinterpret_cast<f32x4v*>(dst + 8 * q) = o;
                 }
             }
