@@ -196,7 +196,8 @@ int front_rows(const Net* n, const Adapters* a, const float* x, int ldx, const u
     g.in = (int)n->in; g.ldx = ldx; g.n1 = (int)n->h1; g.ld1 = w.ld1; g.rank = (int)a->rank; g.ldu = w.ldu; g.scale = a->scale;
     const bool fours = in_fours(x, n->in, ldx) && in_fours(g.w1, n->h1, n->h1) && in_fours(g.b1, n->h1, 0);
     const int waves = (g.n1 + 63) / 64;
-    const size_t lds = (size_t)2 * waves * 16 * 17 * sizeof(float);
+    const size_t lds = (size_t)2 * kFrontGroup * waves * 16 * 17 * sizeof(float);
+    if (int rc = allow_dynamic_lds(fours ? (const void*)front_kernel<true> : (const void*)front_kernel<false>, lds)) return rc;
     const dim3 grid(std::min<unsigned>((rows + 15) / 16, (unsigned)compute_units() * (kFrontWaves / waves))), block(64 * waves);
     ProfScope prof("adapt_h1", s);
     if (fours) hipLaunchKernelGGL((front_kernel<true>), grid, block, lds, s, g);

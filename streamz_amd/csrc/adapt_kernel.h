@@ -238,8 +238,13 @@ __device__ __forceinline__ f32x4 cut_four(f32x4 v, int at, int end)
 // matrix instruction's columns), with unit n0 + 4 (4 (m % 4) + m / 4) + c in row m of the instruction's tile c: a result's
 // register i of the four tiles is units n0 + 16 i + 4 q + 0 .. 3 of one row, a 16-byte store and the next product's operand
 // as it is.  u2, a sum over all units, is joined in LDS, in the order of the waves.  Rows of another slot than the one at
-// hand keep their sums: what a row gets does not depend on its neighbours.  Bound by matrix instructions.
+// hand keep their sums: what a row gets does not depend on its neighbours.
+// 66140 x 60 x 512 with rank 16: 74 us, of which the matrix instructions take 38 and writing h1 28 (the gather, the product
+// and the pass over h1 that it replaces took 17, 57 and 29).  The two waves of a SIMD unit go through products, stores and
+// joins nearly in step, so that these add up; a barrier at every fourth tile instead of every one lets them drift (80 -> 74),
+// 32 rows at a time (82) or raised priority of one of them (80 .. 87) do not help.
 constexpr int kFrontWaves = 8, kFrontIn = 64;
+constexpr int kFrontGroup = 4;  // tiles from one barrier to the next
 struct FrontArgs {
     const float* x;
     const uint32_t* order;   // null: x's rows are in order
@@ -256,7 +261,7 @@ struct FrontArgs {
 template <bool FOURS>
 __global__ __launch_bounds__(64 * kFrontWaves) void front_kernel(FrontArgs a)
 {
-    extern __shared__ __attribute__((aligned(16))) float front_lds[];  // [2][waves][16][17]
+    extern __shared__ __attribute__((aligned(16))) float front_lds[];  // [2 kFrontGroup][waves][16][17]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const int r16 = lane & 15, q = lane >> 4;
     const uint32_t tiles = (a.rows + 15) / 16;
@@ -297,7 +302,7 @@ __global__ __launch_bounds__(64 * kFrontWaves) void front_kernel(FrontArgs a)
     // one of those: behind a store that may not have happened the wait for the next x would be for the store as well.
     float* spare = a.h1 + (size_t)(a.rows + 31) * a.ld1 + 4 * (lane & 7);
     int r_out = threadIdx.x / a.ldu, j_out = threadIdx.x % a.ldu;
-    auto part_of = [&](uint32_t tile) { return reinterpret_cast<float (*)[16][17]>(front_lds) + ((tile - first) & 1) * waves; };
+    auto part_of = [&](uint32_t tile) { return reinterpret_cast<float (*)[16][17]>(front_lds) + ((tile - first) % (2 * kFrontGroup)) * waves; };
     auto join = [&](uint32_t tile) {
         const float (*part)[16][17] = part_of(tile);
         for (int e = threadIdx.x, r = r_out, j = j_out; e < 16 * a.ldu; e += blockDim.x, r = e / a.ldu, j = e % a.ldu) {
@@ -337,7 +342,7 @@ __global__ __launch_bounds__(64 * kFrontWaves) void front_kernel(FrontArgs a)
             for (int e = 0; e < 4; ++e)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) h[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[b][e][c], x[b][e], h[c], 0, 0, 0);
-        if (tile > first) join(tile - 1);  // (beside the matrix instructions)
+        if (tile >= first + kFrontGroup) join(tile - kFrontGroup);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int n = n0 + 16 * i + 4 * q;
@@ -378,12 +383,12 @@ __global__ __launch_bounds__(64 * kFrontWaves) void front_kernel(FrontArgs a)
 #pragma unroll
         for (int b = 0; b < 4; ++b) x[b] = cut_four(next[b], 16 * b + 4 * q, a.in);
         slot_of = slot_next;
-        // (two buffers: who writes the next but one has passed the next barrier, and with it everyone's reads of this one)
+        // (who writes a buffer again has passed the barrier behind everyone's reads of it)
 #pragma unroll
         for (int i = 0; i < 4; ++i) part_of(tile)[wave][4 * q + i][r16] = u[i];
-        __syncthreads();
+        if ((tile - first) % kFrontGroup == kFrontGroup - 1 || tile + 1 == last) __syncthreads();
     }
-    join(last - 1);
+    for (uint32_t tile = last - min(last - first, (uint32_t)kFrontGroup); tile < last; ++tile) join(tile);
 }
 
 // ---- products with the rank columns ----------------------------------------------------------------
