@@ -38,9 +38,9 @@ using namespace adapt;
 constexpr uint64_t kAdaptRows = 131072;
 
 // Calls of up to this many rows go row by row (adapt_rows.h); of half as many in training, whose row kernels do more.
-// Forward, on rows and on tiles: 23 and 36 us at 256 rows of 60-512-256-16, 38 and 40 at 512, 65 and 47 at 1024; 58 and
-// 87 us at 64 rows of 60-2048-2048-256, 124 and 149 at 512, 222 and 178 at 1024.  Training: 61 and 80 us at 256 rows of the
-// small network, 93 and 92 at 512.
+// Forward, on rows and on tiles: 24 and 32 us at 256 rows of 60-512-256-16 with rank 16, 38 and 35 at 512 (rank 32: 38 and 41),
+// 52 and 33 at 768; 65 and 90 us at 96 rows of 60-2048-2048-256, 141 and 152 at 512, 201 and 164 at 768.  Training: 56 and
+// 72 us at 256 rows of the small network, 73 and 62 at 384; 174 and 194 us of the wide one, 219 and 220.
 constexpr uint64_t kFewRows = 512;
 
 inline int round_up(int v, int to) { return (v + to - 1) / to * to; }
