@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "control_kernel.h"
+#include "gemm_kernel.h"
 #include "rng.h"
 
 namespace sz {
@@ -294,23 +295,48 @@ __global__ __launch_bounds__(64 * kFrontWaves) void front_kernel(FrontArgs a)
     for (int b = 0; b < 4; ++b)
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[b][e] = cut_four(w[b][e], unit4, 16 * b + 4 * q + e < a.in ? a.n1 : 0);
+    f32x4 start[4];  // the bias as the products start from it, [tile of the instruction]
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bias[i] = cut_four(bias[i], n0 + 16 * i + 4 * q, a.n1);
+    for (int i = 0; i < 4; ++i) {
+        bias[i] = cut_four(bias[i], n0 + 16 * i + 4 * q, a.n1);
 #pragma unroll
-    for (int b = 0; b < 4; ++b) x[b] = cut_four(x[b], 16 * b + 4 * q, a.in);
+        for (int c = 0; c < 4; ++c) start[c][i] = bias[i][c];
+    }
+    // only the last piece of x can reach beyond the inputs
+    const int tail = (a.in - 1) / 16;
+    auto cut_x = [&](f32x4* v) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+            if (b >= tail) v[b] = cut_four(v[b], 16 * b + 4 * q, a.in);
+    };
+    cut_x(x);
+    // where a lane's four stores of the tile at hand go, and how far on the next tile's are
+    float* dst[4];
+    size_t on[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int n = n0 + 16 * i + 4 * q;
+        dst[i] = n < a.ld1 ? a.h1 + (size_t)(16 * first + r16) * a.ld1 + n : a.h1 + (size_t)(a.rows + 31) * a.ld1 + 4 * (lane & 7);
+        on[i] = n < a.ld1 ? (size_t)16 * a.ld1 : 0;
+    }
     // Every lane stores at every tile, those without a row into the rows behind the last one, those without a unit into
     // one of those: behind a store that may not have happened the wait for the next x would be for the store as well.
-    float* spare = a.h1 + (size_t)(a.rows + 31) * a.ld1 + 4 * (lane & 7);
     int r_out = threadIdx.x / a.ldu, j_out = threadIdx.x % a.ldu;
     auto part_of = [&](uint32_t tile) { return reinterpret_cast<float (*)[16][17]>(front_lds) + ((tile - first) % (2 * kFrontGroup)) * waves; };
-    auto join = [&](uint32_t tile) {
+    auto join_one = [&](uint32_t tile, int r, int j) {
         const float (*part)[16][17] = part_of(tile);
-        for (int e = threadIdx.x, r = r_out, j = j_out; e < 16 * a.ldu; e += blockDim.x, r = e / a.ldu, j = e % a.ldu) {
-            float s = 0.0f;
+        float s = 0.0f;
+        if (waves == kFrontWaves) {
 #pragma unroll
-            for (int v = 0; v < kFrontWaves; ++v) s += keep_if(v < waves, part[min(v, waves - 1)][j][r]);
-            if (16 * tile + r < a.rows) a.u2[(size_t)(16 * tile + r) * a.ldu + j] = j < a.rank ? a.scale * s : 0.0f;
+            for (int v = 0; v < kFrontWaves; ++v) s += part[v][j][r];
+        } else {
+            for (int v = 0; v < waves; ++v) s += part[v][j][r];
         }
+        if (16 * tile + r < a.rows) a.u2[(size_t)(16 * tile + r) * a.ldu + j] = j < a.rank ? a.scale * s : 0.0f;
+    };
+    auto join = [&](uint32_t tile) {
+        if ((int)threadIdx.x < 16 * a.ldu) join_one(tile, r_out, j_out);
+        for (int e = threadIdx.x + blockDim.x; e < 16 * a.ldu; e += blockDim.x) join_one(tile, e / a.ldu, e % a.ldu);
     };
     int have = -1;      // the slot that f belongs to
     float f[4][4];      // A2 of unit n0 + 16 i + 4 q + c, rank column r16
@@ -333,9 +359,7 @@ __global__ __launch_bounds__(64 * kFrontWaves) void front_kernel(FrontArgs a)
         }
         f32x4 h[4];  // [tile of the instruction]
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) h[c][i] = bias[i][c];
+        for (int c = 0; c < 4; ++c) h[c] = start[c];
 #pragma unroll
         for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -345,11 +369,11 @@ __global__ __launch_bounds__(64 * kFrontWaves) void front_kernel(FrontArgs a)
         if (tile >= first + kFrontGroup) join(tile - kFrontGroup);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int n = n0 + 16 * i + 4 * q;
             f32x4 v;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) h[c][i] = v[c] = h[c][i] > 0.0f ? h[c][i] : 0.0f;
-            *reinterpret_cast<f32x4*>(n < a.ld1 ? a.h1 + (size_t)row * a.ld1 + n : spare) = v;
+            for (int c = 0; c < 4; ++c) h[c][i] = v[c] = gemm::relu_of_product(h[c][i]);
+            *reinterpret_cast<f32x4*>(dst[i]) = v;
+            dst[i] += on[i];
         }
         f32x4 u = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         uint32_t left = (uint32_t)__ballot(in && slot_of >= 0) & 0xffffu;
@@ -381,7 +405,8 @@ __global__ __launch_bounds__(64 * kFrontWaves) void front_kernel(FrontArgs a)
             for (int i = 0; i < 4; ++i) u[i] = mem ? v[0][i] + v[1][i] : u[i];
         }
 #pragma unroll
-        for (int b = 0; b < 4; ++b) x[b] = cut_four(next[b], 16 * b + 4 * q, a.in);
+        for (int b = 0; b < 4; ++b) x[b] = next[b];
+        cut_x(x);
         slot_of = slot_next;
         // (who writes a buffer again has passed the barrier behind everyone's reads of it)
 #pragma unroll
