@@ -476,8 +476,8 @@ int szh_wav_info(const char *path, uint64_t *n_frames, uint32_t *sample_rate, ui
  * synchronises the device, writes one line "tag launches total_ms" per kernel tag seen since
  * the previous report into buf (NUL-terminated, truncated to capacity) and returns the full
  * text length.  Tags: mfcc_base, finish, prep, fwd1, fwd2, fwd3, softmax, delta2, delta1,
- * dw3, dw2, dw1, bias, reduce, apply, vote, clip, control, control_loss, adapt_group, adapt_low, adapt_grad,
- * adapt_h1, adapt_h2, adapt_out, adapt_d2. */
+ * dw3, dw2, dw1, bias, reduce, apply, vote, clip, control, control_loss, adapt_group, adapt_h1, adapt_low, w2t, w2split,
+ * adapt_h2, adapt_out, adapt_tail, adapt_back, adapt_d2, adapt_grad, adapt_row_h1, adapt_row_out. */
 int szh_profile_enable(int on);
 int64_t szh_profile_report(char *buf, uint64_t capacity);
 
