@@ -95,6 +95,8 @@ int ensure(Adapters* a, uint64_t rows, bool training, hipStream_t s)
     rows = std::min<uint64_t>(std::max<uint64_t>(rows, 256), kAdaptRows);
     if (a->ws_rows >= rows && (a->ws_training || !training)) return SZH_OK;
     if (capturing(s)) { set_error("adapters: the workspace must be reserved before a stream is captured (szh_adapters_reserve)"); return SZH_EINVAL; }
+    // (at least doubled when it grows: the old ones stay, and together they are no larger than the last)
+    if (rows > a->ws_rows) rows = std::max<uint64_t>(rows, std::min<uint64_t>(2 * a->ws_rows, kAdaptRows));
     rows = std::max<uint64_t>(rows, a->ws_rows);
     rows = (rows + 255) / 256 * 256;
     training = training || a->ws_training;

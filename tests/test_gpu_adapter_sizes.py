@@ -213,3 +213,22 @@ def test_clip_a_group_of_very_many_tensors(count):
     for h, a, k in zip(host, at, lens):
         np.testing.assert_allclose(got[a:a + k], 0.25 * h.astype(np.float64), rtol=2.1 * tr.U, atol=0)
         assert got[a + k] == 0
+
+
+def test_a_workspace_that_grows_call_by_call_stays_in_proportion():
+    """Earlier workspaces are kept for the graphs that work in them; forty calls, each a little larger, must not keep forty of them."""
+    import torch
+    dims = (60, 512, 256, 16)
+    rng = np.random.default_rng(2)
+    params, flat, x = make(rng, dims, 2, 16, 16)
+    net = sz.SimpleNeuralNet(*dims, init=params)
+    bank = sz.Adapters(net, 2, 16, init=flat)
+    n = 4096 + 40 * 256
+    dx, ds, out = torch.zeros(n, 60, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda"), torch.zeros(n, 16, device="cuda")
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for k in range(41):
+        net.forward_adapted_dev(bank, dx.data_ptr(), ds.data_ptr(), 4096 + 256 * k, probs_ptr=out.data_ptr())
+    torch.cuda.synchronize()
+    # 4096, 8192 and 16384 rows of 3.5 KB and three copies of the weights' tables: 110 MB; forty-one of them are 1.4 GB
+    assert free - torch.cuda.mem_get_info()[0] < 300 << 20
