@@ -360,7 +360,8 @@ uint64_t szh_adapters_param_count(const szh_adapters *bank); /* of one slot */
 int szh_adapters_get_params(szh_adapters *bank, uint32_t slot, float *flat);
 int szh_adapters_set_params(szh_adapters *bank, uint32_t slot, const float *flat);
 int szh_adapters_reserve(szh_adapters *bank, uint64_t rows, int training);
-/* logits_dev[n][output] (before any control) and probs_dev[n][output]; either may be NULL.  controls may be NULL. */
+/* logits_dev[n][output] (before any control) and probs_dev[n][output]; either may be NULL, and neither may overlap the other
+ * or the features.  controls may be NULL. */
 int szh_net_forward_adapted_dev(szh_net *net, szh_adapters *bank, const float *feats_dev, const int32_t *slots_dev, uint64_t n,
                                 const szh_logit_controls *controls, float *logits_dev, float *probs_dev, void *stream);
 /* Votes of identify_speaker_list (lib.rs:1391-1402) for many requests at once: a row's top class (the last maximum wins)

@@ -232,3 +232,19 @@ def test_a_workspace_that_grows_call_by_call_stays_in_proportion():
     torch.cuda.synchronize()
     # 4096, 8192 and 16384 rows of 3.5 KB and three copies of the weights' tables: 110 MB; forty-one of them are 1.4 GB
     assert free - torch.cuda.mem_get_info()[0] < 300 << 20
+
+
+def test_results_that_overlap_are_refused():
+    import torch
+    net = sz.SimpleNeuralNet(60, 32, 16, 4, seed=1)
+    bank = sz.Adapters(net, 2, 3)
+    n = 10
+    x, s, o = torch.zeros(n * 60, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda"), torch.zeros(2 * n * 4, device="cuda")
+    a, b = o.data_ptr(), o.data_ptr() + 4 * 4 * n
+    for kw in (dict(logits_ptr=a, probs_ptr=a), dict(logits_ptr=a, probs_ptr=b - 4), dict(logits_ptr=b - 4, probs_ptr=a),
+               dict(probs_ptr=x.data_ptr()), dict(logits_ptr=x.data_ptr() + 4 * (60 * n - 1))):
+        with pytest.raises(sz.StreamzError) as e:
+            net.forward_adapted_dev(bank, x.data_ptr(), s.data_ptr(), n, **kw)
+        assert e.value.code == -1 and "overlap" in str(e.value)
+    net.forward_adapted_dev(bank, x.data_ptr(), s.data_ptr(), n, logits_ptr=a, probs_ptr=b)
+    torch.cuda.synchronize()
