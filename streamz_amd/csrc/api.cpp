@@ -1205,6 +1205,8 @@ int szh_logits_control_dev(const float* logits_dev, uint64_t ld_logits, uint64_t
     if (!logits_dev || !out_dev) { set_error("null argument"); return SZH_EINVAL; }
     if (classes > (1u << 30) || rows > (1ull << 40)) { set_error("too many rows or classes"); return SZH_EINVAL; }
     if (ld_logits < classes || ld_out < classes || ld_logits > (1ull << 40) || ld_out > (1ull << 40)) { set_error("row strides must be at least the number of classes"); return SZH_EINVAL; }
+    if (std::max(ld_logits, ld_out) > (1ull << 46) / rows) { set_error("too many rows or classes"); return SZH_EINVAL; }
+    if (((uintptr_t)logits_dev | (uintptr_t)out_dev) & 3) { set_error("address is not a multiple of 4"); return SZH_EINVAL; }
     const uintptr_t a0 = (uintptr_t)logits_dev, a1 = a0 + ((rows - 1) * ld_logits + classes) * sizeof(float);
     const uintptr_t b0 = (uintptr_t)out_dev, b1 = b0 + ((rows - 1) * ld_out + classes) * sizeof(float);
     if (a0 < b1 && b0 < a1 && !(a0 == b0 && ld_logits == ld_out)) { set_error("logits and result overlap"); return SZH_EINVAL; }

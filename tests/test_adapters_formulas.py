@@ -108,6 +108,17 @@ def test_controls_refuse(kw, text):
     refused(lambda: sz.control_logits_dev(**kw), text)
 
 
+@pytest.mark.parametrize("kw,text", [
+    (dict(rows=1 << 40, ld_logits=1 << 40), "too many"),     # (their product is 0 in 64 bits)
+    (dict(rows=1 << 40, ld_out=1 << 30), "too many"),
+    (dict(logits_ptr=A + 2), "multiple of 4"),
+    (dict(out_ptr=A + (1 << 16) + 1), "multiple of 4"),
+])
+def test_controls_refuse_sizes_and_addresses_that_do_not_exist(kw, text):
+    kw = {**dict(logits_ptr=A, rows=4, classes=16, controls=None, out_ptr=A + (1 << 16)), **kw}
+    refused(lambda: sz.control_logits_dev(**kw), text)
+
+
 def test_controls_refuse_an_unknown_result_and_take_empty_calls():
     L = sz.lib()
     assert L.szh_logits_control_dev(A, 4, 1, 4, None, 2, A + 4096, 4, None) == -1
