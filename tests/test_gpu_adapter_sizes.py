@@ -46,6 +46,7 @@ BORDERS = [
     # hidden products of whole rounds of wide tiles with a few rows behind them
     ((60, 256, 2048, 3), 7, 40, 8197, "runs"),
     ((60, 256, 2048, 3), 7, 16, 8192, "mixed"),
+    ((60, 256, 2048, 3), 7, 16, 7990, "runs"),
 ]
 
 
@@ -248,3 +249,116 @@ def test_results_that_overlap_are_refused():
         assert e.value.code == -1 and "overlap" in str(e.value)
     net.forward_adapted_dev(bank, x.data_ptr(), s.data_ptr(), n, logits_ptr=a, probs_ptr=b)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dims", [(60, 64, 32, 8), (60, 64, 48, 100), (60, 64, 300, 300)])
+@pytest.mark.parametrize("n", [1, 45, 700])
+@pytest.mark.parametrize("asked", ["logits", "probs", "both"])
+@pytest.mark.parametrize("sets", ["one", "by row"])
+def test_forward_with_penalties_and_one_result_or_both(dims, n, asked, sets):
+    import torch
+    slots, rank, C = 3, 5, dims[3]
+    rng = np.random.default_rng(sum(dims) + n)
+    params, flat, x = make(rng, dims, slots, rank, n)
+    s = pick_slots(rng, n, slots, "mixed")
+    net = sz.SimpleNeuralNet(*dims, init=params)
+    bank = sz.Adapters(net, slots, rank, scale=0.7, init=flat)
+    c = host_controls(rng, 4, C, n)
+    c["counts"] = np.maximum(rng.integers(-5, 4, (4, C)), 0).astype(np.uint32)
+    c["repetition"] = rng.uniform(0.6, 1.7, 4).astype(np.float32)
+    c["presence"] = rng.uniform(-1, 1, 4).astype(np.float32)
+    c["frequency"] = rng.uniform(-0.2, 0.2, 4).astype(np.float32)
+    if sets == "one":
+        c.pop("set_of_row")
+    handle, keep = dev_controls(c)
+    if sets == "one":
+        c["set_of_row"] = np.zeros(n, np.int32)
+    dx, ds = dev(x), dev(s)
+    out = [torch.full((n + 1, C), 7.0, device="cuda") for _ in range(2)]
+    net.forward_adapted_dev(bank, dx.data_ptr(), ds.data_ptr(), n, logits_ptr=out[0].data_ptr() if asked != "probs" else 0,
+                            probs_ptr=out[1].data_ptr() if asked != "logits" else 0, controls=handle)
+    torch.cuda.synchronize()
+    want = tr.layers(params, flat, known(slots, s), 0.7, x, rank, dims)[4]
+    if asked != "probs":
+        tr.check(out[0][:n].cpu().numpy(), want, "logits")
+    if asked != "logits":
+        tr.check(out[1][:n].cpu().numpy(), tr.control(want, c, C)[1], "probabilities")
+    assert (out[0][n] == 7).all() and (out[1][n] == 7).all()
+    assert (out[0] == 7).all() or asked != "probs"
+    assert (out[1] == 7).all() or asked != "logits"
+
+
+@pytest.mark.parametrize("dims", [(60, 64, 32, 8), (60, 64, 48, 100), (60, 64, 300, 300)])
+@pytest.mark.parametrize("n", [1, 60, 512, 513])
+def test_votes_of_few_rows_and_of_tiles(dims, n):
+    import torch
+    slots, rank, groups, thr, C = 4, 3, 5, 0.01, dims[3]
+    rng = np.random.default_rng(sum(dims) + n)
+    params, flat, x = make(rng, dims, slots, rank, n)
+    s, group = pick_slots(rng, n, slots, "mixed"), rng.integers(-1, groups + 1, n).astype(np.int32)
+    net = sz.SimpleNeuralNet(*dims, init=params)
+    bank = sz.Adapters(net, slots, rank, init=flat)
+    c = host_controls(rng, 3, C, n)
+    handle, keep = dev_controls(c)
+    _, probs = forward(net, bank, x, s, handle)
+    dx, ds, dg = dev(x), dev(s), dev(group)
+    for groups_of in (dg.data_ptr(), 0):
+        counts = torch.full((groups, C), 3, dtype=torch.int64, device="cuda")
+        net.vote_adapted_dev(bank, dx.data_ptr(), ds.data_ptr(), n, thr, counts.data_ptr(), groups=groups, group_of_row_ptr=groups_of, controls=handle)
+        torch.cuda.synchronize()
+        want = np.full((groups, C), 3, np.int64)
+        for i in range(n):
+            g = group[i] if groups_of else 0
+            if 0 <= g < groups and probs[i].max() > 0 and probs[i].max() >= np.float32(thr):
+                want[g, C - 1 - int(np.argmax(probs[i][::-1]))] += 1
+        assert np.array_equal(counts.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dims,rank", [((60, 512, 64, 8), 16), ((60, 70, 50, 40), 20), ((60, 96, 72, 100), 7)])
+def test_tiles_in_a_graph(dims, rank):
+    """Other inputs and other slots at every replay, eager work between them."""
+    import torch
+    slots, n, C = 6, 1500, dims[3]
+    rng = np.random.default_rng(sum(dims))
+    params, flat, x = make(rng, dims, slots, rank, n)
+    net = sz.SimpleNeuralNet(*dims, init=params)
+    bank = sz.Adapters(net, slots, rank, init=flat)
+    bank.reserve(n, training=True)
+    c = host_controls(rng, 4, C, n)
+    handle, keep = dev_controls(c)
+    dx, ds, dl = dev(x), dev(pick_slots(rng, n, slots, "mixed")), dev(rng.integers(0, C, n).astype(np.int32))
+    logits, probs = torch.zeros(n, C, device="cuda"), torch.zeros(n, C, device="cuda")
+    from helpers import _DevView
+    grad = torch.as_tensor(_DevView(bank.grad_ptr(), bank.grad_len()), device="cuda")
+
+    def work(stream):
+        net.forward_adapted_dev(bank, dx.data_ptr(), ds.data_ptr(), n, logits_ptr=logits.data_ptr(), probs_ptr=probs.data_ptr(), controls=handle,
+                                stream=stream)
+        bank.zero_grad_dev(stream)
+        bank.accumulate_dev(net, dx.data_ptr(), dl.data_ptr(), ds.data_ptr(), n, controls=handle, stream=stream)
+        bank.clip_grad_dev(0.01, 0, stream)
+        bank.apply_grad_dev(0.1, stream)
+
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        work(torch.cuda.current_stream().cuda_stream)
+    for _ in range(4):
+        dx.copy_(torch.from_numpy(rng.standard_normal(x.shape).astype(np.float32)))
+        ds.copy_(torch.from_numpy(pick_slots(rng, n, slots, "mixed")))
+        start = [bank.get_params(k) for k in range(slots)]
+        work(0)
+        torch.cuda.synchronize()
+        want = [t.clone() for t in (logits, probs, grad)]
+        after = [bank.get_params(k) for k in range(slots)]
+        for k in range(slots):
+            bank.set_params(k, start[k])
+        for t in (logits, probs, grad):
+            t.fill_(-1.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((logits, probs, grad), want):
+            assert np.array_equal(a.cpu().numpy(), b.cpu().numpy(), equal_nan=True)
+        for k in range(slots):
+            assert all(np.array_equal(a, b) for a, b in zip(bank.get_params(k), after[k]))
