@@ -124,6 +124,8 @@ int check_pair(const Net* n, const Adapters* a)
     return SZH_OK;
 }
 
+bool overlap(const float* a, uint64_t a_len, const float* b, uint64_t b_len) { return a < b + b_len && b < a + a_len; }
+
 int group_rows(Adapters* a, const int32_t* slots_dev, uint32_t rows, hipStream_t s)
 {
     AdaptWorkspace& w = a->ws;
@@ -631,6 +633,12 @@ int adapters_forward(Net* n, Adapters* a, const float* x, const int32_t* slots_d
 {
     if (int rc = check_pair(n, a)) return rc;
     if (rows == 0 || n->out == 0) return SZH_OK;
+    const uint64_t results = rows * n->out, feats = rows * n->in;
+    if ((logits && probs && overlap(logits, results, probs, results)) || (logits && overlap(logits, results, x, feats)) ||
+        (probs && overlap(probs, results, x, feats))) {
+        set_error("logits, probabilities and features overlap");
+        return SZH_EINVAL;
+    }
     if (int rc = ensure(a, rows, false, s)) return rc;
     for (uint64_t r0 = 0; r0 < rows; r0 += kAdaptRows) {
         const uint32_t R = (uint32_t)std::min<uint64_t>(kAdaptRows, rows - r0);

@@ -1177,11 +1177,6 @@ int szh_clip_run_dev(szh_clip* clip, float max_norm, float* norms_dev, void* str
     return clip_run(c, max_norm, norms_dev, static_cast<hipStream_t>(stream));
 }
 
-static bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes)
-{
-    return (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
-}
-
 static int read_controls(const szh_logit_controls* c, Controls* out)
 {
     *out = Controls{};
@@ -1269,13 +1264,6 @@ int szh_net_forward_adapted_dev(szh_net* net, szh_adapters* bank, const float* f
     SZ_TRY
     if (!net || !bank || (n && (!feats_dev || !slots_dev))) { set_error("null argument"); return SZH_EINVAL; }
     if (n && !logits_dev && !probs_dev) { set_error("no result asked for"); return SZH_EINVAL; }
-    const Net* shape = reinterpret_cast<const Net*>(net);
-    const uint64_t results = n * shape->out * sizeof(float), feats = n * shape->in * sizeof(float);
-    if ((logits_dev && probs_dev && overlap(logits_dev, results, probs_dev, results)) || (logits_dev && overlap(logits_dev, results, feats_dev, feats)) ||
-        (probs_dev && overlap(probs_dev, results, feats_dev, feats))) {
-        set_error("logits, probabilities and features overlap");
-        return SZH_EINVAL;
-    }
     Controls c;
     if (int rc = read_controls(controls, &c)) return rc;
     if (int rc = check_device(reinterpret_cast<Net*>(net)->device)) return rc;
