@@ -236,7 +236,7 @@ int low_out(const Net* n, const Adapters* a, uint32_t rows, hipStream_t s)
     }
 }
 
-// the gradients of a pass's four factors, added to the bank's
+// the gradients of a pass's four factors, its losses and live rows, added to the bank's
 int factor_gradients(Adapters* a, uint32_t rows, hipStream_t s)
 {
     const AdaptWorkspace& w = a->ws;
@@ -266,7 +266,8 @@ int factor_gradients(Adapters* a, uint32_t rows, hipStream_t s)
     case 3: hipLaunchKernelGGL((factor_grad_kernel<3, 2>), grid, block, 0, s, g); break;
     default: hipLaunchKernelGGL((factor_grad_kernel<4, 2>), grid, block, 0, s, g); break;
     }
-    hipLaunchKernelGGL(factor_reduce_kernel, dim3(blocks, a->slots), block, 0, s, g, a->d_grad, a->per_slot());
+    hipLaunchKernelGGL(factor_reduce_kernel, dim3(blocks + 1, a->slots), block, 0, s, g, a->d_grad, a->per_slot(), w.loss, w.live, a->d_sums,
+                       a->d_grad + a->per_slot() * a->slots);
     SZ_HIP(hipGetLastError());
     return SZH_OK;
 }
@@ -708,9 +709,6 @@ int adapters_accumulate(Net* n, Adapters* a, const float* x, const int32_t* labe
         }
         rc = factor_gradients(a, R, s);
         if (rc) return rc;
-        hipLaunchKernelGGL(slot_stats_kernel, dim3(a->slots), dim3(256), 0, s, w.loss, w.live, w.begin, a->d_sums,
-                           a->d_grad + a->per_slot() * a->slots);
-        SZ_HIP(hipGetLastError());
     }
     return SZH_OK;
 }

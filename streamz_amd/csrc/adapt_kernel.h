@@ -1022,29 +1022,11 @@ __global__ __launch_bounds__(256) void factor_grad_kernel(FactorArgs a)
     }
 }
 
-// grad[slot] += the slot's chunks of the slabs; 64-bit sums, in chunk order
-__global__ __launch_bounds__(256) void factor_reduce_kernel(FactorArgs a, float* __restrict__ grad, uint64_t grad_slot)
-{
-    const int slot = blockIdx.y;
-    const uint32_t b = a.begin[slot], e = a.begin[slot + 1];
-    if (b == e) return;
-    const int which = ((int)blockIdx.x >= a.job[1].first_out) + ((int)blockIdx.x >= a.job[2].first_out) + ((int)blockIdx.x >= a.job[3].first_out);
-    const FactorJob g = a.job[which];
-    const int i = ((int)blockIdx.x - g.first_out) * 256 + threadIdx.x;
-    if (i >= g.M * a.rank) return;
-    const uint32_t c0 = b / a.chunk, c1 = (e - 1) / a.chunk;
-    double t = 0.0;
-    for (uint32_t c = c0; c <= c1; ++c) t += (double)g.slab[(size_t)(c + slot) * g.M * a.rank + i];
-    grad[(size_t)slot * grad_slot + g.off + (size_t)(i / a.rank) * g.g_m + (size_t)(i % a.rank) * g.g_j] += (float)t;
-}
-
 // sums[slot] += {loss, live rows} of the slot's rows (64 bits, fixed order); tail = the same as floats
-__global__ __launch_bounds__(256) void slot_stats_kernel(const float* __restrict__ loss, const uint8_t* __restrict__ live,
-                                                         const uint32_t* __restrict__ begin, double* __restrict__ sums,
-                                                         float* __restrict__ tail)
+__device__ __forceinline__ void slot_stats(int slot, const float* __restrict__ loss, const uint8_t* __restrict__ live,
+                                           const uint32_t* __restrict__ begin, double* __restrict__ sums, float* __restrict__ tail)
 {
     __shared__ double sl[256], sc[256];
-    const int slot = blockIdx.x;
     double l = 0.0, c = 0.0;
     // (eight rows a thread in flight; those behind the last as zeros)
     const uint32_t end = begin[slot + 1];
@@ -1067,6 +1049,33 @@ __global__ __launch_bounds__(256) void slot_stats_kernel(const float* __restrict
         sums[2 * slot] = a; sums[2 * slot + 1] = b;
         tail[2 * slot] = (float)a; tail[2 * slot + 1] = (float)b;
     }
+}
+
+// grad[slot] += the slot's chunks of the slabs (64-bit sums, in chunk order); the last workgroup of a slot adds up its rows
+__global__ __launch_bounds__(256) void factor_reduce_kernel(FactorArgs a, float* __restrict__ grad, uint64_t grad_slot, const float* __restrict__ loss,
+                                                            const uint8_t* __restrict__ live, double* __restrict__ sums, float* __restrict__ tail)
+{
+    const int slot = blockIdx.y;
+    if (blockIdx.x == gridDim.x - 1) { slot_stats(slot, loss, live, a.begin, sums, tail); return; }
+    const uint32_t b = a.begin[slot], e = a.begin[slot + 1];
+    if (b == e) return;
+    const int which = ((int)blockIdx.x >= a.job[1].first_out) + ((int)blockIdx.x >= a.job[2].first_out) + ((int)blockIdx.x >= a.job[3].first_out);
+    const FactorJob g = a.job[which];
+    const int i = ((int)blockIdx.x - g.first_out) * 256 + threadIdx.x;
+    if (i >= g.M * a.rank) return;
+    const uint32_t c0 = b / a.chunk, c1 = (e - 1) / a.chunk;
+    float* out = grad + (size_t)slot * grad_slot + g.off + (size_t)(i / a.rank) * g.g_m + (size_t)(i % a.rank) * g.g_j;
+    const float before = *out;
+    double t = 0.0;
+    for (uint32_t c = c0; c <= c1; c += 8) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = g.slab[(size_t)(min(c + k, c1) + slot) * g.M * a.rank + i];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t += (double)keep_if(c + k <= c1, v[k]);
+    }
+    *out = before + (float)t;
 }
 
 // params -= (lr / live) * grad for every slot with live rows (lib.rs:1047-1059, a slot at a time)
