@@ -289,13 +289,13 @@ bool back_fours(const Adapters* a, const BackArgs& g)
 
 // The output layer, the loss and back to d2 and the rank columns in one launch, lg taking d3
 bool tail_applies(const Adapters* a) { return a->out <= 64 && a->rank <= 16; }
-template <int OT>
+template <int OT, int WAVES>
 int launch_tail(const BackArgs& g, bool fours, const TailArgs& o, const Controls& ctl, const ControlRun& c, hipStream_t s)
 {
-    const dim3 grid((g.rows + 31) / 32), block(256);
+    const dim3 grid((g.rows + 31) / 32), block(64 * WAVES);
     ProfScope prof("adapt_tail", s);
-    if (fours) hipLaunchKernelGGL((tail_kernel<OT, true>), grid, block, 0, s, g, o, ctl, c);
-    else hipLaunchKernelGGL((tail_kernel<OT, false>), grid, block, 0, s, g, o, ctl, c);
+    if (fours) hipLaunchKernelGGL((tail_kernel<OT, WAVES, true>), grid, block, 0, s, g, o, ctl, c);
+    else hipLaunchKernelGGL((tail_kernel<OT, WAVES, false>), grid, block, 0, s, g, o, ctl, c);
     SZ_HIP(hipGetLastError());
     return SZH_OK;
 }
@@ -304,9 +304,11 @@ int tail_rows(const Net* n, const Adapters* a, const Controls& ctl, const Contro
     const BackArgs g = back_args(n, a, rows);
     const TailArgs o{n->d_params + n->off_b3(), a->ws.u3, a->ws.lg};
     const bool fours = back_fours(a, g);
-    if (n->out <= 16) return launch_tail<1>(g, fours, o, ctl, c, s);
-    if (n->out <= 32) return launch_tail<2>(g, fours, o, ctl, c, s);
-    return launch_tail<4>(g, fours, o, ctl, c, s);
+    // (a compute unit has at most one workgroup then: eight waves share its tiles; 550 rows 17 us by four, 13 by eight)
+    const bool few = rows <= 32u * (unsigned)compute_units();
+    if (n->out <= 16) return few ? launch_tail<1, 8>(g, fours, o, ctl, c, s) : launch_tail<1, 4>(g, fours, o, ctl, c, s);
+    if (n->out <= 32) return few ? launch_tail<2, 8>(g, fours, o, ctl, c, s) : launch_tail<2, 4>(g, fours, o, ctl, c, s);
+    return launch_tail<4, 4>(g, fours, o, ctl, c, s);
 }
 
 // d3 -> g3, d2, g2 in one launch; up to 64 classes (beyond them the product with w3 wants larger tiles)

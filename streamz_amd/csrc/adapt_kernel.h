@@ -442,6 +442,9 @@ struct LowArgs {
 // 16 k are requested at once: with as many rows as there are, what a wave does is wait.  NT tiles of 16
 // columns: OT of the output layer, then the rank's.  A column beyond the matrix takes another's values and is dropped.
 // FOURS (OT = 0): f_k is 1 and the factor's columns are 16-byte aligned, in fours.
+// Bound by memory: 66140 x 512 with rank 16 29 us (4.7 TB/s) on four waves and four blocks, 39 on eight waves; 26456 x 2048
+// with rank 32 57 us on two blocks (3.8 TB/s), 70 on eight waves, 130 on four blocks (their registers leave too few waves);
+// logits of 16 classes and 16 rank columns of 66140 x 256 in 27 us, 38 with the loads where the compiler puts them.
 template <int NT, int OT, int WAVES, int UNR, bool FOURS>
 __global__ __launch_bounds__(64 * WAVES) void low_kernel(LowArgs a)
 {
@@ -595,7 +598,8 @@ __global__ __launch_bounds__(64 * WAVES) void low_kernel(LowArgs a)
 // and d2, g2, g3 written once.  Everything is computed transposed (rows of the batch along the matrix instruction's
 // columns): a result's four registers then are four neighbouring units of one row, which is what the next product's
 // operand and 16-byte loads and stores want.  The waves deal the hidden units among themselves; g2, a sum over all
-// of them, is joined in LDS.  Bound by memory: at 66140 x 256 x 16 it moves 140 MB.
+// of them, is joined in LDS.  66140 x 256 x 16 with rank 16: 43 us for 140 MB (79 with the factors read value by value, 90
+// and 114 on one wave with 32 and 16 rows).
 struct BackArgs {
     const float *d3, *h2, *w3;        // [rows][ld3], [rows][ld2], [n2][out]
     const float *a3, *b3, *b2;        // slot 0's factors [n2][rank], [rank][out], [rank][n2]
@@ -777,15 +781,17 @@ __global__ __launch_bounds__(64 * WAVES) void back_kernel(BackArgs a)
 
 // The output layer and back in one launch, for up to 16 rank columns and 64 classes (OT tiles of 16): u3, the logits,
 // controls and softmax, the loss, d3, and what back_kernel makes of it.  A workgroup has 32 rows; their logits and
-// d3 stay in LDS, and what of h2 the second half reads is still in the cache.
+// d3 stay in LDS, and what of h2 the second half reads is still in the cache.  66140 x 256 x 16 with rank 16: 68 us (28, 9 and
+// 43 for low_kernel, the controls and back_kernel), 19 of them matrix and 26 vector instructions, which take turns on a SIMD
+// unit, for 150 MB; more waves a unit do not help (71 us at five, 95 at six: registers).
 struct TailArgs {
     const float* bias;
     float *u3, *d3;   // [rows][ldu], [rows][ld3]
 };
-template <int OT, bool FOURS>
-__global__ __launch_bounds__(256) void tail_kernel(BackArgs a, TailArgs o, Controls ctl, ControlRun run)
+template <int OT, int WAVES, bool FOURS>
+__global__ __launch_bounds__(64 * WAVES) void tail_kernel(BackArgs a, TailArgs o, Controls ctl, ControlRun run)
 {
-    constexpr int WAVES = 4, T = 2, LD = 16 * OT + 4;
+    constexpr int T = 2, LD = 16 * OT + 4, PER = 64 * WAVES / (16 * T);  // PER lanes have a row of the softmax
     __shared__ __attribute__((aligned(16))) float sums[WAVES][T][(OT + 1) * 16][17];  // classes, then rank columns
     __shared__ __attribute__((aligned(16))) float z[16 * T][LD];                       // logits, then d3
     __shared__ float us[16 * T][17];
@@ -882,8 +888,7 @@ __global__ __launch_bounds__(256) void tail_kernel(BackArgs a, TailArgs o, Contr
         if (j < a.ldu && row0 + r < a.rows) o.u3[(size_t)(row0 + r) * a.ldu + j] = s;
     }
     __syncthreads();
-    // eight lanes have a row from here on, each every eighth class
-    const int r = threadIdx.x >> 3, l = threadIdx.x & 7;
+    const int r = threadIdx.x / PER, l = threadIdx.x % PER;
     const uint32_t i = min(row0 + r, a.rows - 1);
     const bool real = row0 + r < a.rows;
     const int slot = a.row_slot[i];
@@ -891,7 +896,7 @@ __global__ __launch_bounds__(256) void tail_kernel(BackArgs a, TailArgs o, Contr
     const uint64_t row = run.order ? run.order[i] : i;
     const control::RowControl rc = control::row_control(ctl, a.out, control::row_set(ctl, row));
     float top = -INFINITY;
-    for (int c = l; c < a.out; c += 8) {
+    for (int c = l; c < a.out; c += PER) {
         float b[16], v = 0.0f, low = 0.0f;
 #pragma unroll
         for (int j = 0; j < 16; ++j) b[j] = b3[(size_t)min(j, a.rank - 1) * a.out + c];
@@ -905,19 +910,19 @@ __global__ __launch_bounds__(256) void tail_kernel(BackArgs a, TailArgs o, Contr
         z[r][c] = v;
         top = fmaxf(top, v);
     }
-    top = control::lanes_max<8>(top);
+    top = control::lanes_max<PER>(top);
     const float shift = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
-    for (int c = l; c < a.out; c += 8) {
+    for (int c = l; c < a.out; c += PER) {
         const float e = control::exp_low(z[r][c] - shift);
         z[r][c] = e;
         sum += e;
     }
-    sum = control::lanes_sum<8>(sum);
+    sum = control::lanes_sum<PER>(sum);
     const bool some = !(sum <= 0.0f);  // (a NaN row stays one)
     const float inv = some ? 1.0f / sum : 0.0f;
     const control::TrainRow tr = control::train_row(run, rc, i, row, a.out, some);
-    for (int c = l; c < LD; c += 8) {
+    for (int c = l; c < LD; c += PER) {
         float v = 0.0f;
         if (c < a.out && tr.live) {
             const float p = z[r][c] * inv;
@@ -959,7 +964,9 @@ struct FactorArgs {
 };
 
 // 64 columns of p per workgroup; its four waves take rows in turn and are joined in LDS.  A lane reads 16
-// bytes of a row of p for four matrix instructions: step t's columns are 4 c + t.
+// bytes of a row of p for four matrix instructions: step t's columns are 4 c + t.  G groups of four rows are asked for at
+// once: 13228 rows of the wide network with rank 32 89 us by four groups, 111 by two; 66140 rows of the small one 54 us for
+// 280 MB either way.
 template <int NT, int G>
 __global__ __launch_bounds__(256) void factor_grad_kernel(FactorArgs a)
 {
