@@ -52,12 +52,13 @@ bool capturing(hipStream_t s)
 }
 
 // Rows per chunk of the factor gradients: enough workgroups (tiles x chunks) to fill the chip twice, no more than 512
-// rows (the sums of a chunk's rows are joined by a second launch), no less than 64.
+// rows (the sums of a chunk's rows are joined by a second launch), no less than 64, or 16 of few rows, whose chunks would hold
+// many slots one behind the other (106 rows of 27 slots: 31 us by 16, 41 by 32, 63 by 64; 550 rows of one: 12.4, 10.9, 10.4).
 int factor_tiles(const Adapters* a) { return (int)((a->h1 + 63) / 64 + 2 * ((a->h2 + 63) / 64) + (a->out + 63) / 64); }
 uint32_t factor_chunk(const Adapters* a, uint64_t rows)
 {
-    const uint64_t want = std::max<uint64_t>(1, 1024 / factor_tiles(a));
-    return (uint32_t)std::min<uint64_t>(512, std::max<uint64_t>(64, (rows / want + 63) / 64 * 64));
+    const uint64_t want = std::max<uint64_t>(1, 1024 / factor_tiles(a)), least = rows <= kFewRows ? 16 : 64;
+    return (uint32_t)std::min<uint64_t>(512, std::max<uint64_t>(least, (rows / want + least - 1) / least * least));
 }
 // most chunks that a call of up to `rows` rows makes
 uint64_t factor_chunks_most(const Adapters* a, uint64_t rows) { return std::max<uint64_t>(rows / 512, 1024 / factor_tiles(a)) + 2; }
@@ -289,13 +290,13 @@ bool back_fours(const Adapters* a, const BackArgs& g)
 
 // The output layer, the loss and back to d2 and the rank columns in one launch, lg taking d3
 bool tail_applies(const Adapters* a) { return a->out <= 64 && a->rank <= 16; }
-template <int OT, int WAVES>
+template <int OT, int WAVES, int T>
 int launch_tail(const BackArgs& g, bool fours, const TailArgs& o, const Controls& ctl, const ControlRun& c, hipStream_t s)
 {
-    const dim3 grid((g.rows + 31) / 32), block(64 * WAVES);
+    const dim3 grid((g.rows + 16 * T - 1) / (16 * T)), block(64 * WAVES);
     ProfScope prof("adapt_tail", s);
-    if (fours) hipLaunchKernelGGL((tail_kernel<OT, WAVES, true>), grid, block, 0, s, g, o, ctl, c);
-    else hipLaunchKernelGGL((tail_kernel<OT, WAVES, false>), grid, block, 0, s, g, o, ctl, c);
+    if (fours) hipLaunchKernelGGL((tail_kernel<OT, WAVES, T, true>), grid, block, 0, s, g, o, ctl, c);
+    else hipLaunchKernelGGL((tail_kernel<OT, WAVES, T, false>), grid, block, 0, s, g, o, ctl, c);
     SZ_HIP(hipGetLastError());
     return SZH_OK;
 }
@@ -304,11 +305,17 @@ int tail_rows(const Net* n, const Adapters* a, const Controls& ctl, const Contro
     const BackArgs g = back_args(n, a, rows);
     const TailArgs o{n->d_params + n->off_b3(), a->ws.u3, a->ws.lg};
     const bool fours = back_fours(a, g);
-    // (a compute unit has at most one workgroup then: eight waves share its tiles; 550 rows 17 us by four, 13 by eight)
-    const bool few = rows <= 32u * (unsigned)compute_units();
-    if (n->out <= 16) return few ? launch_tail<1, 8>(g, fours, o, ctl, c, s) : launch_tail<1, 4>(g, fours, o, ctl, c, s);
-    if (n->out <= 32) return few ? launch_tail<2, 8>(g, fours, o, ctl, c, s) : launch_tail<2, 4>(g, fours, o, ctl, c, s);
-    return launch_tail<4, 4>(g, fours, o, ctl, c, s);
+    // (as long as a compute unit has at most one workgroup: fewer rows and more waves for them.  1056 rows x 2048 units 49 us, 68 on
+    // 32 rows and eight waves; 550 x 256 12.8, 13.6, and 17 on four waves)
+    const unsigned cus = (unsigned)compute_units();
+    if (rows <= 16 * cus) {
+        if (n->out <= 16) return launch_tail<1, 16, 1>(g, fours, o, ctl, c, s);
+        if (n->out <= 32) return launch_tail<2, 16, 1>(g, fours, o, ctl, c, s);
+        return launch_tail<4, 8, 1>(g, fours, o, ctl, c, s);
+    }
+    if (n->out <= 16) return rows <= 32 * cus ? launch_tail<1, 8, 2>(g, fours, o, ctl, c, s) : launch_tail<1, 4, 2>(g, fours, o, ctl, c, s);
+    if (n->out <= 32) return rows <= 32 * cus ? launch_tail<2, 8, 2>(g, fours, o, ctl, c, s) : launch_tail<2, 4, 2>(g, fours, o, ctl, c, s);
+    return launch_tail<4, 4, 2>(g, fours, o, ctl, c, s);
 }
 
 // d3 -> g3, d2, g2 in one launch; up to 64 classes (beyond them the product with w3 wants larger tiles)
@@ -317,8 +324,23 @@ int back_rows(const Net* n, const Adapters* a, uint32_t rows, hipStream_t s)
 {
     const BackArgs g = back_args(n, a, rows);
     const bool fours = back_fours(a, g);
-    const dim3 grid((rows + 31) / 32);
     ProfScope prof("adapt_back", s);
+    if (rows <= 16u * (unsigned)compute_units()) {  // (fewer tiles than compute units: half the rows, and eight waves for them)
+        const dim3 grid((rows + 15) / 16), block(512);
+        switch ((a->rank + 15) / 16 * 2 + fours) {
+        case 2: hipLaunchKernelGGL((back_kernel<1, 8, 1, false>), grid, block, 0, s, g); break;
+        case 3: hipLaunchKernelGGL((back_kernel<1, 8, 1, true>), grid, block, 0, s, g); break;
+        case 4: hipLaunchKernelGGL((back_kernel<2, 8, 1, false>), grid, block, 0, s, g); break;
+        case 5: hipLaunchKernelGGL((back_kernel<2, 8, 1, true>), grid, block, 0, s, g); break;
+        case 6: hipLaunchKernelGGL((back_kernel<3, 8, 1, false>), grid, block, 0, s, g); break;
+        case 7: hipLaunchKernelGGL((back_kernel<3, 8, 1, true>), grid, block, 0, s, g); break;
+        case 8: hipLaunchKernelGGL((back_kernel<4, 8, 1, false>), grid, block, 0, s, g); break;
+        default: hipLaunchKernelGGL((back_kernel<4, 8, 1, true>), grid, block, 0, s, g); break;
+        }
+        SZ_HIP(hipGetLastError());
+        return SZH_OK;
+    }
+    const dim3 grid((rows + 31) / 32);
     switch ((a->rank + 15) / 16 * 2 + fours) {
     case 2: hipLaunchKernelGGL((back_kernel<1, 4, 2, false>), grid, dim3(256), 0, s, g); break;
     case 3: hipLaunchKernelGGL((back_kernel<1, 4, 2, true>), grid, dim3(256), 0, s, g); break;

@@ -780,7 +780,7 @@ __global__ __launch_bounds__(64 * WAVES) void back_kernel(BackArgs a)
 }
 
 // The output layer and back in one launch, for up to 16 rank columns and 64 classes (OT tiles of 16): u3, the logits,
-// controls and softmax, the loss, d3, and what back_kernel makes of it.  A workgroup has 32 rows; their logits and
+// controls and softmax, the loss, d3, and what back_kernel makes of it.  A workgroup has 16 T rows; their logits and
 // d3 stay in LDS, and what of h2 the second half reads is still in the cache.  66140 x 256 x 16 with rank 16: 68 us (28, 9 and
 // 43 for low_kernel, the controls and back_kernel), 19 of them matrix and 26 vector instructions, which take turns on a SIMD
 // unit, for 150 MB; more waves a unit do not help (71 us at five, 95 at six: registers).
@@ -788,19 +788,19 @@ struct TailArgs {
     const float* bias;
     float *u3, *d3;   // [rows][ldu], [rows][ld3]
 };
-template <int OT, int WAVES, bool FOURS>
+template <int OT, int WAVES, int T, bool FOURS>
 __global__ __launch_bounds__(64 * WAVES) void tail_kernel(BackArgs a, TailArgs o, Controls ctl, ControlRun run)
 {
-    constexpr int T = 2, LD = 16 * OT + 4, PER = 64 * WAVES / (16 * T);  // PER lanes have a row of the softmax
+    constexpr int LD = 16 * OT + 4, PER = 64 * WAVES / (16 * T);  // PER lanes have a row of the softmax
     __shared__ __attribute__((aligned(16))) float sums[WAVES][T][(OT + 1) * 16][17];  // classes, then rank columns
     __shared__ __attribute__((aligned(16))) float z[16 * T][LD];                       // logits, then d3
     __shared__ float us[16 * T][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int r16 = lane & 15, q = lane >> 4;
     const uint32_t row0 = blockIdx.x * (16 * T);
-    const uint32_t my_row = row0 + (lane & 31);
+    const uint32_t my_row = row0 + (lane & (16 * T - 1));
     const int mine = my_row < a.rows ? a.row_slot[my_row] : -1;
-    const uint32_t adapted = (uint32_t)__ballot(mine >= 0);
+    const uint32_t adapted = (uint32_t)__ballot(mine >= 0) & (T == 2 ? 0xffffffffu : 0xffffu);
     {
         size_t row[T];
 #pragma unroll

@@ -4,6 +4,9 @@
 // With few rows the matrices are what is read, and nearly nothing is computed: a row's workgroup streams the small
 // matrices (w1, the slot's factors, w3) straight from the caches into vector products with its activations in LDS,
 // and the large one, w2, is cut over columns and k so that many compute units read a part each.
+// One row of 60-512-256-16: 20.8 us for the three launches (365 as tensor operations), most of it a compute unit's first reading
+// of matrices and code (about 3000 cycles for a matrix it has not seen); one launch for all three took 24 to 35 us, because a
+// single compute unit then reads w2 as well.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -19,6 +22,14 @@ constexpr int kRowT = 1024, kRowWaves = kRowT / 64;
 // LDS floats of the partial sums: four columns per thread
 constexpr int kRowPart = 4 * kRowT;
 
+// four values from any multiple of four bytes: one load
+__device__ __forceinline__ float4 any_four(const float* p)
+{
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    const f32x4u v = *reinterpret_cast<const f32x4u*>(p);
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+
 // out(n, sum_k x[k] W[k][n] + sum_j u[j] B[j][n]) for n < N, by the whole workgroup; x and u in LDS, W [K][N] and B [J][N]
 // in memory (J may be 0).  A thread takes four neighbouring columns and every ks-th k; partial sums meet by lane
 // exchanges (narrow matrices) and in LDS.  Ends with a barrier; `out` is called by one thread per column.
@@ -27,13 +38,14 @@ __device__ __forceinline__ void row_product(const float* x, int K, const float* 
                                             const float* __restrict__ B, int N, float* part, F out)
 {
     const int t = threadIdx.x;
-    const bool vec = (N & 3) == 0 && ((((uintptr_t)W) | (J ? (uintptr_t)B : 0)) & 15) == 0;
+    const bool vec = N >= 4;
     for (int n0 = 0; n0 < N; n0 += kRowPart) {
         const int cols = min(N - n0, kRowPart), groups = (cols + 3) >> 2;
         int lg = 0;
         while ((1 << lg) < groups) ++lg;  // groups of four columns, rounded up to a power of two
         const int gp = 1 << lg, slices = kRowT >> lg;
         const int c = n0 + 4 * (t & (gp - 1)), ks = t >> lg;
+        const int at = vec ? min(c, N - 4) : c;  // (the last group reads the last four columns; rows may start anywhere)
         float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
         auto run = [&](const float* v, int n_k, const float* __restrict__ M) {
             if (c >= N) return;
@@ -42,7 +54,7 @@ __device__ __forceinline__ void row_product(const float* x, int K, const float* 
                 for (; k + 7 * slices < n_k; k += 8 * slices) {
                     float4 w[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const float4*>(M + (size_t)(k + i * slices) * N + c);
+                    for (int i = 0; i < 8; ++i) w[i] = any_four(M + (size_t)(k + i * slices) * N + at);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float xv = v[k + i * slices];
@@ -57,7 +69,7 @@ __device__ __forceinline__ void row_product(const float* x, int K, const float* 
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int kk = min(k + i * slices, n_k - 1);
-                        w[i] = *reinterpret_cast<const float4*>(M + (size_t)kk * N + c);
+                        w[i] = any_four(M + (size_t)kk * N + at);
                         xv[i] = v[kk];
                     }
 #pragma unroll
@@ -80,6 +92,9 @@ __device__ __forceinline__ void row_product(const float* x, int K, const float* 
         };
         run(x, K, W);
         if (J) run(u, J, B);
+        if (c - at == 1) { a0 = a1; a1 = a2; a2 = a3; }
+        else if (c - at == 2) { a0 = a2; a1 = a3; }
+        else if (c - at == 3) a0 = a3;
         // the k slices of a wave
         for (int o = gp; o < 64; o <<= 1) {
             a0 += __shfl_xor(a0, o); a1 += __shfl_xor(a1, o); a2 += __shfl_xor(a2, o); a3 += __shfl_xor(a3, o);
