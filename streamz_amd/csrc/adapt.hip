@@ -381,33 +381,35 @@ int thin_product(const float* A, int lda, int K, const float* W, const float* ad
 //   256-row tiles: 0.232 K + 18 for every round of one tile per compute unit
 //   128-row tiles: two per unit 0.122 K + 17, one 0.071 K + 12        64-row tiles: 0.0337 K + 4 each, once 0.0085 K
 //   32 x 32 thin tiles: 5 + 0.001 K, and 3.55e-5 K each
-struct ProductPlan { uint32_t wide_rows; int rest; };  // rest: 0 thin, 64, 128
-double rest_time(uint32_t rows, int N, int K, double cus, int* how)
+struct ProductPart { int how; uint32_t rows; };   // how: 256, 128 or 64 rows a tile, 0 thin
+struct ProductPlan { ProductPart part[3]; int parts; double time; };
+
+double part_time(int how, uint32_t rows, int N, int K, double cus)
 {
     auto ceil_div = [](uint64_t a, uint64_t b) { return (double)((a + b - 1) / b); };
-    const double t32 = ceil_div(rows, 32) * ceil_div(N, 32);
-    const double c64 = std::ceil(ceil_div(rows, 64) * ceil_div(N, 128) / cus), c128 = std::ceil(ceil_div(rows, 128) * ceil_div(N, 128) / cus);
-    const double thin = 5 + 0.001 * K + t32 * 3.55e-5 * K;
-    const double g64 = c64 * (0.0337 * K + 4) + 0.0085 * K;
-    const double g128 = std::floor(c128 / 2) * (0.122 * K + 17) + (std::fmod(c128, 2.0) != 0 ? 0.071 * K + 12 : 0);
-    *how = thin <= g64 && thin <= g128 ? 0 : g64 <= g128 ? 64 : 128;
-    return std::min(thin, std::min(g64, g128));
+    if (how == 0) return 5 + 0.001 * K + ceil_div(rows, 32) * ceil_div(N, 32) * 3.55e-5 * K;
+    if (how == 256) return std::ceil(ceil_div(rows, 256) * ceil_div(N, 256) / cus) * (0.232 * K + 18) + 6;  // (W transposed first: a launch)
+    const double c = std::ceil(ceil_div(rows, how) * ceil_div(N, 128) / cus);
+    if (how == 64) return c * (0.0337 * K + 4) + 0.0085 * K;
+    return std::floor(c / 2) * (0.122 * K + 17) + (std::fmod(c, 2.0) != 0 ? 0.071 * K + 12 : 0);
 }
-ProductPlan plan_product(uint32_t rows, int N, int K)
+// The quickest of: one kernel for all rows, or whole rounds of tiles of `most` rows or fewer first and the rest the same way
+// (1056 x 2048 x 2048: 178 us on 64-row tiles alone, whose second round is one row of tiles, 115 with that left to thin ones).
+ProductPlan plan_rows(uint32_t rows, int N, int K, double cus, int most)
 {
-    const double cus = compute_units();
-    ProductPlan best{0, 64};
-    double time = rest_time(rows, N, K, cus, &best.rest);
-    const uint32_t across = (N + 255) / 256, down = (rows + 255) / 256;
-    const uint32_t rounds = (uint32_t)((uint64_t)across * down / (uint64_t)cus);
-    // whole rounds of wide tiles (and one more, partly filled); the transposed weights cost a launch
-    for (uint32_t q = rounds ? rounds : 1; q <= rounds + 1; ++q) {
-        const uint32_t m = (uint32_t)std::min<uint64_t>((uint64_t)q * (uint64_t)cus / across, down);
-        if (m == 0) continue;
-        ProductPlan p{std::min(rows, m * 256), 64};
-        double t = std::ceil((double)m * across / cus) * (0.232 * K + 18) + 6;
-        if (p.wide_rows < rows) t += rest_time(rows - p.wide_rows, N, K, cus, &p.rest) + 2;
-        if (t < time) { time = t; best = p; }
+    ProductPlan best{{{0, rows}}, 1, part_time(0, rows, N, K, cus)};
+    for (const int how : {64, 128, 256}) {
+        if (how > most) continue;
+        const double all = part_time(how, rows, N, K, cus);
+        if (all < best.time) best = {{{how, rows}}, 1, all};
+        const uint64_t across = ((uint64_t)N + (how == 256 ? 255 : 127)) / (how == 256 ? 256 : 128), down = ((uint64_t)rows + how - 1) / how;
+        const uint64_t first = (uint64_t)(across * down / (uint64_t)cus) * (uint64_t)cus / across * how;  // rows of the whole rounds
+        if (first == 0 || first >= rows) continue;
+        const ProductPlan rest = plan_rows(rows - (uint32_t)first, N, K, cus, how == 256 ? 128 : 0);
+        const double time = part_time(how, (uint32_t)first, N, K, cus) + rest.time + 2;
+        if (time >= best.time) continue;
+        best = {{{how, (uint32_t)first}}, 1 + rest.parts, time};
+        for (int i = 0; i < rest.parts; ++i) best.part[1 + i] = rest.part[i];
     }
     return best;
 }
@@ -417,29 +419,36 @@ ProductPlan plan_product(uint32_t rows, int N, int K)
 template <int EPI, int TAG>
 int shared_product(const GemmArgs& g, int Kp, float* wt, hipStream_t s)
 {
-    const ProductPlan p = plan_product((uint32_t)g.M, g.N, g.K);
-    if (p.wide_rows) {
-        {
-            ProfScope prof("w2t", s);
-            hipLaunchKernelGGL(pad_transpose_kernel, dim3((unsigned)(((uint64_t)g.N * Kp + 255) / 256)), dim3(256), 0, s, g.B, g.K, g.N, Kp, wt);
+    const ProductPlan p = plan_rows((uint32_t)g.M, g.N, g.K, compute_units(), 256);
+    GemmArgs h = g;
+    for (int i = 0; i < p.parts; ++i) {
+        h.M = (int)p.part[i].rows;
+        int rc = SZH_OK;
+        if (p.part[i].how == 256) {
+            {
+                ProfScope prof("w2t", s);
+                hipLaunchKernelGGL(pad_transpose_kernel, dim3((unsigned)(((uint64_t)g.N * Kp + 255) / 256)), dim3(256), 0, s, g.B, g.K, g.N, Kp, wt);
+                SZ_HIP(hipGetLastError());
+            }
+            GemmArgs w = h;
+            w.B = wt; w.ldb = Kp; w.K = w.k_chunk = Kp;
+            rc = launch_gemm_f32w<EPI, TAG>(w, s);
+        } else if (p.part[i].how == 64) {
+            rc = launch_gemm_rows<A_ROWS, B_KROWS, EPI, TAG, 64>(h, s);
+        } else if (p.part[i].how == 128) {
+            rc = launch_gemm_rows<A_ROWS, B_KROWS, EPI, TAG, 128>(h, s);
+        } else {
+            ThinArgs t{};
+            t.A = h.A; t.lda = h.lda; t.W = h.B; t.bias = h.bias; t.C = h.C; t.ldc = h.ldc; t.M = h.M; t.N = h.N; t.K = h.K;
+            t.low = h.low; t.up = h.up; t.row_slot = h.row_slot; t.up_slot = h.up_slot; t.ld_low = h.ld_low; t.rank = h.rank;
+            ProfScope prof(kGemmTagName[TAG], s);
+            hipLaunchKernelGGL((thin_kernel<EPI == EPI_ADAPT_TANH>), dim3((t.N + 31) / 32, (t.M + 31) / 32), dim3(64 * kThinWaves), 0, s, t);
             SZ_HIP(hipGetLastError());
         }
-        GemmArgs h = g;
-        h.M = (int)p.wide_rows; h.B = wt; h.ldb = Kp; h.K = h.k_chunk = Kp;
-        if (int rc = launch_gemm_f32w<EPI, TAG>(h, s)) return rc;
-        if ((int)p.wide_rows == g.M) return SZH_OK;
+        if (rc) return rc;
+        const uint32_t m = p.part[i].rows;
+        h.A += (size_t)m * g.lda; h.C += (size_t)m * g.ldc; h.low += (size_t)m * g.ld_low; h.row_slot += m;
     }
-    GemmArgs h = g;
-    h.M -= (int)p.wide_rows;
-    h.A += (size_t)p.wide_rows * g.lda; h.C += (size_t)p.wide_rows * g.ldc; h.low += (size_t)p.wide_rows * g.ld_low; h.row_slot += p.wide_rows;
-    if (p.rest == 64) return launch_gemm_rows<A_ROWS, B_KROWS, EPI, TAG, 64>(h, s);
-    if (p.rest == 128) return launch_gemm_rows<A_ROWS, B_KROWS, EPI, TAG, 128>(h, s);
-    ThinArgs t{};
-    t.A = h.A; t.lda = h.lda; t.W = h.B; t.bias = h.bias; t.C = h.C; t.ldc = h.ldc; t.M = h.M; t.N = h.N; t.K = h.K;
-    t.low = h.low; t.up = h.up; t.row_slot = h.row_slot; t.up_slot = h.up_slot; t.ld_low = h.ld_low; t.rank = h.rank;
-    ProfScope prof(kGemmTagName[TAG], s);
-    hipLaunchKernelGGL((thin_kernel<EPI == EPI_ADAPT_TANH>), dim3((t.N + 31) / 32, (t.M + 31) / 32), dim3(64 * kThinWaves), 0, s, t);
-    SZ_HIP(hipGetLastError());
     return SZH_OK;
 }
 

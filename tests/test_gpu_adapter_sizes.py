@@ -47,6 +47,13 @@ BORDERS = [
     ((60, 256, 2048, 3), 7, 40, 8197, "runs"),
     ((60, 256, 2048, 3), 7, 16, 8192, "mixed"),
     ((60, 256, 2048, 3), 7, 16, 7990, "runs"),
+    # ... of whole rounds of other tiles, and of both
+    ((60, 1024, 2048, 4), 6, 16, 1056, "mixed"),
+    ((60, 512, 2048, 3), 5, 8, 9248, "runs"),
+    # few rows of many slots, chunk by chunk
+    ((60, 70, 50, 20), 90, 5, 130, "mixed"),
+    ((60, 70, 50, 21), 400, 19, 250, "mixed"),
+    ((60, 30, 3, 2), 5, 2, 90, "mixed"),
 ]
 
 
