@@ -21,10 +21,23 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // rows, is the same on every call.
 constexpr int kGroupRows = 512;
 
-__device__ __forceinline__ int group_key(const int32_t* slot, uint64_t r, int slots)
+// f(row, whether it is one of the rows, its key) for the rows r0 .. r1 - 1, 64 at a time, by one wave; the slots of 512 rows are
+// asked for at once
+template <class F>
+__device__ __forceinline__ void each_key(const int32_t* __restrict__ slot, uint32_t r0, uint32_t r1, int slots, F f)
 {
-    const int s = slot ? slot[r] : -1;
-    return s >= 0 && s < slots ? s : slots;
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint32_t r = r0; r < r1; r += 512) {
+        int32_t s[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s[i] = slot[min(r + 64 * i + lane, r1 - 1)];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (r + 64 * i >= r1) break;
+            f(r + 64 * i + lane, r + 64 * i + lane < r1, s[i] >= 0 && s[i] < slots ? s[i] : slots);
+        }
+    }
 }
 
 // count[key][block] of a block of rows
@@ -35,7 +48,7 @@ __global__ __launch_bounds__(64) void group_count_kernel(const int32_t* __restri
     for (int k = threadIdx.x; k <= slots; k += 64) hist[k] = 0;
     __syncthreads();
     const uint32_t r0 = blockIdx.x * kGroupRows, r1 = min(rows, r0 + kGroupRows);
-    for (uint32_t r = r0 + threadIdx.x; r < r1; r += 64) atomicAdd(&hist[group_key(slot, r, slots)], 1u);  // (integers: any order)
+    each_key(slot, r0, r1, slots, [&](uint32_t, bool in, int key) { if (in) atomicAdd(&hist[key], 1u); });  // (integers: any order)
     __syncthreads();
     for (int k = threadIdx.x; k <= slots; k += 64) count[(size_t)k * blocks + blockIdx.x] = hist[k];
 }
@@ -87,9 +100,7 @@ __device__ __forceinline__ void place_rows(const int32_t* __restrict__ slot, uin
                                            uint32_t* __restrict__ order, int32_t* __restrict__ row_slot)
 {
     const int lane = threadIdx.x & 63, bits = 32 - __clz(slots);
-    for (uint32_t r = r0; r < r1; r += 64) {
-        const bool in = r + lane < r1;
-        const int key = in ? group_key(slot, r + lane, slots) : 0;
+    each_key(slot, r0, r1, slots, [&](uint32_t row, bool in, int key) {
         unsigned long long same = __ballot(in);
         for (int b = 0; b < bits; ++b) {
             const bool one = (key >> b) & 1;
@@ -105,10 +116,10 @@ __device__ __forceinline__ void place_rows(const int32_t* __restrict__ slot, uin
         __builtin_amdgcn_wave_barrier();
         if (in) {
             const uint32_t place = base + (uint32_t)__popcll(before);
-            order[place] = r + lane;
+            order[place] = row;
             row_slot[place] = key < slots ? key : -1;
         }
-    }
+    });
 }
 __global__ __launch_bounds__(64) void group_place_kernel(const int32_t* __restrict__ slot, uint32_t rows, int slots, int blocks,
                                                          const uint32_t* __restrict__ count, const uint32_t* __restrict__ begin,
@@ -129,7 +140,7 @@ __global__ __launch_bounds__(64) void group_few_kernel(const int32_t* __restrict
     extern __shared__ uint32_t next[];
     for (int k = threadIdx.x; k <= slots; k += 64) next[k] = 0;
     __syncthreads();
-    for (uint32_t r = threadIdx.x; r < rows; r += 64) atomicAdd(&next[group_key(slot, r, slots)], 1u);
+    each_key(slot, 0, rows, slots, [&](uint32_t, bool in, int key) { if (in) atomicAdd(&next[key], 1u); });
     __syncthreads();
     uint32_t run = 0;
     for (int b = 0; b <= slots; b += 64) {
@@ -158,7 +169,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void group_mid_kernel(const int32
     uint32_t* mine = hist + wave * keys;
     const uint32_t per = ((rows + kGroupWaves - 1) / kGroupWaves + 63) & ~63u;
     const uint32_t r0 = min(rows, wave * per), r1 = min(rows, r0 + per);
-    for (uint32_t r = r0 + lane; r < r1; r += 64) atomicAdd(&mine[group_key(slot, r, slots)], 1u);
+    each_key(slot, r0, r1, slots, [&](uint32_t, bool in, int key) { if (in) atomicAdd(&mine[key], 1u); });
     __syncthreads();
     // keys in order, the waves of a key in order: a thread per key (keys <= 64 kGroupWaves) adds its waves up
     uint32_t sum = 0;
