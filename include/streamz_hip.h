@@ -340,7 +340,8 @@ int szh_logits_control_dev(const float *logits_dev, uint64_t ld_logits, uint64_t
  *   h1 = relu(x w1 + b1)            h2 = tanh(h1 w2 + b2 + scale (h1 a2[s]) b2[s])
  *   logits = h2 w3 + b3 + scale (h2 a3[s]) b3[s]
  * A row of a call names its slot in slots_dev; any value outside 0 .. slots - 1 (say -1) means the net alone.  Rows
- * are independent: what a row gets does not depend on what the other rows and their adapters hold, NaN included.
+ * are independent: what a row gets does not depend on what the other rows and their adapters hold, NaN included (the number
+ * of rows, and a row's place in the order of slots, may decide how its last bits are rounded).
  * The arithmetic mode of the net (szh_net_set_gemm) applies to the hidden-layer product.  No counterpart in the reference.
  *
  * init: NULL -> a2, a3 ~ U(-0.5, 0.5) / sqrt(inputs) from `seed`, b2 = b3 = 0 (a new adapter changes nothing); else

@@ -14,7 +14,8 @@
 //
 // A call's rows are brought into the order of their slots first (a stable counting sort), so that the tiles of
 // every product hold rows of one slot, nearly always, and a slot's rows are one range of every row sum.
-// Rows are independent of one another in every product: what a row gets does not depend on who else is in the call.
+// Rows are independent of one another in every product: what a row gets does not depend on what the others hold (its place
+// in the order may decide which kernel takes it, and with that the order of its sums).
 #include <algorithm>
 #include <cmath>
 #include <new>
