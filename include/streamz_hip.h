@@ -374,8 +374,9 @@ int szh_net_vote_adapted_dev(szh_net *net, szh_adapters *bank, const float *feat
 /* Training of a bank, the net frozen: zero_grad, accumulate over any number of blocks, (all-reduce,) clip, apply.
  * The gradient vector is [slots][param_count] floats, then [slots]{loss sum, live rows}.  A row counts (is live) if it has a slot,
  * a label in 0 .. output - 1 that its candidate list allows, and an input that is not zero after dropout
- * (lib.rs:607-609); the loss is -ln(max(p[label], 1e-12)), its gradient p - t (lib.rs:611-615, 1028).  controls may hold
- * a bias and a candidate list; penalties are refused.  Dropout draws are those of szh_net_accumulate_dev.
+ * (lib.rs:607-609); a row that does not count leaves the gradient as it is, whatever it holds, NaN and infinities included.
+ * The loss is -ln(max(p[label], 1e-12)), its gradient p - t (lib.rs:611-615, 1028).  controls may hold a bias and a
+ * candidate list; penalties are refused.  Dropout draws are those of szh_net_accumulate_dev.
  * Gradients are bit-identical on every call with the same arguments. */
 uint64_t szh_adapters_grad_len(const szh_adapters *bank);
 float *szh_adapters_grad_dev(szh_adapters *bank);

@@ -244,7 +244,7 @@ int factor_gradients(Adapters* a, uint32_t rows, hipStream_t s)
     const AdaptWorkspace& w = a->ws;
     const int h1 = (int)a->h1, h2 = (int)a->h2, out = (int)a->out, r = (int)a->rank;
     FactorArgs g{};
-    g.ldw = w.ldu; g.rank = r; g.slots = (int)a->slots; g.begin = w.begin; g.row_slot = w.row_slot;
+    g.ldw = w.ldu; g.rank = r; g.slots = (int)a->slots; g.begin = w.begin; g.row_slot = w.row_slot; g.live = w.live;
     g.job[0] = {w.h1, w.g2, nullptr, a->off_a2(), w.ld1, h1, r, 1, 0, 0};
     g.job[1] = {w.d2, w.u2, nullptr, a->off_b2(), w.ld2, h2, 1, h2, 0, 0};
     g.job[2] = {w.h2, w.g3, nullptr, a->off_a3(), w.ld2, h2, r, 1, 0, 0};

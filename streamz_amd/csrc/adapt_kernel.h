@@ -954,7 +954,8 @@ __global__ __launch_bounds__(64 * WAVES) void tail_kernel(BackArgs a, TailArgs o
 
 // ---- factor gradients -----------------------------------------------------------------------------
 // The four factors' gradients are four contractions over rows, grad[slot][m][j] = sum over the slot's rows of
-// p[i][m] w[i][j], m up to a layer's width and j the rank columns; one launch does all four.
+// p[i][m] w[i][j], m up to a layer's width and j the rank columns; one launch does all four.  A row that does not count has
+// zeros for either operand, whatever its activations are (0 x inf would be a NaN in every element of the slot).
 // slab[chunk + slot][m][j] takes the part of a chunk of rows: rows are sorted by slot, so (chunk, slot) pairs that
 // hold rows lie on a staircase and chunk + slot numbers them without a table; factor_reduce_kernel adds a slot's chunks.
 struct FactorJob {
@@ -970,6 +971,7 @@ struct FactorArgs {
     FactorJob job[4];
     const uint32_t* begin; // [slots + 2]
     const int32_t* row_slot;
+    const uint8_t* live;
     int ldw, rank, slots;
     uint32_t chunk;        // rows per chunk
 };
@@ -1001,18 +1003,20 @@ __global__ __launch_bounds__(256) void factor_grad_kernel(FactorArgs a)
         for (uint32_t i = r + 4 * wave; i < stop; i += 16 * G) {
             f32x4 pv[G];
             float wv[G][NT];
+            uint32_t live[G];
             const int col = m0 + 4 * c16;
 #pragma unroll
             for (int g2 = 0; g2 < G; ++g2) {
                 const size_t row = min(i + 16 * g2 + q, stop - 1);
                 pv[g2] = *reinterpret_cast<const f32x4*>(g.p + row * g.ldp + min(col, g.ldp - 4));
+                live[g2] = a.live[row];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) wv[g2][n] = g.w[row * a.ldw + min(16 * n + c16, a.rank - 1)];
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int g2 = 0; g2 < G; ++g2) {
-                const bool in = i + 16 * g2 + q < stop;
+                const bool in = i + 16 * g2 + q < stop && live[g2] != 0;
                 pv[g2] = cut_four(pv[g2], col, in ? g.M : 0);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
