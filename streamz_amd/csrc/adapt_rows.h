@@ -75,8 +75,9 @@ __device__ __forceinline__ void row_product(const float* x, int K, const float* 
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const bool on = k + i * slices < n_k;
-                        a0 = __builtin_fmaf(xv[i], on ? w[i].x : 0.0f, a0); a1 = __builtin_fmaf(xv[i], on ? w[i].y : 0.0f, a1);
-                        a2 = __builtin_fmaf(xv[i], on ? w[i].z : 0.0f, a2); a3 = __builtin_fmaf(xv[i], on ? w[i].w : 0.0f, a3);
+                        const float q = on ? xv[i] : 0.0f;   // (either may be none)
+                        a0 = __builtin_fmaf(q, on ? w[i].x : 0.0f, a0); a1 = __builtin_fmaf(q, on ? w[i].y : 0.0f, a1);
+                        a2 = __builtin_fmaf(q, on ? w[i].z : 0.0f, a2); a3 = __builtin_fmaf(q, on ? w[i].w : 0.0f, a3);
                     }
                 }
             } else {

@@ -43,3 +43,33 @@ def test_rows_that_do_not_count_leave_no_trace(dims, rank, n, mode):
     assert [int(v) for v in stats[:, 1]] == [int(((row % 5 > 2) & (s == k)).sum()) for k in range(slots)]
     g2, stats2 = grads(net, bank, y, labels, s, handle)
     assert np.array_equal(stats, stats2) and np.array_equal(g, g2)
+
+
+@pytest.mark.parametrize("dims,rank", [((60, 512, 256, 16), 16), ((7, 33, 21, 5), 3), ((61, 37, 30, 70), 9), ((60, 64, 300, 300), 5)])
+@pytest.mark.parametrize("n", [1, 9, 600])
+@pytest.mark.parametrize("value", [np.inf, -np.inf])
+@pytest.mark.parametrize("at", [0, -1])
+def test_an_infinite_feature_is_carried_through(dims, rank, n, value, at):
+    """With weights of one sign behind the first layer, an infinite feature makes hidden units 0 or inf, and tanh(inf) = 1: the logits
+    are finite and known, in every kernel."""
+    slots, (i, n1, n2, out) = 2, dims
+    rng = np.random.default_rng(sum(dims) + n)
+    params, flat, x = make(rng, dims, slots, rank, n, zero_rows=False)
+    params[2], flat = np.abs(params[2]) + np.float32(0.01), np.abs(flat) + np.float32(0.01)
+    assert (params[0][at] > 0).any() and (params[0][at] < 0).any()
+    x[:, at] = value
+    s = (np.arange(n) % 3 - 1).astype(np.int32)
+    net = sz.SimpleNeuralNet(*dims, init=params)
+    bank = sz.Adapters(net, slots, rank, scale=0.7, init=flat)
+    logits, probs = forward(net, bank, x, s)
+    one = tr.T(np.ones((1, n2)))
+    for k in range(-1, slots):
+        want = tr.dot(one, tr.T(params[4]), rank + 1)
+        if k >= 0:
+            a3, b3 = tr.split(flat[k], tr.adapter_shapes(dims, rank))[2:]
+            want = tr.add(want, tr.dot(tr.mul(tr.dot(one, tr.T(a3)), tr.T(np.float64(np.float32(0.7)))), tr.T(b3)))
+        want = tr.add(want, tr.T(params[5]))
+        rows = np.flatnonzero(s == k)
+        want = tr.T(np.repeat(want.v, len(rows), 0), np.repeat(want.e, len(rows), 0))
+        tr.check(logits[rows], want, "logits")
+        tr.check(probs[rows], tr.control(want, None, out)[1], "probabilities")
