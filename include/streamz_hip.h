@@ -313,7 +313,8 @@ int szh_clip_run_dev(szh_clip *clip, float max_norm, float *norms_dev, void *str
  *   z = l;   n > 0:  z = (z > 0 ? z / repetition[k] : z * repetition[k]) - presence[k]
  *   z = z - frequency[k] * n + bias[k][c];   z = -inf where class c is not allowed
  *   p = exp(z - max z) / sum of exp(z - max z); a class that is not allowed, whatever its logit, has p = 0, and a row
- *   without any class left (every z = -inf) has p = 0 throughout.
+ *   without any class left (every z = -inf) has p = 0 throughout.  A candidate's NaN or +inf makes the p of every
+ *   candidate a NaN; the other classes keep p = 0.
  * allow: bit c % 32 of word c / 32 set = class c is a candidate.  Penalties need counts; below zero (or a repetition
  * below one) they favour who has spoken already.  No counterpart in the reference. */
 typedef struct szh_logit_controls {
@@ -367,7 +368,7 @@ int szh_net_forward_adapted_dev(szh_net *net, szh_adapters *bank, const float *f
                                 const szh_logit_controls *controls, float *logits_dev, float *probs_dev, void *stream);
 /* Votes of identify_speaker_list (lib.rs:1391-1402) for many requests at once: a row's top class (the last maximum wins)
  * is counted in counts_dev[group_of_row[row]][output] if its probability is >= threshold; a row without a
- * candidate, and one whose group is outside 0 .. groups - 1, votes for nobody.  group_of_row NULL: group 0. */
+ * candidate, one whose probabilities are NaN, and one whose group is outside 0 .. groups - 1, votes for nobody.  group_of_row NULL: group 0. */
 int szh_net_vote_adapted_dev(szh_net *net, szh_adapters *bank, const float *feats_dev, const int32_t *slots_dev, uint64_t n,
                              const szh_logit_controls *controls, float threshold, const int32_t *group_of_row_dev, uint32_t groups,
                              unsigned long long *counts_dev, void *stream);

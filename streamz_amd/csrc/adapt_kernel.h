@@ -938,6 +938,7 @@ __global__ __launch_bounds__(64 * WAVES) void tail_kernel(BackArgs a, TailArgs o
         if (c < a.out && tr.live) {
             const float p = z[r][c] * inv;
             v = c == tr.label ? p - 1.0f : p;
+            if (inv != inv && !control::allowed(rc, c)) v = 0.0f;
             if (real && c == tr.label) run.loss[i] = -logf(fmaxf(p, 1e-12f));
         }
         z[r][c] = v;

@@ -270,7 +270,7 @@ __global__ __launch_bounds__(kRowT) void row_out_kernel(RowArgs a, Controls ctl,
         return;
     }
     if (OUT == OUT_INFER) {
-        for (int n = threadIdx.x; n < C; n += kRowT) c.out[row * c.ld_out + n] = z[n] * inv;
+        for (int n = threadIdx.x; n < C; n += kRowT) c.out[row * c.ld_out + n] = control::probability(rc, z[n], inv, n);
         return;
     }
     const int label = c.labels[row];
@@ -281,6 +281,10 @@ __global__ __launch_bounds__(kRowT) void row_out_kernel(RowArgs a, Controls ctl,
         if (live && n == label) c.loss[i] = -logf(fmaxf(p, 1e-12f));
         z[n] = v;
         a.d3[i * a.ld3 + n] = v;
+    }
+    if (inv != inv && rc.allow) {  // (the classes off the list of a row of NaNs)
+        for (int n = threadIdx.x; n < C; n += kRowT)
+            if (!control::allowed(rc, n)) a.d3[i * a.ld3 + n] = z[n] = 0.0f;
     }
     if (threadIdx.x == 0) {
         c.live[i] = live ? 1 : 0;

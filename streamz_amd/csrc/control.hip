@@ -23,6 +23,19 @@ namespace {
 
 using namespace control;
 
+// out[c] = 0 for a lane's classes that are off the list of a row of NaNs (in a training row that does not count all are 0
+// already).  Found again from the row's number: what this rare case needs takes no registers from the others.
+template <int LANES>
+__device__ __forceinline__ void clear_off_list(const Controls& ctl, uint64_t row, int C, int l, float* out)
+{
+    asm volatile("" : "+v"(row));
+    const RowControl rc = row_control(ctl, C, row_set(ctl, row));
+#pragma unroll 1
+    for (int c = 4 * l; c < C; c += 4 * LANES)
+        for (int k = c; k < min(c + 4, C); ++k)
+            if (!allowed(rc, k)) out[k] = 0.0f;
+}
+
 // LANES lanes of a wave per row, Q groups of four classes per lane: class 4 (l + LANES q) + e.  A row's logits
 // and the number of its set are asked for while the row before is worked on.
 template <int MODE, int LANES, int Q>
@@ -106,6 +119,7 @@ __global__ __launch_bounds__(256) void control_rows_kernel(Controls ctl, Control
 #pragma unroll
             for (int e = 0; e < 4; ++e) z[q][e] = c + e < C && ((bits >> e) & 1u) ? z[q][e] : -INFINITY;
         }
+        bool nans = false;
         if (MODE != M_INFER || a.probs) {
             float top = -INFINITY;
 #pragma unroll
@@ -122,6 +136,7 @@ __global__ __launch_bounds__(256) void control_rows_kernel(Controls ctl, Control
             sum = lanes_sum<LANES>(sum);
             const bool some = !(sum <= 0.0f);  // (a NaN row stays one)
             const float inv = some ? 1.0f / sum : 0.0f;
+            nans = !(inv == inv);
 #pragma unroll
             for (int q = 0; q < Q; ++q)
 #pragma unroll
@@ -172,6 +187,7 @@ __global__ __launch_bounds__(256) void control_rows_kernel(Controls ctl, Control
                     if (c + e < C) out[c + e] = z[q][e];
             }
         }
+        if (nans) clear_off_list<LANES>(ctl, row, C, l, out);
     }
 }
 
@@ -304,8 +320,15 @@ __global__ __launch_bounds__(kRowThreads) void control_row_kernel(Controls ctl, 
                 if (part[w] > bp || (part[w] == bp && part_c[w] > best)) { bp = part[w]; best = part_c[w]; }
             cast_vote(a, row, C, some, bp, best);
         }
-    } else if (MODE == M_INFER) {
+        return;
+    }
+    const bool mend = !(inv == inv) && rc.allow;  // (the classes off the list of a row of NaNs)
+    if (MODE == M_INFER) {
         each([&](float& v, uint32_t c) { out[c] = prob(v); });
+        if (mend) {
+            for (int c = threadIdx.x; c < C; c += kRowThreads)
+                if (!allowed(rc, c)) out[c] = 0.0f;
+        }
     } else {
         const TrainRow t = train_row(a, rc, i, row, C, some);
         if (threadIdx.x == 0 && !(t.label >= 0 && t.label < C)) { a.loss[i] = 0.0f; a.live[i] = 0; }
@@ -314,6 +337,10 @@ __global__ __launch_bounds__(kRowThreads) void control_row_kernel(Controls ctl, 
             if ((int)c == t.label) { a.loss[i] = t.live ? -logf(fmaxf(p, 1e-12f)) : 0.0f; a.live[i] = t.live ? 1 : 0; }
             out[c] = t.live ? ((int)c == t.label ? p - 1.0f : p) : 0.0f;
         });
+        if (mend && t.live) {
+            for (int c = threadIdx.x; c < C; c += kRowThreads)
+                if (!allowed(rc, c)) out[c] = 0.0f;
+        }
     }
 }
 

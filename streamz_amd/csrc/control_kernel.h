@@ -39,6 +39,13 @@ __device__ __forceinline__ RowControl row_control(const Controls& c, int C, int3
 
 __device__ __forceinline__ bool allowed(const RowControl& r, int c) { return !r.allow || ((r.allow[c >> 5] >> (c & 31)) & 1u); }
 
+// a class's probability from its exponential: 0 off the list, also in a row whose sum is a NaN
+__device__ __forceinline__ float probability(const RowControl& r, float e, float inv, int c)
+{
+    const float p = e * inv;
+    return p == p || allowed(r, c) ? p : 0.0f;
+}
+
 // (the division by the repetition penalty is a product with its reciprocal: two roundings instead of one)
 __device__ __forceinline__ float penalised(const RowControl& r, float z, uint32_t count)
 {

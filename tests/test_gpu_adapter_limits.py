@@ -73,3 +73,62 @@ def test_an_infinite_feature_is_carried_through(dims, rank, n, value, at):
         want = tr.T(np.repeat(want.v, len(rows), 0), np.repeat(want.e, len(rows), 0))
         tr.check(logits[rows], want, "logits")
         tr.check(probs[rows], tr.control(want, None, out)[1], "probabilities")
+
+
+def masks_around(rng, classes, sets):
+    """About half of the classes, class 1 among them and class 0 not."""
+    allow = rng.integers(0, 1 << 32, (sets, (classes + 31) // 32), dtype=np.uint32)
+    allow[:, 0] = (allow[:, 0] & ~np.uint32(1)) | np.uint32(2)
+    bits = (allow[:, np.arange(classes) // 32] >> (np.arange(classes) % 32).astype(np.uint32)) & 1
+    return allow, bits.astype(bool)
+
+
+@pytest.mark.parametrize("classes", [2, 7, 16, 33, 64, 100, 250, 500, 1000, 2000, 6000, 12000, 51000, 60001])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_class_off_the_list_has_no_probability_whatever_the_row_holds(classes, value, in_place):
+    """A candidate's NaN or infinity makes every candidate's probability a NaN; the others stay at 0."""
+    import torch
+    rows = 6
+    rng = np.random.default_rng(classes)
+    z = rng.standard_normal((rows, classes)).astype(np.float32)
+    allow, bits = masks_around(rng, classes, rows)
+    z[::2, 1] = value
+    z[1::2, 0] = value
+    c = {"sets": rows, "allow": allow, "set_of_row": np.arange(rows, dtype=np.int32)}
+    handle, keep = dev_controls(c)
+    d = dev(z)
+    out = d if in_place else torch.full_like(d, 7.0)
+    sz.control_logits_dev(d.data_ptr(), rows, classes, handle, out.data_ptr(), probs=True)
+    torch.cuda.synchronize()
+    got = out.cpu().numpy()
+    assert not got[~bits].any()
+    assert np.isnan(got[::2][bits[::2]]).all() and np.isfinite(got[1::2]).all()
+
+
+@pytest.mark.parametrize("dims,rank", [((60, 64, 32, 16), 4), ((60, 64, 48, 100), 20), ((60, 64, 32, 1200), 4), ((60, 64, 300, 300), 4)])
+@pytest.mark.parametrize("n", [5, 600])
+def test_a_class_off_the_list_has_no_probability_behind_the_adapters(dims, rank, n):
+    slots, out = 2, dims[3]
+    rng = np.random.default_rng(sum(dims) + n)
+    params, flat, x = make(rng, dims, slots, rank, n)
+    s = (np.arange(n) % 2).astype(np.int32)
+    flat[1, -1] = np.nan                     # the last class's factor: that logit of slot 1 alone is none
+    allow, bits = masks_around(rng, out, 2)
+    allow[:, -1] |= np.uint32(1 << ((out - 1) % 32))
+    bits[:, -1] = True
+    net = sz.SimpleNeuralNet(*dims, init=params)
+    bank = sz.Adapters(net, slots, rank, init=flat)
+    c = {"sets": 2, "allow": allow, "set_of_row": s}
+    handle, keep = dev_controls(c)
+    logits, probs = forward(net, bank, x, s, handle)
+    off = ~bits[s]
+    assert np.isnan(logits[s == 1, -1]).all() and np.isfinite(logits[:, :-1]).all() and np.isfinite(logits[s == 0]).all()
+    assert not probs[off].any() and np.isfinite(probs[s == 0]).all()
+    assert np.isnan(probs[s == 1][bits[s[s == 1]]]).all()
+    # the loss takes nothing from there either: the classes' own factors get no gradient
+    labels = np.full(n, out - 1, np.int32)
+    g, _ = grads(net, bank, x, labels, s, handle)
+    b3 = g[:, rank * (dims[1] + 2 * dims[2]):].reshape(2, rank, out)
+    for k in range(2):
+        assert not b3[k][:, ~bits[k]].any()
