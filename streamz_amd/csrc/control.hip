@@ -11,6 +11,7 @@
 // between the maximum, the sum and the result, so nothing is read twice up to kRowMax classes: some lanes of a
 // wave per row up to 1024 classes (control_rows_kernel), a workgroup per row beyond (control_row_kernel).
 #include <algorithm>
+#include <type_traits>
 
 #include "control_kernel.h"
 #include "internal.h"
@@ -300,8 +301,10 @@ __global__ __launch_bounds__(kRowThreads) void control_row_kernel(Controls ctl, 
     each([&](float& v, uint32_t) { top = fmaxf(top, v); });
     top = join_waves(lanes_max<64>(top), part, [](float x, float y) { return fmaxf(x, y); });
     const float shift = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
-    each([&](float& v, uint32_t) { v = exp_low(v - shift); sum += v; });
+    // (up to 50 values a thread in registers are added in 32 bits; of any number of them a small one would be lost beside the sum of the others)
+    std::conditional_t<V != 0, float, double> mine = 0;
+    each([&](float& v, uint32_t) { v = exp_low(v - shift); mine += v; });
+    float sum = (float)mine;
     sum = join_waves(lanes_sum<64>(sum), part, [](float x, float y) { return x + y; });
     const bool some = !(sum <= 0.0f);
     const float inv = some ? 1.0f / sum : 0.0f;

@@ -132,3 +132,23 @@ def test_a_class_off_the_list_has_no_probability_behind_the_adapters(dims, rank,
     b3 = g[:, rank * (dims[1] + 2 * dims[2]):].reshape(2, rank, out)
     for k in range(2):
         assert not b3[k][:, ~bits[k]].any()
+
+
+def test_the_sum_of_a_row_of_very_many_classes():
+    """1024 classes at the top and two million that are 2^-25 of them each: together 6 %, every one less than half a step of a sum
+    that holds a top class."""
+    import torch
+    classes = (1 << 21) + 3
+    low = np.float32(np.log(2.0 ** -25))
+    z = np.full((2, classes), low, np.float32)
+    z[0, :1024] = 0.0
+    z[1, -1024:] = 0.0
+    d = dev(z)
+    out = torch.empty_like(d)
+    sz.control_logits_dev(d.data_ptr(), 2, classes, None, out.data_ptr(), probs=True)
+    torch.cuda.synchronize()
+    e = np.exp(z.astype(np.float64))
+    p = e / e.sum(axis=1, keepdims=True)
+    # an exponential of at most 2 ulp and its exponent's rounding (18 U at most) in numerator and sum; a thread's sum in 64 bits, its rounding,
+    # 6 + 15 additions across lanes and waves; the reciprocal and the product
+    np.testing.assert_allclose(out.cpu().numpy(), p, rtol=(2 * (4 + 18) + 1 + 21 + 2) * tr.U, atol=0)
