@@ -312,6 +312,7 @@ int szh_clip_run_dev(szh_clip *clip, float max_norm, float *norms_dev, void *str
  * outside 0 .. sets - 1 the row has no control.  With n = counts[k][c], how often class c was answered already:
  *   z = l;   n > 0:  z = (z > 0 ? z / repetition[k] : z * repetition[k]) - presence[k]
  *   z = z - frequency[k] * n + bias[k][c];   z = -inf where class c is not allowed
+ *   (the quotient is z times the reciprocal, two roundings, for every repetition)
  *   p = exp(z - max z) / sum of exp(z - max z); a class that is not allowed, whatever its logit, has p = 0, and a row
  *   without any class left (every z = -inf) has p = 0 throughout.  A candidate's NaN or +inf makes the p of every
  *   candidate a NaN; the other classes keep p = 0.

@@ -14,7 +14,8 @@ struct RowControl {
     const float* bias;
     const uint32_t* allow;
     const uint32_t* counts;
-    float repetition, inverse, presence, frequency;
+    // z / repetition = z scale * inverse: scale is 1, or 2^+-64 for a repetition whose own reciprocal is no normal number
+    float repetition, scale, inverse, presence, frequency;
 };
 
 __device__ __forceinline__ int32_t row_set(const Controls& c, uint64_t row)
@@ -24,13 +25,18 @@ __device__ __forceinline__ int32_t row_set(const Controls& c, uint64_t row)
 
 __device__ __forceinline__ RowControl row_control(const Controls& c, int C, int32_t set)
 {
-    RowControl r{nullptr, nullptr, nullptr, 1.0f, 1.0f, 0.0f, 0.0f};
+    RowControl r{nullptr, nullptr, nullptr, 1.0f, 1.0f, 1.0f, 0.0f, 0.0f};
     if (set < 0 || (uint32_t)set >= c.sets) return r;
     if (c.bias) r.bias = c.bias + (uint64_t)set * C;
     if (c.allow) r.allow = c.allow + (uint64_t)set * ((C + 31) / 32);
     if (c.counts) {
         r.counts = c.counts + (uint64_t)set * C;
-        if (c.repetition) { r.repetition = c.repetition[set]; r.inverse = 1.0f / r.repetition; }
+        if (c.repetition) {
+            r.repetition = c.repetition[set];
+            const float size = fabsf(r.repetition);
+            r.scale = size < 0x1p-126f ? 0x1p64f : size > 0x1p126f ? 0x1p-64f : 1.0f;
+            r.inverse = 1.0f / (r.repetition * r.scale);
+        }
         if (c.presence) r.presence = c.presence[set];
         if (c.frequency) r.frequency = c.frequency[set];
     }
@@ -46,11 +52,12 @@ __device__ __forceinline__ float probability(const RowControl& r, float e, float
     return p == p || allowed(r, c) ? p : 0.0f;
 }
 
-// (the division by the repetition penalty is a product with its reciprocal: two roundings instead of one)
+// (the division by the repetition penalty is a product with its reciprocal: two roundings instead of one.  The division itself: 661400 x 64
+// 90 us instead of 86, 1024 x 50001 177 instead of 170)
 __device__ __forceinline__ float penalised(const RowControl& r, float z, uint32_t count)
 {
     const float n = (float)count;
-    const float seen = (z > 0.0f ? z * r.inverse : z * r.repetition) - r.presence;
+    const float seen = (z > 0.0f ? z * r.scale : z) * (z > 0.0f ? r.inverse : r.repetition) - r.presence;
     return (n > 0.0f ? seen : z) - r.frequency * n;
 }
 

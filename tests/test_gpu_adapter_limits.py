@@ -152,3 +152,29 @@ def test_the_sum_of_a_row_of_very_many_classes():
     # an exponential of at most 2 ulp and its exponent's rounding (18 U at most) in numerator and sum; a thread's sum in 64 bits, its rounding,
     # 6 + 15 additions across lanes and waves; the reciprocal and the product
     np.testing.assert_allclose(out.cpu().numpy(), p, rtol=(2 * (4 + 18) + 1 + 21 + 2) * tr.U, atol=0)
+
+
+@pytest.mark.parametrize("classes", [16, 500, 3000])
+@pytest.mark.parametrize("repetition", [2e-39, 1e-30, 1.3, 1e30, 1.6e38, 3.3e38])
+def test_a_repetition_near_the_ends_of_the_range(classes, repetition):
+    """z / repetition, that of the reciprocal and that of the product, also where the reciprocal of the repetition is no normal number."""
+    import torch
+    rng = np.random.default_rng(classes)
+    z = (np.exp(rng.uniform(-80, 80, (4, classes))) * rng.choice([-1, 1], (4, classes))).astype(np.float32)
+    rep = np.full(1, repetition, np.float32)
+    c = {"sets": 1, "counts": np.ones((1, classes), np.uint32), "repetition": rep}
+    handle, keep = dev_controls(c)
+    d = dev(z)
+    out = torch.empty_like(d)
+    sz.control_logits_dev(d.data_ptr(), 4, classes, handle, out.data_ptr(), probs=False)
+    torch.cuda.synchronize()
+    wide = z.astype(np.float64)
+    with np.errstate(over="ignore"):
+        want = np.where(wide > 0, wide / np.float64(rep[0]), wide * np.float64(rep[0]))
+    near = np.abs(np.abs(want) / 2.0 ** 128 - 1) < 4 * tr.U   # (these may round to infinity or not)
+    inf = (np.abs(want) >= 2.0 ** 128) & ~near
+    got = out.cpu().numpy().astype(np.float64)
+    assert np.array_equal(np.isinf(got[~near]), inf[~near]) and (np.sign(got[inf]) == np.sign(want[inf])).all()
+    # two roundings, (1 + U)^2 - 1, and that of a result below the normal numbers
+    fine = ~inf & ~near
+    np.testing.assert_array_less(np.abs(got[fine] - want[fine]), 2.001 * tr.U * np.abs(want[fine]) + 2.0 ** -150 + 1e-60)
