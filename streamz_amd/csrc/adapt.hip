@@ -64,6 +64,9 @@ uint32_t factor_chunk(const Adapters* a, uint64_t rows)
 // most chunks that a call of up to `rows` rows makes
 uint64_t factor_chunks_most(const Adapters* a, uint64_t rows) { return std::max<uint64_t>(rows / 512, 1024 / factor_tiles(a)) + 2; }
 
+// whether the output layer goes with its rank columns (low_out) instead of being a product of its own
+bool low_out_applies(const Adapters* a) { return a->out <= 64; }
+
 // How the arrays of a pass lie in the workspace; `base` null: only the size.
 size_t lay_out(const Adapters* a, uint64_t rows, bool training, char* base, AdaptWorkspace* w)
 {
@@ -75,7 +78,7 @@ size_t lay_out(const Adapters* a, uint64_t rows, bool training, char* base, Adap
     AdaptWorkspace t;
     AdaptWorkspace& o = w ? *w : t;
     const uint64_t blocks = (rows + kGroupRows - 1) / kGroupRows, S = a->slots;
-    o.ldx = a->in + 1 <= 64 ? 64 : round_up((int)a->in + 1, 128);
+    o.ldx = round_up((int)a->in, 32);
     o.ld1 = round_up((int)a->h1, 32); o.ld2 = round_up((int)a->h2, 32); o.ld3 = round_up((int)std::max(a->out, 1u), 4);
     o.ldu = round_up((int)a->rank, 8);
     take(o.order, rows); take(o.row_slot, rows); take(o.begin, S + 2); take(o.count, (S + 1) * blocks); take(o.total, S + 1);
@@ -83,7 +86,8 @@ size_t lay_out(const Adapters* a, uint64_t rows, bool training, char* base, Adap
     take(o.h1, (rows + 32) * o.ld1); take(o.h2, (rows + 32) * o.ld2); take(o.lg, (rows + 32) * o.ld3);
     take(o.u2, rows * o.ldu); take(o.u3, rows * o.ldu);
     take(o.add2, kFewRows * o.ld2); take(o.add3, kFewRows * o.ld3);
-    take(o.w1t, (uint64_t)a->h1 * o.ldx); take(o.w2t, (uint64_t)o.ld1 * a->h2); take(o.w3t, (uint64_t)o.ld2 * std::max(a->out, 1u));
+    take(o.w2t, (uint64_t)o.ld1 * a->h2);
+    if (!low_out_applies(a)) take(o.w3t, (uint64_t)o.ld2 * a->out);
     take(o.w2s, 3 * ((uint64_t)a->h1 * a->h2 + 1) / 2 + 4);
     if (training) {
         take(o.d2, (rows + 32) * o.ld2); take(o.g2, rows * o.ldu); take(o.g3, rows * o.ldu); take(o.loss, rows);
@@ -212,8 +216,7 @@ int front_rows(const Net* n, const Adapters* a, const float* x, int ldx, const u
     return SZH_OK;
 }
 
-// Output layers of up to 64 classes: u3 and the logits in one pass over h2
-bool low_out_applies(const Adapters* a) { return a->out <= 64; }
+// u3 and the logits of up to 64 classes in one pass over h2
 int low_out(const Net* n, const Adapters* a, uint32_t rows, hipStream_t s)
 {
     const AdaptWorkspace& w = a->ws;

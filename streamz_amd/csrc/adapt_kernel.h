@@ -191,7 +191,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void group_mid_kernel(const int32
 }
 
 // ---- rows in that order -------------------------------------------------------------------------
-// xs[i] = [x[order[i]] | 1 | 0 ...] with input dropout (element j of row r zeroed where uniform01(seed,
+// xs[i] = [x[order[i]] | 0 ...] with input dropout (element j of row r zeroed where uniform01(seed,
 // counter0 + r, j) < dropout: the draws of szh_net_accumulate_dev), live[i] = any element left.  One wave per row.
 __global__ __launch_bounds__(256) void gather_rows_kernel(const float* __restrict__ x, const uint32_t* __restrict__ order,
                                                           uint32_t rows, int in, float dropout, uint64_t seed, uint64_t counter0,
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(256) void gather_rows_kernel(const float* __restric
     const int lane = threadIdx.x & 63;
     bool any = false;
     for (int j = lane; j < ldx; j += 64) {
-        float v = j == in ? 1.0f : 0.0f;
+        float v = 0.0f;
         if (j < in) {
             v = x[(size_t)r * in + j];
             if (dropout > 0.0f && uniform01(seed, counter0 + r, (uint64_t)j) < dropout) v = 0.0f;

@@ -300,12 +300,11 @@ struct ControlRun {
 int control_run(const Controls& ctl, const ControlRun& a, hipStream_t s);
 
 // ---- low-rank adapters (adapt.hip) ---------------------------------------------------------
-constexpr uint32_t kAdaptMaxSlots = 8192, kAdaptMaxRank = 64;
 struct AdaptWorkspace {
     int ldx = 0, ld1 = 0, ld2 = 0, ld3 = 0, ldu = 0;  // row strides
     uint32_t *order = nullptr, *begin = nullptr, *count = nullptr, *total = nullptr, *w2s = nullptr;
     int32_t* row_slot = nullptr;
-    float *xs = nullptr, *h1 = nullptr, *h2 = nullptr, *lg = nullptr, *u2 = nullptr, *u3 = nullptr, *w1t = nullptr, *w2t = nullptr,
+    float *xs = nullptr, *h1 = nullptr, *h2 = nullptr, *lg = nullptr, *u2 = nullptr, *u3 = nullptr, *w2t = nullptr,
           *w3t = nullptr, *add2 = nullptr, *add3 = nullptr, *d2 = nullptr, *g2 = nullptr, *g3 = nullptr, *loss = nullptr, *slab = nullptr;
     uint8_t *live0 = nullptr, *live = nullptr;
 };
