@@ -61,8 +61,13 @@ uint32_t factor_chunk(const Adapters* a, uint64_t rows)
     const uint64_t want = std::max<uint64_t>(1, 1024 / factor_tiles(a)), least = rows <= kFewRows ? 16 : 64;
     return (uint32_t)std::min<uint64_t>(512, std::max<uint64_t>(least, (rows / want + least - 1) / least * least));
 }
-// most chunks that a call of up to `rows` rows makes
-uint64_t factor_chunks_most(const Adapters* a, uint64_t rows) { return std::max<uint64_t>(rows / 512, 1024 / factor_tiles(a)) + 2; }
+// Most chunks that a call of up to `rows` rows makes.  Below 512 rows a chunk they are as many as wanted, and what is left over by the
+// division of the rows among them: fewer rows than chunks are wanted, in chunks of 64 and more.
+uint64_t factor_chunks_most(const Adapters* a, uint64_t rows)
+{
+    const uint64_t want = std::max<uint64_t>(1, 1024 / factor_tiles(a));
+    return std::max<uint64_t>(rows / 512, want + want / 64) + 2;
+}
 
 // whether the output layer goes with its rank columns (low_out) instead of being a product of its own
 bool low_out_applies(const Adapters* a) { return a->out <= 64; }

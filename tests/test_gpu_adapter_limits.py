@@ -178,3 +178,18 @@ def test_a_repetition_near_the_ends_of_the_range(classes, repetition):
     # two roundings, (1 + U)^2 - 1, and that of a result below the normal numbers
     fine = ~inf & ~near
     np.testing.assert_array_less(np.abs(got[fine] - want[fine]), 2.001 * tr.U * np.abs(want[fine]) + 2.0 ** -150 + 1e-60)
+
+
+@pytest.mark.parametrize("dims,rank,n", [((60, 64, 64, 16), 4, 16639), ((60, 128, 64, 16), 16, 13259), ((60, 30, 20, 70), 3, 13200), ((60, 64, 64, 16), 4, 33023)])
+def test_gradients_of_just_fewer_rows_than_a_whole_step_of_chunks(dims, rank, n):
+    """As many chunks of rows as a call can make beyond those that fill the chip."""
+    slots = 3
+    rng = np.random.default_rng(n)
+    params, flat, x = make(rng, dims, slots, rank, n)
+    s, labels = pick_slots(rng, n, slots, "mixed"), rng.integers(-1, dims[3], n).astype(np.int32)
+    net = sz.SimpleNeuralNet(*dims, init=params)
+    bank = sz.Adapters(net, slots, rank, scale=0.7, init=flat)
+    g, stats = grads(net, bank, x, labels, s)
+    want, want_stats = tr.train(params, flat, known(slots, s), 0.7, x, labels, rank, dims)
+    tr.check(stats, want_stats, "loss and live rows")
+    tr.check(g, want, "gradient")
