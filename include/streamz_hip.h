@@ -349,8 +349,9 @@ int szh_logits_control_dev(const float *logits_dev, uint64_t ld_logits, uint64_t
  * init: NULL -> a2, a3 ~ U(-0.5, 0.5) / sqrt(inputs) from `seed`, b2 = b3 = 0 (a new adapter changes nothing); else
  * [slots][szh_adapters_param_count] floats.
  * The *_dev calls on one bank share its workspace and must be serialised by the caller (two streams, two captured graphs
- * in flight race); banks may be used beside one another on one net.  The workspace grows to the largest call so far, at least to
- * twice its size at a time, and the earlier ones are kept until the bank goes (a captured graph may work in them);
+ * in flight race); banks may be used beside one another on one net.  What of it goes by rows grows to the largest call
+ * so far, at least to twice its size at a time, and the earlier arrays, together no larger than the last, are kept until the bank
+ * goes (a captured graph may work in them); the rest, in training a partial gradient of every slot among it, is there once.
  * szh_adapters_reserve sizes it (and the tables of szh_adapters_clip_grad_dev) ahead, which a caller that captures calls into a
  * graph does first.  Calls of more than 131072 rows are walked in pieces of that size. */
 #define SZH_ADAPTER_MAX_RANK 64

@@ -61,66 +61,98 @@ uint32_t factor_chunk(const Adapters* a, uint64_t rows)
     const uint64_t want = std::max<uint64_t>(1, 1024 / factor_tiles(a)), least = rows <= kFewRows ? 16 : 64;
     return (uint32_t)std::min<uint64_t>(512, std::max<uint64_t>(least, (rows / want + least - 1) / least * least));
 }
-// Most chunks that a call of up to `rows` rows makes.  Below 512 rows a chunk they are as many as wanted, and what is left over by the
-// division of the rows among them: fewer rows than chunks are wanted, in chunks of 64 and more.
-uint64_t factor_chunks_most(const Adapters* a, uint64_t rows)
+// Most chunks that a call makes whose chunks are shorter than 512 rows: as many as wanted, and those of what is left over by the division of
+// the rows among them (fewer rows than chunks are wanted, in chunks of 64 and more).  And that one of up to `rows` rows makes.
+uint64_t factor_chunks_any(const Adapters* a)
 {
     const uint64_t want = std::max<uint64_t>(1, 1024 / factor_tiles(a));
-    return std::max<uint64_t>(rows / 512, want + want / 64) + 2;
+    return want + want / 64 + 2;
 }
+uint64_t factor_chunks_most(const Adapters* a, uint64_t rows) { return std::max<uint64_t>((rows + 511) / 512, factor_chunks_any(a)); }
 
 // whether the output layer goes with its rank columns (low_out) instead of being a product of its own
 bool low_out_applies(const Adapters* a) { return a->out <= 64; }
 
-// How the arrays of a pass lie in the workspace; `base` null: only the size.
-size_t lay_out(const Adapters* a, uint64_t rows, bool training, char* base, AdaptWorkspace* w)
+// The workspace is in four parts: what a bank needs whatever its calls (the partial gradients of many slots are the largest of
+// it), the same for training, and the arrays that go by rows, with those of training by themselves.  Only the latter two grow.
+enum Part { PART_BANK, PART_TRAIN_BANK, PART_ROWS, PART_TRAIN_ROWS };
+
+// How the arrays of a part for `rows` rows lie; `base` null: only the size.
+size_t lay_out(const Adapters* a, Part part, uint64_t rows, char* base, AdaptWorkspace& o)
 {
     size_t at = 0;
     auto take = [&](auto*& p, uint64_t count) {
         p = reinterpret_cast<std::decay_t<decltype(p)>>(base + at);
         at += (count * sizeof(*p) + 255) / 256 * 256;
     };
-    AdaptWorkspace t;
-    AdaptWorkspace& o = w ? *w : t;
     const uint64_t blocks = (rows + kGroupRows - 1) / kGroupRows, S = a->slots;
     o.ldx = round_up((int)a->in, 32);
     o.ld1 = round_up((int)a->h1, 32); o.ld2 = round_up((int)a->h2, 32); o.ld3 = round_up((int)std::max(a->out, 1u), 4);
     o.ldu = round_up((int)a->rank, 8);
-    take(o.order, rows); take(o.row_slot, rows); take(o.begin, S + 2); take(o.count, (S + 1) * blocks); take(o.total, S + 1);
-    take(o.xs, rows * o.ldx); take(o.live0, rows); take(o.live, rows);
-    take(o.h1, (rows + 32) * o.ld1); take(o.h2, (rows + 32) * o.ld2); take(o.lg, (rows + 32) * o.ld3);
-    take(o.u2, rows * o.ldu); take(o.u3, rows * o.ldu);
-    take(o.add2, kFewRows * o.ld2); take(o.add3, kFewRows * o.ld3);
-    take(o.w2t, (uint64_t)o.ld1 * a->h2);
-    if (!low_out_applies(a)) take(o.w3t, (uint64_t)o.ld2 * a->out);
-    take(o.w2s, 3 * ((uint64_t)a->h1 * a->h2 + 1) / 2 + 4);
-    if (training) {
-        take(o.d2, (rows + 32) * o.ld2); take(o.g2, rows * o.ldu); take(o.g3, rows * o.ldu); take(o.loss, rows);
-        take(o.slab, (factor_chunks_most(a, rows) + S) * a->per_slot());
+    switch (part) {
+    case PART_BANK:
+        take(o.begin, S + 2); take(o.total, S + 1);
+        take(o.add2, kFewRows * o.ld2); take(o.add3, kFewRows * o.ld3);
+        take(o.w2t, (uint64_t)o.ld1 * a->h2);
+        if (!low_out_applies(a)) take(o.w3t, (uint64_t)o.ld2 * a->out);
+        take(o.w2s, 3 * ((uint64_t)a->h1 * a->h2 + 1) / 2 + 4);
+        break;
+    case PART_TRAIN_BANK:
+        take(o.slot_slab, S * a->per_slot());
+        o.chunks = factor_chunks_any(a);
+        take(o.chunk_slab, o.chunks * a->per_slot());
+        break;
+    case PART_ROWS:
+        take(o.order, rows); take(o.row_slot, rows); take(o.count, (S + 1) * blocks);
+        take(o.xs, rows * o.ldx); take(o.live0, rows);
+        take(o.h1, (rows + 32) * o.ld1); take(o.h2, (rows + 32) * o.ld2); take(o.lg, (rows + 32) * o.ld3);
+        take(o.u2, rows * o.ldu); take(o.u3, rows * o.ldu);
+        break;
+    default:
+        take(o.live, rows); take(o.loss, rows);
+        take(o.d2, (rows + 32) * o.ld2); take(o.g2, rows * o.ldu); take(o.g3, rows * o.ldu);
+        if (factor_chunks_most(a, rows) > factor_chunks_any(a)) {  // (else those of the bank are enough)
+            o.chunks = factor_chunks_most(a, rows);
+            take(o.chunk_slab, o.chunks * a->per_slot());
+        }
     }
     return at;
 }
 
-int ensure(Adapters* a, uint64_t rows, bool training, hipStream_t s)
+// Arrays that grow are at least doubled, and beyond half of the most rows become the largest at once: the earlier ones, which stay,
+// are together no larger than the last.
+uint64_t grown(uint64_t rows, uint64_t have)
 {
-    rows = std::min<uint64_t>(std::max<uint64_t>(rows, 256), kAdaptRows);
-    if (a->ws_rows >= rows && (a->ws_training || !training)) return SZH_OK;
-    if (capturing(s)) { set_error("adapters: the workspace must be reserved before a stream is captured (szh_adapters_reserve)"); return SZH_EINVAL; }
-    // (at least doubled when it grows: the old ones stay, and together they are no larger than the last)
-    if (rows > a->ws_rows) rows = std::max<uint64_t>(rows, std::min<uint64_t>(2 * a->ws_rows, kAdaptRows));
-    rows = std::max<uint64_t>(rows, a->ws_rows);
-    rows = (rows + 255) / 256 * 256;
-    training = training || a->ws_training;
+    rows = std::max<uint64_t>((rows + 255) / 256 * 256, 256);
+    if (have) rows = std::max<uint64_t>(rows, 2 * have);
+    return rows > kAdaptRows || (have && rows > kAdaptRows / 2) ? kAdaptRows : rows;
+}
+
+int add_part(Adapters* a, Part part, uint64_t rows)
+{
     char* p = nullptr;
-    const size_t bytes = lay_out(a, rows, training, nullptr, nullptr);
+    AdaptWorkspace w = a->ws;
+    const size_t bytes = lay_out(a, part, rows, nullptr, w);
     SZ_HIP(hipMalloc((void**)&p, bytes));
     try { a->arenas.push_back(p); } catch (...) { (void)hipFree(p); throw; }
     SZ_HIP(hipMemset(p, 0, bytes));  // the columns between a row's end and its stride are read as zeros
     SZ_HIP(hipDeviceSynchronize());
-    // the old workspace stays until the handle goes: a captured graph may still work in it
-    lay_out(a, rows, training, p, &a->ws);
-    a->ws_rows = rows;
-    a->ws_training = training;
+    // the old arrays stay until the handle goes: a captured graph may still work in them
+    lay_out(a, part, rows, p, a->ws);
+    a->ws_have[part] = rows;
+    return SZH_OK;
+}
+
+int ensure(Adapters* a, uint64_t rows, bool training, hipStream_t s)
+{
+    rows = std::min<uint64_t>(std::max<uint64_t>(rows, 1), kAdaptRows);
+    const uint64_t need[4] = {1, training ? 1u : 0u, rows, training ? rows : 0};
+    for (const Part part : {PART_BANK, PART_TRAIN_BANK, PART_ROWS, PART_TRAIN_ROWS}) {
+        if (a->ws_have[part] >= need[part]) continue;
+        if (capturing(s)) { set_error("adapters: the workspace must be reserved before a stream is captured (szh_adapters_reserve)"); return SZH_EINVAL; }
+        const bool by_row = part == PART_ROWS || part == PART_TRAIN_ROWS;
+        if (int rc = add_part(a, part, by_row ? grown(need[part], a->ws_have[part]) : 1)) return rc;
+    }
     return SZH_OK;
 }
 
@@ -253,20 +285,21 @@ int factor_gradients(Adapters* a, uint32_t rows, hipStream_t s)
     const int h1 = (int)a->h1, h2 = (int)a->h2, out = (int)a->out, r = (int)a->rank;
     FactorArgs g{};
     g.ldw = w.ldu; g.rank = r; g.slots = (int)a->slots; g.begin = w.begin; g.row_slot = w.row_slot; g.live = w.live;
-    g.job[0] = {w.h1, w.g2, nullptr, a->off_a2(), w.ld1, h1, r, 1, 0, 0};
-    g.job[1] = {w.d2, w.u2, nullptr, a->off_b2(), w.ld2, h2, 1, h2, 0, 0};
-    g.job[2] = {w.h2, w.g3, nullptr, a->off_a3(), w.ld2, h2, r, 1, 0, 0};
-    g.job[3] = {w.lg, w.u3, nullptr, a->off_b3(), w.ld3, out, 1, out, 0, 0};
+    g.job[0] = {w.h1, w.g2, nullptr, nullptr, a->off_a2(), w.ld1, h1, r, 1, 0, 0};
+    g.job[1] = {w.d2, w.u2, nullptr, nullptr, a->off_b2(), w.ld2, h2, 1, h2, 0, 0};
+    g.job[2] = {w.h2, w.g3, nullptr, nullptr, a->off_a3(), w.ld2, h2, r, 1, 0, 0};
+    g.job[3] = {w.lg, w.u3, nullptr, nullptr, a->off_b3(), w.ld3, out, 1, out, 0, 0};
     g.chunk = factor_chunk(a, rows);
     const uint64_t chunks = (rows + g.chunk - 1) / g.chunk;
-    if (chunks > factor_chunks_most(a, a->ws_rows)) { set_error("adapters: more chunks than the workspace holds"); return SZH_EINVAL; }
-    float* slab = w.slab;
+    if (chunks > w.chunks) { set_error("adapters: more chunks than the workspace holds"); return SZH_EINVAL; }
+    float *slot_slab = w.slot_slab, *chunk_slab = w.chunk_slab;
     int tiles = 0, blocks = 0;
     for (FactorJob& j : g.job) {
-        j.first = tiles; j.first_out = blocks; j.slab = slab;
+        j.first = tiles; j.first_out = blocks; j.slot_slab = slot_slab; j.chunk_slab = chunk_slab;
         tiles += (j.M + 63) / 64;
         blocks += (j.M * r + 255) / 256;
-        slab += (chunks + a->slots) * (uint64_t)j.M * r;
+        slot_slab += a->slots * (uint64_t)j.M * r;
+        chunk_slab += chunks * (uint64_t)j.M * r;
     }
     const dim3 grid(tiles, (unsigned)chunks), block(256);
     ProfScope prof("adapt_grad", s);

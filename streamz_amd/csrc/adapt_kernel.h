@@ -957,12 +957,13 @@ __global__ __launch_bounds__(64 * WAVES) void tail_kernel(BackArgs a, TailArgs o
 // The four factors' gradients are four contractions over rows, grad[slot][m][j] = sum over the slot's rows of
 // p[i][m] w[i][j], m up to a layer's width and j the rank columns; one launch does all four.  A row that does not count has
 // zeros for either operand, whatever its activations are (0 x inf would be a NaN in every element of the slot).
-// slab[chunk + slot][m][j] takes the part of a chunk of rows: rows are sorted by slot, so (chunk, slot) pairs that
-// hold rows lie on a staircase and chunk + slot numbers them without a table; factor_reduce_kernel adds a slot's chunks.
+// Rows are sorted by slot, so a chunk of rows holds the rest of one slot that begins in an earlier chunk, if of any, and slots that begin
+// in it: the part of the former goes to chunk_slab[chunk][m][j], those of the latter to slot_slab[slot][m][j], which needs no table and no
+// more room for the slots, however many rows there are.  factor_reduce_kernel adds a slot's chunks.
 struct FactorJob {
     const float* p;        // [rows][ldp], 16-byte aligned rows
     const float* w;        // [rows][ldw], the rank columns
-    float* slab;
+    float *slot_slab, *chunk_slab;
     uint64_t off;          // the factor's place in a slot's gradient: element (m, j) at off + m * g_m + j * g_j
     int ldp, M, g_m, g_j;
     int first;             // first tile of 64 columns of this job
@@ -1034,7 +1035,8 @@ __global__ __launch_bounds__(256) void factor_grad_kernel(FactorArgs a)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) part[wave][4 * (4 * q + i) + t][16 * n + c16] = acc[t][n][i];
         __syncthreads();
-        float* slab = g.slab + ((size_t)blockIdx.y + slot) * g.M * a.rank;
+        const bool begins = a.begin[slot] >= blockIdx.y * a.chunk;
+        float* slab = (begins ? g.slot_slab + (size_t)slot * g.M * a.rank : g.chunk_slab + (size_t)blockIdx.y * g.M * a.rank);
         for (int e = threadIdx.x; e < 64 * a.rank; e += 256) {
             const int m = e / a.rank, j = e % a.rank;
             if (m0 + m < g.M)
@@ -1085,7 +1087,8 @@ __global__ __launch_bounds__(256) void factor_reduce_kernel(FactorArgs a, float*
     const int which = ((int)blockIdx.x >= a.job[1].first_out) + ((int)blockIdx.x >= a.job[2].first_out) + ((int)blockIdx.x >= a.job[3].first_out);
     const FactorJob g = a.job[which];
     const int i = ((int)blockIdx.x - g.first_out) * 256 + threadIdx.x;
-    if (i >= g.M * a.rank) return;
+    const int size = g.M * a.rank;
+    if (i >= size) return;
     const uint32_t c0 = b / a.chunk, c1 = (e - 1) / a.chunk;
     float* out = grad + (size_t)slot * grad_slot + g.off + (size_t)(i / a.rank) * g.g_m + (size_t)(i % a.rank) * g.g_j;
     const float before = *out;
@@ -1093,7 +1096,10 @@ __global__ __launch_bounds__(256) void factor_reduce_kernel(FactorArgs a, float*
     for (uint32_t c = c0; c <= c1; c += 8) {
         float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = g.slab[(size_t)(min(c + k, c1) + slot) * g.M * a.rank + i];
+        for (int k = 0; k < 8; ++k) {
+            const float* at = c + k == c0 ? g.slot_slab + (size_t)slot * size : g.chunk_slab + (size_t)min(c + k, c1) * size;
+            v[k] = at[i];
+        }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < 8; ++k) t += (double)keep_if(c + k <= c1, v[k]);

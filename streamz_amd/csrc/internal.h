@@ -302,11 +302,20 @@ int control_run(const Controls& ctl, const ControlRun& a, hipStream_t s);
 // ---- low-rank adapters (adapt.hip) ---------------------------------------------------------
 struct AdaptWorkspace {
     int ldx = 0, ld1 = 0, ld2 = 0, ld3 = 0, ldu = 0;  // row strides
-    uint32_t *order = nullptr, *begin = nullptr, *count = nullptr, *total = nullptr, *w2s = nullptr;
+    // of the bank, whatever the call
+    uint32_t *begin = nullptr, *total = nullptr, *w2s = nullptr;
+    float *w2t = nullptr, *w3t = nullptr, *add2 = nullptr, *add3 = nullptr;
+    float* slot_slab = nullptr;   // training: partial gradients, one of every slot
+    // by row
+    uint32_t *order = nullptr, *count = nullptr;
     int32_t* row_slot = nullptr;
-    float *xs = nullptr, *h1 = nullptr, *h2 = nullptr, *lg = nullptr, *u2 = nullptr, *u3 = nullptr, *w2t = nullptr,
-          *w3t = nullptr, *add2 = nullptr, *add3 = nullptr, *d2 = nullptr, *g2 = nullptr, *g3 = nullptr, *loss = nullptr, *slab = nullptr;
-    uint8_t *live0 = nullptr, *live = nullptr;
+    float *xs = nullptr, *h1 = nullptr, *h2 = nullptr, *lg = nullptr, *u2 = nullptr, *u3 = nullptr;
+    uint8_t* live0 = nullptr;
+    // by row, training
+    float *d2 = nullptr, *g2 = nullptr, *g3 = nullptr, *loss = nullptr;
+    float* chunk_slab = nullptr;  // partial gradients, one of every chunk of rows
+    uint64_t chunks = 0;
+    uint8_t* live = nullptr;
 };
 struct Adapters {
     uint32_t in = 0, h1 = 0, h2 = 0, out = 0, slots = 0, rank = 0;
@@ -317,9 +326,8 @@ struct Adapters {
     double* d_sums = nullptr;   // [slots]{loss, live rows} since zero_grad
     Clip* clip = nullptr;
     AdaptWorkspace ws;
-    uint64_t ws_rows = 0;
-    bool ws_training = false;
-    std::vector<char*> arenas;  // the last one holds ws; earlier ones stay for graphs captured in them
+    uint64_t ws_have[4] = {};   // the rows that each part of it is large enough for
+    std::vector<char*> arenas;  // earlier arrays stay for graphs captured in them
 
     uint64_t off_a2() const { return 0; }
     uint64_t off_b2() const { return (uint64_t)h1 * rank; }

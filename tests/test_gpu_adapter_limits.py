@@ -193,3 +193,66 @@ def test_gradients_of_just_fewer_rows_than_a_whole_step_of_chunks(dims, rank, n)
     want, want_stats = tr.train(params, flat, known(slots, s), 0.7, x, labels, rank, dims)
     tr.check(stats, want_stats, "loss and live rows")
     tr.check(g, want, "gradient")
+
+
+@pytest.mark.parametrize("dims,slots,rank,steps", [((60, 512, 256, 16), 2000, 16, (256, 700, 1300, 2100, 4000, 8192)),
+                                                   ((60, 512, 256, 16), 3, 8, (300, 9000, 40000, 70000, 131072)),
+                                                   ((60, 1024, 512, 100), 300, 32, (10, 500, 513, 3000, 6000))])
+def test_a_training_workspace_that_grows_stays_in_proportion(dims, slots, rank, steps):
+    """What a bank keeps after growing step by step, forward and training in turn, is at most twice what one that is reserved for the last
+    step at once takes: the arrays of earlier steps together are no larger than the last ones, and what does not grow with the rows is there once."""
+    import torch
+    net = sz.SimpleNeuralNet(*dims, seed=1)
+    banks = [sz.Adapters(net, slots, rank) for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def taken(call):
+        before = torch.cuda.mem_get_info()[0]
+        call()
+        torch.cuda.synchronize()
+        return before - torch.cuda.mem_get_info()[0]
+
+    def grow():
+        for n in steps:
+            banks[1].reserve(n)
+            banks[1].reserve(n, training=True)
+
+    once, grown = taken(lambda: banks[0].reserve(steps[-1], training=True)), taken(grow)
+    # (each allocation is rounded up to 2 MiB: two for the rows of every step and four for the rest)
+    assert once > 0 and grown <= 2 * once + (2 * len(steps) + 4) * (2 << 20)
+
+
+def test_a_graph_keeps_its_arrays_while_the_workspace_grows():
+    """Captured with the arrays of a small bank, replayed after larger calls have brought larger ones and worked in both."""
+    import torch
+    from helpers import _DevView
+    dims, slots, rank, n = (60, 64, 64, 16), 5, 16, 300
+    rng = np.random.default_rng(31)
+    params, flat, x = make(rng, dims, slots, rank, 40000)
+    s, labels = pick_slots(rng, 40000, slots, "mixed"), rng.integers(0, 16, 40000).astype(np.int32)
+    net = sz.SimpleNeuralNet(*dims, init=params)
+    bank = sz.Adapters(net, slots, rank, scale=0.7, init=flat)
+    want = grads(net, bank, x[:n], labels[:n], s[:n])
+    dx, ds, dl = dev(x), dev(s), dev(labels)
+    probs = torch.zeros(n, 16, device="cuda")
+    net.forward_adapted_dev(bank, dx.data_ptr(), ds.data_ptr(), n, probs_ptr=probs.data_ptr())
+    torch.cuda.synchronize()
+    want_probs = probs.clone()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        st = torch.cuda.current_stream().cuda_stream
+        bank.zero_grad_dev(st)
+        bank.accumulate_dev(net, dx.data_ptr(), dl.data_ptr(), ds.data_ptr(), n, stream=st)
+        net.forward_adapted_dev(bank, dx.data_ptr(), ds.data_ptr(), n, probs_ptr=probs.data_ptr(), stream=st)
+    P = bank.param_count()
+    for more in (700, 5000, 40000):
+        forward(net, bank, x[:more], s[:more])
+        big = grads(net, bank, x[:more], labels[:more], s[:more])
+        probs.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        g = torch.as_tensor(_DevView(bank.grad_ptr(), bank.grad_len()), device="cuda").cpu().numpy()
+        assert np.array_equal(g[:slots * P].reshape(slots, P), want[0]) and np.array_equal(g[slots * P:].reshape(slots, 2), want[1])
+        assert torch.equal(probs, want_probs)
+        again = grads(net, bank, x[:more], labels[:more], s[:more])
+        assert np.array_equal(big[0], again[0])
