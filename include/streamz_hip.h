@@ -298,7 +298,8 @@ int szh_net_clip_grad_dev(szh_net *net, float max_norm, float *norm_dev, void *s
  * its scaled values go to out[t] (out == NULL, or out[t] == in[t]: in place; otherwise the two must not overlap).
  * group[t] < groups (group == NULL: all in group 0).  live_dev (optional): groups floats that the norms are divided by,
  * read when the call runs; a group whose value is not > 0 has norm 0.  The handle keeps the addresses: the tensors must
- * outlive it.  norms_dev (optional) receives `groups` floats.  Addresses are multiples of 4 bytes.
+ * outlive it.  norms_dev (optional) receives `groups` floats.  Addresses are multiples of 4 bytes.  A handle takes fewer than 2^24 - 1 tensors
+ * (every 2^24 values of a longer one, and up to three at the head of one that is not 16-byte aligned, count as one more).
  * Calls on one handle share its workspace: they must not overlap (two streams, two graphs in flight). */
 typedef struct szh_clip szh_clip;
 int szh_clip_create(const float *const *in, float *const *out, const uint64_t *lengths, const uint32_t *group, uint32_t n_tensors,

@@ -36,6 +36,7 @@ __device__ __forceinline__ double block_sum(double v)
 // A thread's four 16-byte pieces of a round of the workgroup's 4096 values: at + 1024 j.  Pieces are cut so that
 // those of a tensor are 16-byte aligned where both its addresses can be (ClipPiece::vec).
 constexpr uint32_t kClipRound = 16 * kClipThreads;
+constexpr uint64_t kClipMostPieces = (1ull << 32) / kClipThreads - 1;  // (a launch has fewer than 2^32 threads)
 
 // a store that leaves the caches to the gradients still to be read again (38.8 M of them: 97 -> 80 us)
 typedef float vec4 __attribute__((ext_vector_type(4)));
@@ -154,6 +155,7 @@ int clip_create(const ClipTensor* tensors, uint32_t n, uint32_t groups, const fl
         // a first piece of up to three values, if that makes both addresses behind it multiples of 16 bytes
         const uint64_t skew = ((uintptr_t)t.src & 15) / sizeof(float);
         const bool vec = ((uintptr_t)t.src & 15) == ((uintptr_t)t.dst & 15);
+        if (pieces.size() + t.len / piece + 2 > kClipMostPieces) { set_error("too many tensors, or too long ones"); return SZH_EINVAL; }
         uint64_t at = 0;
         if (vec && skew && t.len > 64) {
             at = 4 - skew;
@@ -165,7 +167,6 @@ int clip_create(const ClipTensor* tensors, uint32_t n, uint32_t groups, const fl
         }
     }
     while (g < groups) first[++g] = (uint32_t)pieces.size();
-    if (pieces.size() > 0x7fffffffu) { set_error("too many tensors"); return SZH_EINVAL; }
     Clip* c = new (std::nothrow) Clip();
     if (!c) { set_error("out of host memory"); return SZH_ENOMEM; }
     c->n_pieces = (uint32_t)pieces.size();
