@@ -256,3 +256,152 @@ def test_a_graph_keeps_its_arrays_while_the_workspace_grows():
         assert torch.equal(probs, want_probs)
         again = grads(net, bank, x[:more], labels[:more], s[:more])
         assert np.array_equal(big[0], again[0])
+
+
+# 1024 classes and fewer: lanes of a wave a row; then a workgroup a row with 2, 4, 8, 16, 32 or 50 values a thread, then none kept
+CLASSES = [1023, 1024, 1025, 2048, 2049, 4096, 4097, 8192, 8193, 16384, 16385, 32768, 32769, 51200, 51201]
+
+
+@pytest.mark.parametrize("classes", CLASSES)
+def test_controls_of_many_classes(classes):
+    import torch
+    rows, sets = 7, 3
+    rng = np.random.default_rng(classes)
+    z = (3 * rng.standard_normal((rows, classes))).astype(np.float32)
+    c = host_controls(rng, sets, classes, rows)
+    c["counts"] = np.maximum(rng.integers(-5, 4, (sets, classes)), 0).astype(np.uint32)
+    c["repetition"] = rng.uniform(0.6, 1.7, sets).astype(np.float32)
+    c["presence"] = rng.uniform(-1, 1, sets).astype(np.float32)
+    c["frequency"] = rng.uniform(-0.2, 0.2, sets).astype(np.float32)
+    handle, keep = dev_controls(c)
+    want_z, want_p = tr.control(tr.T(z), c, classes)
+    for probs, want in ((True, want_p), (False, want_z)):
+        d = dev(z)
+        out = torch.full((rows + 1, classes), 7.0, device="cuda")
+        sz.control_logits_dev(d.data_ptr(), rows, classes, handle, out.data_ptr(), probs=probs)
+        sz.control_logits_dev(d.data_ptr(), rows, classes, handle, d.data_ptr(), probs=probs)
+        torch.cuda.synchronize()
+        tr.check(out[:rows].cpu().numpy(), want, "probabilities" if probs else "logits")
+        assert torch.equal(d, out[:rows]) and (out[rows] == 7).all()
+
+
+@pytest.mark.parametrize("classes", CLASSES)
+def test_gradients_of_many_classes(classes):
+    """Candidate lists, priors, labels that are missing, do not exist or are off the list."""
+    dims, slots, rank, n = (60, 16, 8, classes), 3, 2, 261
+    rng = np.random.default_rng(classes + 1)
+    params, flat, x = make(rng, dims, slots, rank, n)
+    s = pick_slots(rng, n, slots, "mixed")
+    labels = rng.integers(0, classes, n).astype(np.int32)
+    labels[::17], labels[5::17], labels[9::17], labels[12::17] = -1, classes, 0, classes - 1
+    net = sz.SimpleNeuralNet(*dims, init=params)
+    bank = sz.Adapters(net, slots, rank, scale=0.7, init=flat)
+    c = host_controls(rng, 4, classes, n)
+    handle, keep = dev_controls(c)
+    g, stats = grads(net, bank, x, labels, s, handle)
+    want, want_stats = tr.train(params, flat, known(slots, s), 0.7, x, labels, rank, dims, c)
+    tr.check(stats, want_stats, "loss and live rows")
+    tr.check(g, want, "gradient")
+    assert want_stats.v[:, 1].min() > 0
+    again, stats2 = grads(net, bank, x, labels, s, handle)
+    assert np.array_equal(g, again) and np.array_equal(stats, stats2)
+
+
+@pytest.mark.parametrize("classes", CLASSES)
+def test_votes_of_many_classes(classes):
+    """The last of the largest, also where equal ones lie in other lanes, waves and steps of a thread."""
+    import torch
+    dims, slots, rank, n, groups, thr = (60, 16, 8, classes), 2, 2, 530, 3, 1e-7
+    rng = np.random.default_rng(classes + 2)
+    params, flat, x = make(rng, dims, slots, rank, n)
+    # several classes with the same weights, which no other class can beat
+    equal = np.unique(np.concatenate([rng.integers(0, classes, 5), [classes // 2, classes - 1 - classes // 3]]))
+    params[4][:, equal] = params[4][:, equal[:1]]
+    params[5][equal] = 30.0
+    factors = flat.reshape(slots, -1)
+    b3 = factors[:, rank * (16 + 2 * 8):].reshape(slots, rank, classes)
+    b3[:, :, equal] = b3[:, :, equal[:1]]
+    s, group = pick_slots(rng, n, slots, "mixed"), rng.integers(-1, groups + 1, n).astype(np.int32)
+    net = sz.SimpleNeuralNet(*dims, init=params)
+    bank = sz.Adapters(net, slots, rank, init=factors)
+    c = {"sets": 3, "set_of_row": rng.integers(0, 3, n).astype(np.int32), "allow": np.full((3, (classes + 31) // 32), 0xffffffff, np.uint32)}
+    last = equal[-1]
+    c["allow"][1, last // 32] &= ~np.uint32(1 << (last % 32))   # the last of them is no candidate
+    c["allow"][2] = 0
+    handle, keep = dev_controls(c)
+    dx, ds, dg = dev(x), dev(s), dev(group)
+    counts = torch.ones(groups, classes, dtype=torch.int64, device="cuda")
+    net.vote_adapted_dev(bank, dx.data_ptr(), ds.data_ptr(), n, thr, counts.data_ptr(), groups=groups, group_of_row_ptr=dg.data_ptr(), controls=handle)
+    torch.cuda.synchronize()
+    want = np.ones((groups, classes), np.int64)
+    for i in range(n):
+        if 0 <= group[i] < groups and c["set_of_row"][i] < 2:
+            want[group[i], equal[-1 - c["set_of_row"][i]]] += 1
+    assert np.array_equal(counts.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dims,rank,n", [((60, 256, 512, 16), 16, 1100), ((60, 512, 256, 100), 24, 1500), ((60, 256, 256, 20), 40, 1024)])
+def test_gradients_in_split_bf16(dims, rank, n, monkeypatch):
+    slots = 3
+    rng = np.random.default_rng(sum(dims))
+    params, flat, x = make(rng, dims, slots, rank, n)
+    s, labels = pick_slots(rng, n, slots, "mixed"), rng.integers(-1, dims[3], n).astype(np.int32)
+    net = sz.SimpleNeuralNet(*dims, init=params)
+    net.set_gemm("bf16x3")
+    bank = sz.Adapters(net, slots, rank, scale=0.7, init=flat)
+    g, stats = grads(net, bank, x, labels, s)
+    # products below 2^-24 of a term are dropped, one more rounding a product: every bound is linear in the rounding unit
+    monkeypatch.setattr(tr, "U", 2 * tr.U)
+    want, want_stats = tr.train(params, flat, known(slots, s), 0.7, x, labels, rank, dims)
+    tr.check(stats, want_stats, "loss and live rows")
+    tr.check(g, want, "gradient")
+    again, _ = grads(net, bank, x, labels, s)
+    assert np.array_equal(g, again)
+
+
+@pytest.mark.parametrize("dims,rank", [((60, 512, 256, 16), 16), ((60, 40, 24, 70), 20), ((65, 64, 300, 300), 5)])
+@pytest.mark.parametrize("n", [3, 600])
+@pytest.mark.parametrize("at", [0, 31, -1])
+def test_an_undefined_feature_leaves_no_hidden_unit(dims, rank, n, at):
+    """v > 0 ? v : 0 of a NaN is 0 (lib.rs:882), in every kernel: the row's logits are those of hidden units of 0."""
+    slots = 2
+    rng = np.random.default_rng(sum(dims) + n)
+    params, flat, x = make(rng, dims, slots, rank, n)
+    x[:, at] = np.nan
+    s = (np.arange(n) % 3 - 1).astype(np.int32)
+    net = sz.SimpleNeuralNet(*dims, init=params)
+    bank = sz.Adapters(net, slots, rank, scale=0.7, init=flat)
+    logits, _ = forward(net, bank, x, s)
+    none = [np.zeros_like(p) for p in params[:2]] + params[2:]
+    tr.check(logits, tr.layers(none, flat, known(slots, s), 0.7, np.zeros_like(x), rank, dims)[4], "logits")
+
+
+@pytest.mark.parametrize("n", [60, 900])
+def test_votes_in_a_graph(n):
+    """Counts go on from replay to replay, beside eager calls of the same bank."""
+    import torch
+    dims, slots, rank, groups = (60, 64, 32, 8), 4, 3, 5
+    rng = np.random.default_rng(n)
+    params, flat, x = make(rng, dims, slots, rank, n)
+    net = sz.SimpleNeuralNet(*dims, init=params)
+    bank = sz.Adapters(net, slots, rank, init=flat)
+    bank.reserve(n)
+    dx, ds, dg = dev(x), dev(pick_slots(rng, n, slots, "mixed")), dev(rng.integers(-1, groups + 1, n).astype(np.int32))
+    counts, eager = (torch.zeros(groups, 8, dtype=torch.int64, device="cuda") for _ in range(2))
+
+    def work(out, stream):
+        net.vote_adapted_dev(bank, dx.data_ptr(), ds.data_ptr(), n, 0.15, out.data_ptr(), groups=groups, group_of_row_ptr=dg.data_ptr(), stream=stream)
+
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        work(counts, torch.cuda.current_stream().cuda_stream)
+    for k in range(4):
+        dx.copy_(torch.from_numpy(rng.standard_normal(x.shape).astype(np.float32)))
+        ds.copy_(torch.from_numpy(pick_slots(rng, n, slots, "mixed")))
+        torch.cuda.synchronize()
+        work(eager, 0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(counts, eager) and int(counts.sum()) > 0
