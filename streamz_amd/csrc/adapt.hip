@@ -128,30 +128,31 @@ uint64_t grown(uint64_t rows, uint64_t have)
     return rows > kAdaptRows || (have && rows > kAdaptRows / 2) ? kAdaptRows : rows;
 }
 
-int add_part(Adapters* a, Part part, uint64_t rows)
-{
-    char* p = nullptr;
-    AdaptWorkspace w = a->ws;
-    const size_t bytes = lay_out(a, part, rows, nullptr, w);
-    SZ_HIP(hipMalloc((void**)&p, bytes));
-    try { a->arenas.push_back(p); } catch (...) { (void)hipFree(p); throw; }
-    SZ_HIP(hipMemset(p, 0, bytes));  // the columns between a row's end and its stride are read as zeros
-    SZ_HIP(hipDeviceSynchronize());
-    // the old arrays stay until the handle goes: a captured graph may still work in them
-    lay_out(a, part, rows, p, a->ws);
-    a->ws_have[part] = rows;
-    return SZH_OK;
-}
-
 int ensure(Adapters* a, uint64_t rows, bool training, hipStream_t s)
 {
     rows = std::min<uint64_t>(std::max<uint64_t>(rows, 1), kAdaptRows);
-    const uint64_t need[4] = {1, training ? 1u : 0u, rows, training ? rows : 0};
-    for (const Part part : {PART_BANK, PART_TRAIN_BANK, PART_ROWS, PART_TRAIN_ROWS}) {
-        if (a->ws_have[part] >= need[part]) continue;
-        if (capturing(s)) { set_error("adapters: the workspace must be reserved before a stream is captured (szh_adapters_reserve)"); return SZH_EINVAL; }
-        const bool by_row = part == PART_ROWS || part == PART_TRAIN_ROWS;
-        if (int rc = add_part(a, part, by_row ? grown(need[part], a->ws_have[part]) : 1)) return rc;
+    const Part parts[] = {PART_BANK, PART_TRAIN_BANK, PART_ROWS, PART_TRAIN_ROWS};
+    const uint64_t need[] = {1, training ? 1u : 0u, rows, training ? rows : 0};
+    AdaptWorkspace w = a->ws;
+    uint64_t get[4] = {};
+    size_t bytes = 0;
+    for (const Part p : parts) {
+        if (a->ws_have[p] >= need[p]) continue;
+        get[p] = p == PART_ROWS || p == PART_TRAIN_ROWS ? grown(need[p], a->ws_have[p]) : 1;
+        bytes += lay_out(a, p, get[p], nullptr, w);
+    }
+    if (bytes == 0) return SZH_OK;
+    if (capturing(s)) { set_error("adapters: the workspace must be reserved before a stream is captured (szh_adapters_reserve)"); return SZH_EINVAL; }
+    char* at = nullptr;
+    SZ_HIP(hipMalloc((void**)&at, bytes));
+    try { a->arenas.push_back(at); } catch (...) { (void)hipFree(at); throw; }
+    SZ_HIP(hipMemset(at, 0, bytes));  // the columns between a row's end and its stride are read as zeros
+    SZ_HIP(hipDeviceSynchronize());
+    // the old arrays stay until the handle goes: a captured graph may still work in them
+    for (const Part p : parts) {
+        if (!get[p]) continue;
+        at += lay_out(a, p, get[p], at, a->ws);
+        a->ws_have[p] = get[p];
     }
     return SZH_OK;
 }
