@@ -424,6 +424,8 @@ int thin_product(const float* A, int lda, int K, const float* W, const float* ad
 //   256-row tiles: 0.232 K + 18 for every round of one tile per compute unit
 //   128-row tiles: two per unit 0.122 K + 17, one 0.071 K + 12        64-row tiles: 0.0337 K + 4 each, once 0.0085 K
 //   32 x 32 thin tiles: 5 + 0.001 K, and 3.55e-5 K each
+// These are of the product alone: the rank columns added behind it are in no term.  With rank 16 the 145 us above are 180 (172 and 8); at
+// 13228 x 2048 x 2048 with rank 32 the round of 256-row tiles takes 587 instead of 499, the 64-row tiles beside it 416 instead of 382.
 struct ProductPart { int how; uint32_t rows; };   // how: 256, 128 or 64 rows a tile, 0 thin
 struct ProductPlan { ProductPart part[3]; int parts; double time; };
 
